@@ -508,6 +508,78 @@ int slx_dec_attn_ws_floats(int Hq, int Hkv, int lmax);
 int slx_dec_attn(void* cache, int64_t ld, int Hq, int Hkv, const float* cos_tab, const float* sin_tab, int lmax,
                  float* ws, void* out, const slx_dec_state* st, slx_stream_t s);
 
+/* ---- paged key/value cache: decoding many sequences that share a prompt (csrc/paged.hip) --------------------------
+ * Beside the one-sequence greedy decode above (llm.py:178-250 re-runs the prefix for every token and sample): the
+ * questions / instructions about one camera frame and the beams of one answer share the image prompt's keys.
+ * A pool is a pair of bf16 arrays [n_pages][page][heads][head_dim] with the element strides given (both alike, d
+ * contiguous, multiples of 8; 16-B aligned). A table row names the pages of one sequence in order: key j is slot
+ * j % page of page table[seq][j / page]. page: a power of two (1 = a table of single slots). head_dim 64 or 128.
+ * Tables, positions and lengths are read on the device: lengths are cut to the bounds given, keys on a page outside
+ * [0, n_pages) are masked, rows that name no slot are left out.                                                      */
+typedef struct slx_kv_pool {
+  void* k; void* v;
+  int64_t page_stride, slot_stride, head_stride;
+  int n_pages, page, heads, head_dim;
+} slx_kv_pool;
+typedef struct slx_kv_append_desc {
+  slx_kv_pool pool;
+  const void* qkv; int64_t ldqkv;            /* bf16 rows q (Hq heads) | k | v (pool.heads each)                       */
+  void* q_out; int64_t ldq;                  /* rotated q rows [rows][Hq * head_dim]; may be qkv itself; NULL: q is not read */
+  const int* table; int64_t ldt; int n_seq, cols;
+  const int* seq;                            /* [rows] sequence of each row; NULL: row / rows_per_seq                  */
+  const int* pos;                            /* [rows] position in the sequence; < 0: padding, nothing is written      */
+  int rows_per_seq, Hq;
+  int64_t rows;
+  const float* cos_tab; const float* sin_tab; int rope_rows; /* f32 [rope_rows][head_dim / 2]; NULL: no rotation; a
+                                                position >= rope_rows counts as padding                               */
+} slx_kv_append_desc;
+/* rotate_half RoPE of q and k (f32, rounded once), k and v into their slots, in one pass. Two rows of one call must not
+ * name the same slot.                                                                                                */
+int slx_kv_append(const slx_kv_append_desc* d, slx_stream_t s);
+typedef struct slx_prefix_attn_desc {
+  slx_kv_pool prefix_pool, own_pool;
+  const void* q; int64_t ldq;                /* bf16 rows [groups * width * n_q][Hq * head_dim], a sequence's n_q tokens together */
+  void* out; int64_t ldo;                    /* bf16 [rows][Hq * head_dim]                                             */
+  float* lse;                                /* optional f32 [rows][Hq]: natural log of the softmax sum (-inf: no key) */
+  const int* ptab; int64_t ldpt; const int* plen;  /* [groups] prefixes; ptab NULL: none                               */
+  const int* otab; int64_t ldot; const int* olen;  /* [groups * width] own keys, the n_q new tokens' last among them   */
+  int max_prefix, max_own;                   /* bounds of plen and olen (longer ones are cut to them)                  */
+  int pcols, ocols;                          /* table columns                                                          */
+  int groups, width, n_q, Hq;
+  float scale;
+  float* ws; int64_t ws_floats;              /* slx_prefix_attn_ws_floats(d); one call at a time                       */
+} slx_prefix_attn_desc;
+/* token t of a sequence's n_q attends the plen[group] keys of its group's prefix and its own keys j <= olen - n_q + t; a
+ * row without any key gives zeros.                                                                                   */
+int slx_prefix_attn(const slx_prefix_attn_desc* d, slx_stream_t s);
+int64_t slx_prefix_attn_ws_floats(const slx_prefix_attn_desc* d); /* < 0: bad argument                                 */
+
+/* ---- beam search (csrc/beam.hip) ----------------------------------------------------------------------------------
+ * Beside the greedy choice of llm.py:145-160. score(b, w, t) = score[b][w] + x[b, w, t] - log sum_t' e^x[b, w, t'];
+ * the k best of a batch entry's width * vocab scores in descending order, ties to the lowest w * vocab + t. A row that
+ * has finished offers one continuation, `pad`, with its score unchanged. A score that is not a number (a row of -inf, a
+ * row with a NaN or +inf logit) counts as -inf. score_out and finished_out may be score and finished when k == width. */
+typedef struct slx_beam_select_desc {
+  const void* logits; int64_t ldx; int logits_bf16;  /* [batch * width][vocab] f32 or bf16, any alignment of the type  */
+  int batch, width, vocab, k;                /* width, k <= 64; vocab <= 262144                                        */
+  const float* score;                        /* [batch * width]; -inf: the beam is out                                 */
+  const unsigned char* finished; int pad;    /* optional [batch * width]                                               */
+  float* score_out; int* parent; int* token; /* [batch][k]                                                             */
+  unsigned char* finished_out; int eos;      /* optional [batch][k]: finished[parent] or token == eos                  */
+  void* ws; int64_t ws_bytes;                /* slx_beam_select_ws_bytes(d); one call at a time                        */
+} slx_beam_select_desc;
+int slx_beam_select(const slx_beam_select_desc* d, slx_stream_t s);
+int64_t slx_beam_select_ws_bytes(const slx_beam_select_desc* d); /* < 0: bad argument                                  */
+/* dst[i0][i1][b * width + w] = src[i0][i1][b * width + parent[b][w]], rows of row_bytes; strides in bytes. dst is src (in
+ * place, equal strides) or does not overlap it. A parent outside [0, width) leaves its row (in place) or copies row w. */
+typedef struct slx_beam_reorder_desc {
+  const void* src; void* dst;
+  int64_t s0, s1, src_row, d0, d1, dst_row, row_bytes;
+  int n0, n1, batch, width;                  /* width <= 64                                                            */
+  const int* parent;                         /* [batch][width]                                                         */
+} slx_beam_reorder_desc;
+int slx_beam_reorder(const slx_beam_reorder_desc* d, slx_stream_t s);
+
 /* ---- collate image path: uint8 frames -> InternVL2 pixel tiles (csrc/frames.hip) --------
  * Replaces preprocess_image_batch (simlingo_training/utils/internvl2_utils.py:179-203) per batch: the bottom crop
  * (dataloader/dataset_base.py:464-467) is a row count, dynamic_preprocess (internvl2_utils.py:231-266) picks the

@@ -1,0 +1,400 @@
+// Beam search on the device: the choice of the k best continuations over all beams and the whole vocabulary, and the
+// reordering of any state by the beams chosen. They stand beside the greedy choice (simlingo_training/models/
+// language_model/llm.py:145-160 argmax; decode.hip folds it into the LM head).
+//
+// score(b, w, t) = s[b, w] + x[b, w, t] - log sum_t' e^{x[b, w, t']}; the k largest of a batch entry's width * V
+// scores, ties to the lowest w * V + t. One pass over the logits: within a row the order of the scores is the order of
+// the logits, so every 4096-column chunk hands on its k largest logits and its (max, sum) of the softmax, and the
+// second launch forms the row sums, the scores (64 bits, from exact 32-bit maxima and sums of at most 4096 terms each)
+// and the k best of all rows.
+#include "common.h"
+#include "../../include/slx.h"
+
+namespace slx {
+
+typedef unsigned long long u64;
+typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+constexpr int kSelE = 16;                // logits a thread
+constexpr int kSelChunk = 256 * kSelE;   // columns a workgroup
+constexpr int kSelMaxChunks = 64;        // one lane each in the second launch
+constexpr int kSelMaxK = 64, kSelMaxW = 64;
+constexpr int kSelList = 256;            // candidates of a chunk that are ranked at once
+
+struct SelArgs {
+  const void* x; long ldx;
+  const float* score; const unsigned char* fin;
+  float* score_out; int *parent, *token; unsigned char* fin_out;
+  int B, W, V, K, C, pad, eos;
+  float2* ml;  // [B * W][C] (max, sum)
+  u64* keys;   // [B * W][C][K], descending; 0 = none
+};
+
+// order-preserving bits of a float; NaN below everything (its row's sum is NaN, so the row offers nothing)
+__device__ __forceinline__ unsigned ord_f(float v) {
+  const unsigned u = __float_as_uint(v);
+  return v != v ? 0u : (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+}
+__device__ __forceinline__ float unord_f(unsigned u) {
+  return __uint_as_float((u & 0x80000000u) ? (u & 0x7FFFFFFFu) : ~u);
+}
+__device__ __forceinline__ u64 key_of(unsigned ord, int idx) { return ((u64)ord << 32) | (0xFFFFFFFFu - (unsigned)idx); }
+__device__ __forceinline__ int key_idx(u64 k) { return (int)(0xFFFFFFFFu - (unsigned)k); }
+
+// the largest of a value over the wave: DPP within rows of 16 lanes, then the 4 rows' results
+template <int CTRL>
+__device__ __forceinline__ unsigned dpp_u(unsigned v) {
+  return (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xF, 0xF, false);
+}
+__device__ __forceinline__ unsigned wave_umax(unsigned x) {
+  x = max(x, dpp_u<0xB1>(x));   // quad_perm [1,0,3,2]
+  x = max(x, dpp_u<0x4E>(x));   // quad_perm [2,3,0,1]
+  x = max(x, dpp_u<0x141>(x));  // row_half_mirror
+  x = max(x, dpp_u<0x140>(x));  // row_mirror
+  const unsigned a = (unsigned)__builtin_amdgcn_readlane((int)x, 0), b = (unsigned)__builtin_amdgcn_readlane((int)x, 16);
+  const unsigned c = (unsigned)__builtin_amdgcn_readlane((int)x, 32), d = (unsigned)__builtin_amdgcn_readlane((int)x, 48);
+  return max(max(a, b), max(c, d));
+}
+// the largest key over the wave (uniform): high words first, then the low words of the lanes that hold that high word
+__device__ __forceinline__ u64 wave_kmax(u64 k) {
+  const unsigned hi = wave_umax((unsigned)(k >> 32));
+  const unsigned lo = wave_umax((unsigned)(k >> 32) == hi ? (unsigned)k : 0u);
+  return ((u64)hi << 32) | lo;
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void beam_chunk_kernel(SelArgs a) {
+  __shared__ float2 sml[4];
+  __shared__ unsigned stv[4];
+  __shared__ int scount;
+  __shared__ u64 list[kSelList];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int c = blockIdx.x, row = blockIdx.y;
+  // rows that have ended, or are out of the search already, are not read
+  const float s = a.score[row];
+  if ((a.fin && a.fin[row]) || s == -INFINITY || s != s) return;
+  constexpr int VEC = 16 / (int)sizeof(T), U = kSelE / VEC;  // 16-B loads, VEC columns each
+  const T* xr = (const T*)a.x + (long)row * a.ldx;
+  const int c0 = c * kSelChunk;
+  auto col = [&](int e) { return c0 + ((e / VEC) * 256 + tid) * VEC + e % VEC; };
+  float v[kSelE];
+  int n = kSelE;  // this thread's columns (a prefix of its order in a full chunk; all or by column in the last)
+  if (c0 + kSelChunk <= a.V) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      T t[VEC];
+      __builtin_memcpy(t, xr + c0 + (u * 256 + tid) * VEC, 16);  // rows of odd length: any alignment of T
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) v[u * VEC + j] = (float)t[j] + 0.f;  // -0 ties with 0
+    }
+  } else {
+    n = 0;
+#pragma unroll
+    for (int e = 0; e < kSelE; ++e) {
+      const bool in = col(e) < a.V;
+      v[e] = in ? (float)xr[col(e)] + 0.f : -INFINITY;
+      n += in;
+    }
+  }
+  // ordered bits, 0 for what is not there; columns past V have no key
+  unsigned o[kSelE], om = 0;
+  float m = -INFINITY;
+#pragma unroll
+  for (int e = 0; e < kSelE; ++e) {
+    o[e] = ord_f(v[e]);
+    m = fmaxf(m, v[e]);
+  }
+  // a thread's columns below V come first in its order, so its n first are the ones that count
+#pragma unroll
+  for (int e = 0; e < kSelE; ++e) om = e < n ? max(om, o[e]) : om;
+  const unsigned top = wave_umax(n ? om : 0u);
+  const float mw = unord_f(wave_umax(ord_f(m)));
+  const float ms = mw == -INFINITY ? 0.f : mw;
+  float l = 0.f;
+#pragma unroll
+  for (int e = 0; e < kSelE; ++e) l += __expf(v[e] - ms);
+  l = warp_sum(l);
+
+  // a threshold with at least K of the chunk's columns at or above it: the lanes' own maxima, halved into from both ends
+  unsigned tv = 0;
+  if (__popcll(__ballot(n > 0)) >= a.K) {
+    unsigned lo = ~wave_umax(~(n ? om : 0u)), hi = top;  // every lane is >= lo
+    for (int it = 0; it < 12 && lo < hi; ++it) {
+      const unsigned mid = lo + (hi - lo) / 2 + 1;
+      if (__popcll(__ballot(n > 0 && om >= mid)) >= a.K) lo = mid;
+      else hi = mid - 1;
+    }
+    tv = lo;
+  }
+  if (lane == 0) {
+    sml[wave] = make_float2(mw, l);
+    stv[wave] = tv;
+  }
+  if (tid == 0) scount = 0;
+  __syncthreads();
+  tv = max(max(stv[0], stv[1]), max(stv[2], stv[3]));
+#pragma unroll
+  for (int e = 0; e < kSelE; ++e) {
+    if (e < n && o[e] >= tv) {
+      const int at = atomicAdd(&scount, 1);
+      if (at < kSelList) list[at] = key_of(o[e], col(e));
+    }
+  }
+  __syncthreads();
+  int cnt = scount;
+  if (cnt > kSelList) {  // many equal logits: each wave draws its K largest keys one by one
+    __syncthreads();
+    u64 last = ~0ull;
+    for (int i = 0; i < a.K; ++i) {
+      u64 best = 0;
+#pragma unroll
+      for (int e = 0; e < kSelE; ++e) {
+        const u64 k = key_of(o[e], col(e));
+        if (e < n && k < last && k > best) best = k;
+      }
+      best = wave_kmax(best);
+      if (lane == 0) list[wave * a.K + i] = best;
+      last = best;  // 0 once the wave has no more: nothing is below it
+    }
+    cnt = 4 * a.K;
+    __syncthreads();
+  }
+  u64* out = a.keys + ((long)row * a.C + c) * a.K;
+  if (tid < cnt) {  // every key is its own: the rank is the number of greater ones
+    const u64 k = list[tid];
+    int rank = 0;
+    for (int i = 0; i < cnt; ++i) rank += list[i] > k;
+    if (k && rank < a.K) out[rank] = k;
+  }
+  // fewer columns than K (the last chunk): the rest of the list is empty
+  const int have = min(a.V - c0, kSelChunk);
+  if (tid >= have && tid < a.K) out[tid] = 0;
+  if (tid == 0) {
+    float M = sml[0].x;
+    for (int w = 1; w < 4; ++w) M = fmaxf(M, sml[w].x);
+    float L = 0.f;
+    for (int w = 0; w < 4; ++w) L += sml[w].x == -INFINITY && sml[w].y == 0.f ? 0.f : sml[w].y * __expf(sml[w].x - (M == -INFINITY ? 0.f : M));
+    a.ml[(long)row * a.C + c] = make_float2(M, L);
+  }
+}
+
+__device__ __forceinline__ u64 ord_d(double v) {
+  const u64 u = (u64)__double_as_longlong(v);
+  return (u >> 63) ? ~u : (u | 0x8000000000000000ull);
+}
+
+// One workgroup a batch entry, one wave a row: the row's sum, then its k best of the chunks' sorted lists (a lane holds
+// a list's head), then every candidate's rank over all rows' lists by binary search (they are sorted alike).
+__global__ __launch_bounds__(1024) void beam_pick_kernel(SelArgs a) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  u64* sc = reinterpret_cast<u64*>(smem);             // [W][K] ordered bits of the scores, descending
+  int* ti = reinterpret_cast<int*>(sc + a.W * a.K);   // [W][K] tokens; -1 = none
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, nw = blockDim.x >> 6;
+  const int b = blockIdx.x, K = a.K;
+  const u64 ninf = ord_d(-INFINITY);
+  __shared__ float sin_s[kSelMaxW];
+  __shared__ unsigned char fin_s[kSelMaxW];
+  for (int w = tid; w < a.W; w += blockDim.x) {
+    sin_s[w] = a.score[(long)b * a.W + w];
+    fin_s[w] = a.fin ? a.fin[(long)b * a.W + w] : 0;
+  }
+  __syncthreads();
+  for (int w = wave; w < a.W; w += nw) {
+    const long row = (long)b * a.W + w;
+    const float s = sin_s[w];
+    const bool fin = fin_s[w] != 0;
+    double M = 0.0, lt = 0.0;  // the row's maximum, and the log of its sum of e^{x - M}: apart, since M may be huge
+    bool live = !fin && !(s == -INFINITY || s != s);
+    if (live) {
+      const float2 x = lane < a.C ? a.ml[row * a.C + lane] : make_float2(-INFINITY, 0.f);
+      M = (double)unord_f(wave_umax(ord_f(x.x)));
+      double t = lane < a.C ? (x.x == -INFINITY && x.y == 0.f ? 0.0 : (double)x.y * exp((double)x.x - M)) : 0.0;
+      for (int k = 32; k > 0; k >>= 1) t += __shfl_xor(t, k, 64);
+      lt = log(t);
+      live = t > 0.0 && lt - lt == 0.0 && M - M == 0.0;  // a row of -inf, or with a NaN or +inf, offers nothing
+    }
+    if (live) {
+      const u64* lp = a.keys + (row * a.C + lane) * K;
+      u64 cur = lane < a.C ? lp[0] : 0, nxt = lane < a.C && K > 1 ? lp[1] : 0;
+      int at = 2;
+      for (int i = 0; i < K; ++i) {
+        const u64 best = wave_kmax(cur);
+        if (lane == 0) {
+          double v = (double)s + (((double)unord_f((unsigned)(best >> 32)) - M) - lt) + 0.0;
+          if (v != v) v = -INFINITY;  // +inf score and a -inf logit
+          sc[w * K + i] = ord_d(v);
+          ti[w * K + i] = best ? key_idx(best) : -1;
+        }
+        if (cur == best && best) {
+          cur = nxt;
+          nxt = at < K ? lp[at] : 0;
+          ++at;
+        }
+      }
+    } else {
+      // every score is -inf, but the one continuation of a row that has ended: the lowest tokens stand for the rest
+      const bool keep = fin && s == s && s != -INFINITY;
+      for (int i = lane; i < K; i += 64) {
+        int t = i;
+        u64 v = ninf;
+        if (keep) {
+          if (i == 0) { t = a.pad; v = ord_d((double)s + 0.0); }
+          else t = i - 1 < a.pad ? i - 1 : i;
+        }
+        sc[w * K + i] = v;
+        ti[w * K + i] = t < a.V ? t : -1;
+      }
+    }
+  }
+  __syncthreads();
+  for (int i = tid; i < a.W * K; i += blockDim.x) {
+    const int w = i / K, t = ti[i];
+    if (t < 0) continue;
+    const u64 v = sc[i];
+    int rank = i - w * K;  // within its own list
+    for (int u = 0; u < a.W && rank < K; ++u) {
+      if (u == w) continue;
+      int lo = 0, hi = K;  // how many of list u come before (v, w * V + t)
+      while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        const bool before = ti[u * K + mid] >= 0 && (sc[u * K + mid] > v || (sc[u * K + mid] == v && u < w));
+        if (before) lo = mid + 1;
+        else hi = mid;
+      }
+      rank += lo;
+    }
+    if (rank < K) {
+      const long o = (long)b * K + rank;
+      const u64 u = (v >> 63) ? (v & 0x7FFFFFFFFFFFFFFFull) : ~v;
+      a.score_out[o] = (float)__longlong_as_double((long long)u);
+      a.parent[o] = w;
+      a.token[o] = t;
+      if (a.fin_out) a.fin_out[o] = fin_s[w] || t == a.eos;
+    }
+  }
+}
+
+// ---- slx_beam_reorder: x[o, b, w] = x[o, b, parent[b, w]] -------------------------------------------------------
+// A thread takes one column of all `width` rows of a batch entry: every row is loaded before any is stored, so the
+// state may be reordered in place, whatever the parents; in place, rows that stay are neither read nor written.
+struct ReorderArgs {
+  const char* src; char* dst;
+  long s0, s1, sr, d0, d1, dr;  // byte strides: two outer axes and the rows, of source and destination
+  int n0, n1, B, W;
+  long cols;                    // columns (elements of the access type) of a row
+  const int* parent;
+  int in_place;
+};
+
+template <typename T, int MW>
+__global__ __launch_bounds__(256) void beam_reorder_kernel(ReorderArgs a) {
+  const long c = (long)blockIdx.x * 256 + threadIdx.x;
+  if (c >= a.cols) return;
+  for (long o = blockIdx.y; o < (long)a.n0 * a.n1 * a.B; o += gridDim.y) {
+    const long b = o % a.B, q = o / a.B, i1 = q % a.n1, i0 = q / a.n1;
+    const int* par = a.parent + b * a.W;
+    const char* sp = a.src + i0 * a.s0 + i1 * a.s1 + b * a.W * a.sr + c * (long)sizeof(T);
+    char* dp = a.dst + i0 * a.d0 + i1 * a.d1 + b * a.W * a.dr + c * (long)sizeof(T);
+    T v[MW];
+    bool mv[MW];
+#pragma unroll
+    for (int w = 0; w < MW; ++w) {
+      mv[w] = w < a.W;
+      if (mv[w]) {
+        int p = par[w];
+        if ((unsigned)p >= (unsigned)a.W) p = w;  // no such beam: the row stays
+        mv[w] = !(a.in_place && p == w);
+        if (mv[w]) v[w] = *reinterpret_cast<const T*>(sp + p * a.sr);
+      }
+    }
+#pragma unroll
+    for (int w = 0; w < MW; ++w)
+      if (mv[w]) *reinterpret_cast<T*>(dp + w * a.dr) = v[w];
+  }
+}
+
+template <typename T>
+static void reorder_launch(const ReorderArgs& a, hipStream_t st) {
+  const long n = (long)a.n0 * a.n1 * a.B;
+  const dim3 grid((unsigned)((a.cols + 255) / 256), (unsigned)(n < 65535 ? n : 65535));
+  if (a.W <= 4) hipLaunchKernelGGL((beam_reorder_kernel<T, 4>), grid, dim3(256), 0, st, a);
+  else if (a.W <= 8) hipLaunchKernelGGL((beam_reorder_kernel<T, 8>), grid, dim3(256), 0, st, a);
+  else if (a.W <= 16) hipLaunchKernelGGL((beam_reorder_kernel<T, 16>), grid, dim3(256), 0, st, a);
+  else if (a.W <= 32) hipLaunchKernelGGL((beam_reorder_kernel<T, 32>), grid, dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((beam_reorder_kernel<T, 64>), grid, dim3(256), 0, st, a);
+}
+
+static int check_select(const slx_beam_select_desc* d) {
+  SLX_CHECK_ARG(d != nullptr, "slx_beam_select: null desc");
+  SLX_CHECK_ARG(d->batch >= 0 && d->batch <= 65535 / kSelMaxW && d->width > 0 && d->width <= kSelMaxW,
+                "slx_beam_select: 0 <= batch <= %d, 0 < width <= %d", 65535 / kSelMaxW, kSelMaxW);
+  SLX_CHECK_ARG(d->vocab > 0 && d->vocab <= kSelChunk * kSelMaxChunks, "slx_beam_select: 0 < vocab <= %d", kSelChunk * kSelMaxChunks);
+  SLX_CHECK_ARG(d->k > 0 && d->k <= kSelMaxK && d->k <= (int64_t)d->width * d->vocab, "slx_beam_select: 0 < k <= %d and <= width * vocab", kSelMaxK);
+  SLX_CHECK_ARG(d->ldx >= d->vocab, "slx_beam_select: ldx >= vocab");
+  SLX_CHECK_ARG(!d->finished || (d->pad >= 0 && d->pad < d->vocab), "slx_beam_select: pad outside the vocabulary");
+  return 0;
+}
+
+}  // namespace slx
+
+using namespace slx;
+
+extern "C" {
+
+int64_t slx_beam_select_ws_bytes(const slx_beam_select_desc* d) {
+  if (int rc = check_select(d)) return rc;
+  const int64_t C = (d->vocab + kSelChunk - 1) / kSelChunk;
+  return (int64_t)d->batch * d->width * C * (8 + 8 * (int64_t)d->k);
+}
+
+int slx_beam_select(const slx_beam_select_desc* d, slx_stream_t s) {
+  if (int rc = check_select(d)) return rc;
+  if (d->batch == 0) return 0;
+  SLX_CHECK_ARG(d->logits && d->score && d->score_out && d->parent && d->token, "slx_beam_select: null argument");
+  const int64_t need = slx_beam_select_ws_bytes(d);
+  SLX_CHECK_ARG(d->ws && ((uintptr_t)d->ws & 7) == 0 && d->ws_bytes >= need, "slx_beam_select: needs an 8-B aligned workspace of %lld bytes", (long long)need);
+  SelArgs a;
+  memset(&a, 0, sizeof(a));
+  a.x = d->logits; a.ldx = d->ldx; a.score = d->score; a.fin = d->finished;
+  a.score_out = d->score_out; a.parent = d->parent; a.token = d->token; a.fin_out = d->finished_out;
+  a.B = d->batch; a.W = d->width; a.V = d->vocab; a.K = d->k; a.pad = d->pad; a.eos = d->eos;
+  a.C = (d->vocab + kSelChunk - 1) / kSelChunk;
+  a.ml = (float2*)d->ws;
+  a.keys = (u64*)((char*)d->ws + (int64_t)a.B * a.W * a.C * 8);
+  const dim3 grid(a.C, a.B * a.W);
+  if (d->logits_bf16) hipLaunchKernelGGL(beam_chunk_kernel<bf16>, grid, dim3(256), 0, (hipStream_t)s, a);
+  else hipLaunchKernelGGL(beam_chunk_kernel<float>, grid, dim3(256), 0, (hipStream_t)s, a);
+  SLX_LAUNCH_CHECK("slx_beam_select (chunks)");
+  const int nw = a.W < 16 ? a.W : 16;
+  hipLaunchKernelGGL(beam_pick_kernel, dim3(a.B), dim3(64 * nw), (size_t)a.W * a.K * 12, (hipStream_t)s, a);
+  SLX_LAUNCH_CHECK("slx_beam_select");
+  return 0;
+}
+
+int slx_beam_reorder(const slx_beam_reorder_desc* d, slx_stream_t s) {
+  SLX_CHECK_ARG(d != nullptr, "slx_beam_reorder: null desc");
+  SLX_CHECK_ARG(d->n0 >= 0 && d->n1 >= 0 && d->batch >= 0 && d->row_bytes >= 0 && d->width > 0 && d->width <= kSelMaxW,
+                "slx_beam_reorder: extents >= 0, 0 < width <= %d", kSelMaxW);
+  if (d->n0 == 0 || d->n1 == 0 || d->batch == 0 || d->row_bytes == 0) return 0;
+  SLX_CHECK_ARG(d->src && d->dst && d->parent, "slx_beam_reorder: null argument");
+  ReorderArgs a;
+  memset(&a, 0, sizeof(a));
+  a.src = (const char*)d->src; a.dst = (char*)d->dst;
+  a.s0 = d->s0; a.s1 = d->s1; a.sr = d->src_row; a.d0 = d->d0; a.d1 = d->d1; a.dr = d->dst_row;
+  a.n0 = d->n0; a.n1 = d->n1; a.B = d->batch; a.W = d->width; a.parent = d->parent;
+  a.in_place = d->src == d->dst;
+  SLX_CHECK_ARG(!a.in_place || (a.s0 == a.d0 && a.s1 == a.d1 && a.sr == a.dr), "slx_beam_reorder: in place needs equal strides");
+  // the widest access that the row's length and every stride and address allow
+  const uint64_t u = (uint64_t)(uintptr_t)d->src | (uint64_t)(uintptr_t)d->dst | (uint64_t)d->s0 | (uint64_t)d->s1 |
+                     (uint64_t)d->src_row | (uint64_t)d->d0 | (uint64_t)d->d1 | (uint64_t)d->dst_row | (uint64_t)d->row_bytes;
+  const int w = (u & 15) == 0 ? 16 : (u & 3) == 0 ? 4 : (u & 1) == 0 ? 2 : 1;
+  a.cols = d->row_bytes / w;
+  SLX_CHECK_ARG((a.cols + 255) / 256 < 2147483648L, "slx_beam_reorder: rows too long");
+  if (w == 16) reorder_launch<u32x4>(a, (hipStream_t)s);
+  else if (w == 4) reorder_launch<unsigned>(a, (hipStream_t)s);
+  else if (w == 2) reorder_launch<unsigned short>(a, (hipStream_t)s);
+  else reorder_launch<unsigned char>(a, (hipStream_t)s);
+  SLX_LAUNCH_CHECK("slx_beam_reorder");
+  return 0;
+}
+
+}  // extern "C"
