@@ -427,7 +427,10 @@ __global__ __launch_bounds__(256) void norm_bwd_wave1024_kernel(NormArgs a) {
       dv[0] = r.df[i].x; dv[1] = r.df[i].y; dv[2] = r.df[i].z; dv[3] = r.df[i].w;
     }
   };
+  // Which products fuse into an add is written out here: left to the compiler, the LS and the plain form of this kernel
+  // fused differently and dx differed in its last bit between them.
   auto process = [&](const RowIn& cur, long row) {
+#pragma clang fp contract(off)
     const float mu = cur.mu, rs = cur.rs;
     float s1 = 0.f, s2 = 0.f;
 #pragma unroll
@@ -442,7 +445,7 @@ __global__ __launch_bounds__(256) void norm_bwd_wave1024_kernel(NormArgs a) {
         const float xh = (tv[e] - mu) * rs;
         const float gd = dv[e] * gv[e];
         s1 += gd;
-        s2 += gd * xh;
+        s2 = __builtin_fmaf(gd, xh, s2);
         ag[e] = dv[e] * (RMS ? (float)(bf16)xh : xh);
       }
       acc4(0, col, ag);
@@ -462,11 +465,11 @@ __global__ __launch_bounds__(256) void norm_bwd_wave1024_kernel(NormArgs a) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const float xh = (tv[e] - mu) * rs;
-          const float gd = __fmul_rn(dv[e], gv[e]);  // a rounded product, as norm_bwd_wave_kernel keeps it
-          ov[e] = rs * (gd - m1 - xh * m2);
+          const float gd = dv[e] * gv[e];  // a rounded product, as norm_bwd_wave_kernel keeps it
+          const float dxo[4] = {cur.dxo[i].x, cur.dxo[i].y, cur.dxo[i].z, cur.dxo[i].w};
+          ov[e] = __builtin_fmaf(rs, __builtin_fmaf(-xh, m2, gd - m1), dxo[e]);
         }
       }
-      ov[0] += cur.dxo[i].x; ov[1] += cur.dxo[i].y; ov[2] += cur.dxo[i].z; ov[3] += cur.dxo[i].w;
       *reinterpret_cast<float4*>(a.dx + row * a.lddx + col) = make_float4(ov[0], ov[1], ov[2], ov[3]);
       if constexpr (LS) {
         const float4 l4 = *reinterpret_cast<const float4*>(&gl[LS ? 1 : 0][col]);
