@@ -546,7 +546,7 @@ typedef struct slx_prefix_attn_desc {
   int max_prefix, max_own;                   /* bounds of plen and olen (longer ones are cut to them)                  */
   int pcols, ocols;                          /* table columns                                                          */
   int groups, width, n_q, Hq;
-  float scale;
+  float scale;                               /* > 0                                                                    */
   float* ws; int64_t ws_floats;              /* slx_prefix_attn_ws_floats(d); one call at a time                       */
 } slx_prefix_attn_desc;
 /* token t of a sequence's n_q attends the plen[group] keys of its group's prefix and its own keys j <= olen - n_q + t; a

@@ -93,16 +93,24 @@ __global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs a) {
 // o = sum_p e^{m_p - m} o_p / sum_p e^{m_p - m} l_p over the parts p of a row's keys, each with its own maximum m_p,
 // sum l_p and unnormalised output o_p (the softmax is over the union, so any split of the keys is exact).
 //
-// The prefix of a group is read once for all of its width * n_q * (Hq / Hkv) query rows of a kv head: a workgroup
-// takes 16 * NQ of those rows and one range of the prefix, whose 32-key tiles its 4 waves share out; the sequences'
-// own keys are workgroups of the same launch, with the n_q * (Hq / Hkv) rows of one sequence. Each writes (m, l, o) of
-// its range, and a second launch joins a row's parts.
+// The prefix of a group is read once for all of its width * n_q * (Hq / Hkv) query rows of a kv head; the sequences'
+// own keys are workgroups of the same launch, with the n_q * (Hq / Hkv) rows of one sequence. A workgroup takes a tile
+// of rows and one range of the keys and writes (m, l, o) of it; a second launch joins a row's parts.
 //
-// Per tile and wave: S^T = K Q^T on v_mfma_f32_16x16x32_bf16 with the keys as rows and the queries as columns, so a
+// Per 32 keys and wave: S^T = K Q^T on v_mfma_f32_16x16x32_bf16 with the keys as rows and the queries as columns, so a
 // lane holds 8 keys of ONE query, and the probabilities are already the B operand of O^T += V^T P^T (the sum over keys
-// may take them in any order: slot j of lane group q is key 4q + j, or 16 + 4q + j - 4). V^T's A operand needs 8 keys
-// of one d: a lane loads D/16 neighbouring d of each of its 8 keys and pairs them with v_perm_b32 (the MFMA row r of
-// product e stands for d = (D/16) r + e), so nothing goes through LDS before the final merge of the waves.
+// may take them in any order: slot j of lane group g is key 4g + j, or 16 + 4g + j - 4). V^T's A operand needs 8 keys
+// of one d: a lane takes D/16 neighbouring d of each of its 8 keys and pairs them with v_perm_b32 (the MFMA row r of
+// product e stands for d = (D/16) r + e). The row sums are one more MFMA, with an A operand of ones.
+//
+// Two forms of a workgroup (4 waves), by the rows that share the keys:
+//   direct (up to 32 rows): all waves have the same rows; each takes every fourth 32-key tile straight into registers
+//     (K's next tile is requested once the scores have used the last, V's after the output has), the waves' states are
+//     merged through LDS at the end. Few rows: the bytes in flight count, and no wave waits for another.
+//   streamed (more rows): 64 or 128 rows, 16 or 32 a wave, so the keys are fetched once for all of them: tiles of 32 keys
+//     arrive by LDS-DMA in a ring of 4, one barrier a tile. Rows of K and V lie in LDS with their 16-B chunks XOR-ed by
+//     the slot (and slots with bits 0 and 2 swapped), which keeps both operands' reads free of bank conflicts. One page
+//     number a wave and tile (scalar load), so pages of at least 8 slots; smaller ones take the direct form.
 struct Seg {
   PoolView p;
   const int* tab; long ldt;
@@ -116,99 +124,277 @@ struct PAttnArgs {
   float* lse;
   Seg pre, own;
   int W, Tq, Hq, Hkv, gq;
-  float c;  // scale * log2(e)
+  unsigned gmul;  // r / gq = umulhi(r, gmul) (0: gq == 1)
+  float c;        // scale * log2(e) > 0
   int mt_pre, mt_own;
-  long n_pre;  // workgroups of the prefix part
-  int direct;  // one part per row: the workgroups write the output themselves
-  long R;      // rows * Hq
-  float* ws;   // o [parts][R][D], then (m, l) [parts][R]
+  long groups, n_pre;  // n_pre: workgroups of the prefix part
+  int direct;     // one part per row: the workgroups write the output themselves
+  long R;         // rows * Hq
+  float* ws;      // o [parts][R][D], then (m, l) [parts][R]
 };
 
 __host__ __device__ __forceinline__ int split_keys(int len, int ns) { return ((len + ns - 1) / ns + 127) & ~127; }
 __device__ __forceinline__ int seg_len(const Seg& s, long i) { return s.len ? max(0, min(s.len[i], s.cap)) : 0; }
+__device__ __forceinline__ int row_token(const PAttnArgs& a, int r) { return a.gmul ? (int)__umulhi((unsigned)r, a.gmul) : r; }
+
+// one workgroup's share, uniform
+struct Item {
+  const bf16 *k, *v;  // of the kv head
+  long ps, ss;
+  int n_pages, shift;
+  const int* tab;
+  int len, kb, ke;    // keys of the sequence; this range
+  bool causal;
+  int kvh, ntok, mt, part;
+  long tok0;          // first query token
+};
 
 template <int D, int NQ>
-__device__ __forceinline__ void attn_item(const PAttnArgs& a, const Seg& sg, const int* tab, bool causal, int len, int kb,
-                                          int ke, int kvh, long tok0, int ntok, int mt, int part, char* smem) {
-  constexpr int KK = D / 32, NE = D / 16;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 15, grp = lane >> 4;
-  const int rows = ntok * a.gq, r0 = mt * 16 * NQ;
-  const int shift = sg.p.shift, mask = (1 << shift) - 1;
-  const unsigned npg = (unsigned)sg.p.n_pages;
-  const bf16* kbase = sg.p.k + kvh * sg.p.hs + 8 * grp;
-  const bf16* vbase = sg.p.v + kvh * sg.p.hs + NE * col;
-  // the causal edge of an own segment: token t of Tq sees keys <= len - Tq + t
-  const int tmin = r0 / a.gq, tmax = (min(r0 + 16 * NQ, rows) - 1) / a.gq;
-  const int free_end = causal ? min(ke, len - a.Tq + tmin + 1) : ke;  // keys below it are seen by every row
-  if (causal) ke = min(ke, len - a.Tq + tmax + 1);
+struct State {
+  float m[NQ];
+  f32x4 l[NQ], o[NQ][D / 16];
+};
 
+template <int D, int NQ>
+__device__ __forceinline__ void state_init(State<D, NQ>& st) {
+#pragma unroll
+  for (int n = 0; n < NQ; ++n) {
+    st.m[n] = -INFINITY;
+    st.l[n] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int e = 0; e < D / 16; ++e) st.o[n][e] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+}
+
+// query rows r0 .. of a wave as B operands; lim: the keys each row sees
+template <int D, int NQ>
+__device__ __forceinline__ void load_rows(const PAttnArgs& a, const Item& w, int r0, bf16x8 (&qf)[NQ][D / 32], int (&lim)[NQ]) {
+  const int col = threadIdx.x & 15, grp = (threadIdx.x & 63) >> 4, rows = w.ntok * a.gq;
+#pragma unroll
+  for (int n = 0; n < NQ; ++n) {
+    const int r = min(r0 + 16 * n + col, rows - 1), t = row_token(a, r);
+    const bf16* qp = a.q + (w.tok0 + t) * a.ldq + (long)(w.kvh * a.gq + r - t * a.gq) * D + 8 * grp;
+#pragma unroll
+    for (int k = 0; k < D / 32; ++k) qf[n][k] = *reinterpret_cast<const bf16x8*>(qp + 32 * k);
+    lim[n] = w.causal ? min(w.ke, w.len - a.Tq + t + 1) : w.ke;
+  }
+}
+
+template <int D, int NQ>
+__device__ __forceinline__ void scores(const bf16x8 (&kf)[2][D / 32], const bf16x8 (&qf)[NQ][D / 32], f32x4 (&s)[NQ][2]) {
+#pragma unroll
+  for (int n = 0; n < NQ; ++n)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      s[n][h] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int k = 0; k < D / 32; ++k) s[n][h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[h][k], qf[n][k], s[n][h], 0, 0, 0);
+    }
+}
+
+// Scores to probabilities. `edge`: the tile holds keys that some row does not see (room: how many of the tile's keys each
+// row sees) or that are not there (dead: bit j of the lane's 8 keys).
+template <int D, int NQ>
+__device__ __forceinline__ void softmax_step(f32x4 (&s)[NQ][2], float c, bool edge, unsigned dead, const int (&lim)[NQ], int k0,
+                                             State<D, NQ>& st, bf16x8 (&pb)[NQ]) {
+  const int grp = (threadIdx.x & 63) >> 4;
+#pragma unroll
+  for (int n = 0; n < NQ; ++n) {
+    if (edge) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if ((dead >> j & 1) || k0 + 16 * (j >> 2) + 4 * grp + (j & 3) >= lim[n]) s[n][j >> 2][j & 3] = -INFINITY;
+    }
+    float mx = s[n][0][0];
+#pragma unroll
+    for (int j = 1; j < 8; ++j) mx = fmaxf(mx, s[n][j >> 2][j & 3]);
+    mx *= c;
+    // the running maximum moves only when a score passes it by 2^8 (exact all the same: it cancels in o / l)
+    if (__any(mx > st.m[n] + 8.0f)) {
+      mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+      mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+      const float mn = fmaxf(st.m[n], mx);
+      const float r = st.m[n] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(st.m[n] - mn);
+      st.m[n] = mn;
+      st.l[n] *= r;
+#pragma unroll
+      for (int e = 0; e < D / 16; ++e) st.o[n][e] *= r;
+    }
+    const float mu = st.m[n] == -INFINITY ? 0.f : st.m[n];
+    // P in bf16 for the MFMA (half a step, 2^-8 of each term at most, as the output itself is rounded); l sums the same
+    // rounded values, so what is left is the terms' own scatter
+#pragma unroll
+    for (int j = 0; j < 8; ++j) pb[n][j] = (bf16)__builtin_amdgcn_exp2f(__builtin_fmaf(s[n][j >> 2][j & 3], c, -mu));
+  }
+}
+
+// V of keys that are not there becomes 0 (0 * NaN would reach every row); with `sift`, so do values that are not finite
+// in keys that some row does not see yet -> whether there were any (they are added at the end: add_nonfinite)
+template <int D>
+__device__ __forceinline__ bool clean_v(unsigned (&vr)[8][D / 32], unsigned dead, bool sift) {
+  bool odd = false;
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) {
+      unsigned x = (dead >> j & 1) ? 0u : vr[j][i];
+      if (sift) {
+        const bool lo = (x & 0x7F80u) == 0x7F80u, hi = (x & 0x7F800000u) == 0x7F800000u;
+        odd = odd || lo || hi;
+        x = (lo ? 0u : (x & 0xFFFFu)) | (hi ? 0u : (x & 0xFFFF0000u));
+      }
+      vr[j][i] = x;
+    }
+  return odd;
+}
+
+template <int D, int NQ>
+__device__ __forceinline__ void output_step(const unsigned (&vr)[8][D / 32], const bf16x8 (&pb)[NQ], State<D, NQ>& st) {
+  union { unsigned u[4]; bf16x8 b; } vt;
+  vt.u[0] = vt.u[1] = vt.u[2] = vt.u[3] = 0x3F803F80u;  // ones
+#pragma unroll
+  for (int n = 0; n < NQ; ++n) st.l[n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vt.b, pb[n], st.l[n], 0, 0, 0);
+#pragma unroll
+  for (int e = 0; e < D / 16; ++e) {
+#pragma unroll
+    for (int p = 0; p < 4; ++p)
+      vt.u[p] = __builtin_amdgcn_perm(vr[2 * p + 1][e >> 1], vr[2 * p][e >> 1], (e & 1) ? 0x07060302u : 0x05040100u);
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) st.o[n][e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vt.b, pb[n], st.o[n][e], 0, 0, 0);
+  }
+}
+
+// A row's (m, l, o) to the output or the workspace; a lane has d = (D/4) grp + (D/16) i + e of row r.
+template <int D>
+__device__ __forceinline__ void store_row(const PAttnArgs& a, const Item& w, int r, float m, float l, const f32x4 (&o)[D / 16]) {
+  constexpr int NE = D / 16;
+  const int grp = (threadIdx.x & 63) >> 4, t = row_token(a, r), head = w.kvh * a.gq + r - t * a.gq;
+  const long row = (w.tok0 + t) * a.Hq + head;
+  if (a.direct) {
+    const float inv = l > 0.f || l != l ? 1.0f / l : 0.f;  // no key seen: zeros
+    bf16* op = a.out + (w.tok0 + t) * a.ldo + (long)head * D + (D / 4) * grp;
+#pragma unroll
+    for (int b = 0; b < NE / 2; ++b) {
+      bf16x8 y;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) y[j] = (bf16)(o[(8 * b + j) % NE][(8 * b + j) / NE] * inv);
+      *reinterpret_cast<bf16x8*>(op + 8 * b) = y;
+    }
+    if (a.lse && grp == 0) a.lse[row] = m == -INFINITY ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
+  } else {
+    float* op = a.ws + ((long)w.part * a.R + row) * D + (D / 4) * grp;
+#pragma unroll
+    for (int b = 0; b < NE; ++b) {
+      f32x4 y;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) y[j] = o[(4 * b + j) % NE][(4 * b + j) / NE];
+      *reinterpret_cast<f32x4*>(op + 4 * b) = y;
+    }
+    if (grp == 0) {
+      float* ml = a.ws + (long)(a.pre.ns + a.own.ns) * a.R * D + ((long)w.part * a.R + row) * 2;
+      *reinterpret_cast<float2*>(ml) = make_float2(m, l);
+    }
+  }
+}
+
+// Values that are not finite, of the keys from the first that some row of the tile does not see: onto the rows that see
+// them (p > 0 there, so inf and NaN arrive whatever p is), in what this thread has just stored. Rare, so kept small.
+template <int D>
+__device__ __forceinline__ void add_nonfinite(const PAttnArgs& a, const Item& w, int r) {
+  const int grp = (threadIdx.x & 63) >> 4, t = row_token(a, r), head = w.kvh * a.gq + r - t * a.gq;
+  const int from = max(w.kb, (max(0, w.len - a.Tq)) & ~31), to = min(w.ke, w.len - a.Tq + t + 1);
+  bf16* op = a.out + (w.tok0 + t) * a.ldo + (long)head * D + (D / 4) * grp;
+  float* wp = a.ws + ((long)w.part * a.R + (w.tok0 + t) * a.Hq + head) * D + (D / 4) * grp;
+#pragma unroll 1
+  for (int key = from; key < to; ++key) {
+    const int e = w.tab[key >> w.shift];
+    if ((unsigned)e >= (unsigned)w.n_pages) continue;
+    const bf16* p = w.v + (long)e * w.ps + (long)(key & ((1 << w.shift) - 1)) * w.ss + (D / 4) * grp;
+#pragma unroll 1
+    for (int d = 0; d < D / 4; ++d) {
+      const float v = (float)p[d];
+      if (fabsf(v) < INFINITY) continue;
+      if (a.direct) op[d] = (bf16)((float)op[d] + v);
+      else wp[d] += v;
+    }
+  }
+}
+
+template <int D, int NQ>
+__device__ __forceinline__ void attn_direct(const PAttnArgs& a, Item w, char* smem) {
+  constexpr int KK = D / 32, NE = D / 16;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, grp = lane >> 4;
+  const int rows = w.ntok * a.gq, r0 = w.mt * 16 * NQ;
+  const int shift = w.shift, mask = (1 << shift) - 1;
   bf16x8 qf[NQ][KK];
   int lim[NQ];
-#pragma unroll
-  for (int n = 0; n < NQ; ++n) {
-    const int r = min(r0 + 16 * n + col, rows - 1), t = r / a.gq;
-    const bf16* qp = a.q + (tok0 + t) * a.ldq + (long)(kvh * a.gq + r - t * a.gq) * D + 8 * grp;
-#pragma unroll
-    for (int k = 0; k < KK; ++k) qf[n][k] = *reinterpret_cast<const bf16x8*>(qp + 32 * k);
-    lim[n] = causal ? min(ke, len - a.Tq + t + 1) : ke;
-  }
-
-  float m[NQ], l[NQ];
-  f32x4 o[NQ][NE];
-#pragma unroll
-  for (int n = 0; n < NQ; ++n) {
-    m[n] = -INFINITY;
-    l[n] = 0.f;
-#pragma unroll
-    for (int e = 0; e < NE; ++e) o[n][e] = f32x4{0.f, 0.f, 0.f, 0.f};
-  }
+  load_rows<D, NQ>(a, w, r0, qf, lim);
+  // the causal edge of an own segment: token t of Tq sees keys <= len - Tq + t
+  const int free_end = w.causal ? min(w.ke, w.len - a.Tq + row_token(a, r0) + 1) : w.ke;  // keys below it are seen by every row
+  const int ke = w.causal ? min(w.ke, w.len - a.Tq + row_token(a, min(r0 + 16 * NQ, rows) - 1) + 1) : w.ke;
+  const bf16 *kbase = w.k + 8 * grp, *vbase = w.v + NE * col;
+  State<D, NQ> st;
+  state_init(st);
 
   bf16x8 kf[2][KK];
-  unsigned vr[8][NE / 2];  // NE d of each of the lane's 8 keys
-  bool vok[8];
-  const bool fine = shift < 2;  // pages of 1 or 2 slots: a page number for each key of a lane's four
-  auto entry = [&](int key) { return tab[min(key, len - 1) >> shift]; };
-  auto offset = [&](int e, int key) {
-    return (unsigned)e < npg ? (long)e * sg.p.ps + (long)(min(key, len - 1) & mask) * sg.p.ss : 0L;
+  unsigned vr[8][NE / 2], bad = 0;  // bad: bit j = the lane's key j is on no page
+  const bool fine = shift < 2;      // pages of 1 or 2 slots: a page number for each of a lane's keys
+  auto entry = [&](int key) { return w.tab[min(key, w.len - 1) >> shift]; };
+  auto at = [&](const bf16* base, int e, int key) {
+    return base + ((unsigned)e < (unsigned)w.n_pages ? (long)e * w.ps : 0L) + (long)(key & mask) * w.ss;
+  };
+  auto ldv = [&](int j, const bf16* p) {
+    if constexpr (NE == 4) {
+      const u32x2 x = *reinterpret_cast<const u32x2*>(p);
+      vr[j][0] = x[0]; vr[j][1] = x[1];
+    } else {
+      const u32x4 x = *reinterpret_cast<const u32x4*>(p);
+#pragma unroll
+      for (int i = 0; i < NE / 2; ++i) vr[j][i] = x[i];
+    }
   };
   int ek[2], ev[2];  // page numbers of the next tile to load
   auto entries_k = [&](int k0) {
-    if (k0 >= ke) return;
 #pragma unroll
     for (int s = 0; s < 2; ++s) ek[s] = entry(k0 + 16 * s + col);
   };
   auto entries_v = [&](int k0) {
-    if (k0 >= ke || fine) return;
+    if (fine) return;
 #pragma unroll
     for (int s = 0; s < 2; ++s) ev[s] = entry(k0 + 16 * s + 4 * grp);
   };
   auto load_k = [&](int k0) {
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
-      const bf16* p = kbase + offset(ek[s], k0 + 16 * s + col);
+      const bf16* p = at(kbase, ek[s], k0 + 16 * s + col);
 #pragma unroll
       for (int k = 0; k < KK; ++k) kf[s][k] = *reinterpret_cast<const bf16x8*>(p + 32 * k);
     }
   };
   auto load_v = [&](int k0) {
+    bad = 0;
+    if (fine) {
+      int e[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int key = k0 + 16 * (j >> 2) + 4 * grp + (j & 3);
-      const int e = fine ? entry(key) : ev[j >> 2];
-      vok[j] = (unsigned)e < npg && key < len;
-      const bf16* p = vbase + offset(e, key);
-      if constexpr (NE == 4) {
-        const u32x2 x = *reinterpret_cast<const u32x2*>(p);
-        vr[j][0] = x[0]; vr[j][1] = x[1];
-      } else {
-        const u32x4 x = *reinterpret_cast<const u32x4*>(p);
+      for (int j = 0; j < 8; ++j) e[j] = entry(k0 + 16 * (j >> 2) + 4 * grp + (j & 3));
 #pragma unroll
-        for (int i = 0; i < NE / 2; ++i) vr[j][i] = x[i];
+      for (int j = 0; j < 8; ++j) {
+        bad |= ((unsigned)e[j] >= (unsigned)w.n_pages ? 1u : 0u) << j;
+        ldv(j, at(vbase, e[j], k0 + 4 * grp + (j & 3)));
+      }
+    } else {
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        bad |= ((unsigned)ev[s] >= (unsigned)w.n_pages ? 15u : 0u) << (4 * s);
+        const bf16* p = at(vbase, ev[s], k0 + 16 * s + 4 * grp);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) ldv(4 * s + j, p + j * w.ss);
       }
     }
   };
 
-  int k0 = kb + 32 * wave;
+  bool odd = false;
+  int k0 = w.kb + 32 * wave;
   if (k0 < ke) {
     entries_k(k0);
     entries_v(k0);
@@ -219,164 +405,74 @@ __device__ __forceinline__ void attn_item(const PAttnArgs& a, const Seg& sg, con
   }
   for (; k0 < ke; k0 += 128) {
     f32x4 s[NQ][2];
+    bf16x8 pb[NQ];
+    scores<D, NQ>(kf, qf, s);
+    const bool edge = k0 + 32 > free_end || __any(bad != 0);
+    unsigned dead = bad;
+    if (edge) {
 #pragma unroll
-    for (int n = 0; n < NQ; ++n)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        s[n][h] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int k = 0; k < KK; ++k) s[n][h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[h][k], qf[n][k], s[n][h], 0, 0, 0);
-      }
-    bool good = true;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) good = good && vok[j];
-    const bool edge = k0 + 32 > free_end || __any(!good);
-    bool vk[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) vk[j] = vok[j];
-    if (k0 + 128 < ke) {
+      for (int j = 0; j < 8; ++j) dead |= (k0 + 16 * (j >> 2) + 4 * grp + (j & 3) >= w.len ? 1u : 0u) << j;
+    }
+    const bool more = k0 + 128 < ke;
+    if (more) {
       load_k(k0 + 128);
       entries_k(k0 + 256);
     }
-    bf16x8 pb[NQ];
-#pragma unroll
-    for (int n = 0; n < NQ; ++n) {
-      float x[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = s[n][j >> 2][j & 3] * a.c;
-      if (edge) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (!vk[j] || k0 + 16 * (j >> 2) + 4 * grp + (j & 3) >= lim[n]) x[j] = -INFINITY;
-      }
-      float mx = x[0];
-#pragma unroll
-      for (int j = 1; j < 8; ++j) mx = fmaxf(mx, x[j]);
-      // the running maximum moves only when a score passes it by 2^8 (exact all the same: it cancels in o / l)
-      if (__any(mx > m[n] + 8.0f)) {
-        mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-        mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-        const float mn = fmaxf(m[n], mx);
-        const float r = m[n] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[n] - mn);
-        m[n] = mn;
-        l[n] *= r;
-#pragma unroll
-        for (int e = 0; e < NE; ++e)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) o[n][e][i] *= r;
-      }
-      const float mu = m[n] == -INFINITY ? 0.f : m[n];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        // P in bf16 for the MFMA (half a step, 2^-9 of each term, as the output itself is rounded); l sums the same
-        // rounded values, so what is left is the terms' own scatter
-        const float p = __builtin_amdgcn_exp2f(x[j] - mu);
-        pb[n][j] = (bf16)p;
-        l[n] += (float)pb[n][j];
-      }
-    }
-    if (edge) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-#pragma unroll
-        for (int i = 0; i < NE / 2; ++i) vr[j][i] = vk[j] ? vr[j][i] : 0u;
-      if (causal && k0 + 32 > free_end) {
-        // keys that some row does not see yet: 0 * inf would reach it through the MFMA, so non-finite values leave the
-        // operand and are added to the rows that see them
-        bool odd = false;
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-#pragma unroll
-          for (int i = 0; i < NE / 2; ++i) {
-            const unsigned x = vr[j][i];
-            const bool lo = (x & 0x7F80u) == 0x7F80u, hi = (x & 0x7F800000u) == 0x7F800000u;
-            odd = odd || lo || hi;
-            vr[j][i] = (lo ? 0u : (x & 0xFFFFu)) | (hi ? 0u : (x & 0xFFFF0000u));
-          }
-        if (__any(odd)) {
-          for (int kk = 0; kk < 32 && k0 + kk < ke; ++kk) {
-            const int e = entry(k0 + kk);
-            if ((unsigned)e >= npg) continue;
-            const bf16* p = sg.p.v + kvh * sg.p.hs + offset(e, k0 + kk) + (D / 4) * grp;
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-              for (int ee = 0; ee < NE; ++ee) {
-                const float v = (float)p[NE * i + ee];
-                const bool nf = !(fabsf(v) < INFINITY);
-#pragma unroll
-                for (int n = 0; n < NQ; ++n)
-                  if (nf && k0 + kk < lim[n]) o[n][ee][i] += v;
-              }
-          }
-        }
-      }
-    }
-#pragma unroll
-    for (int e = 0; e < NE; ++e) {
-      union { unsigned u[4]; bf16x8 b; } vt;
-#pragma unroll
-      for (int p = 0; p < 4; ++p)
-        vt.u[p] = __builtin_amdgcn_perm(vr[2 * p + 1][e >> 1], vr[2 * p][e >> 1], (e & 1) ? 0x07060302u : 0x05040100u);
-#pragma unroll
-      for (int n = 0; n < NQ; ++n) o[n][e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vt.b, pb[n], o[n][e], 0, 0, 0);
-    }
-    if (k0 + 128 < ke) {
+    softmax_step<D, NQ>(s, a.c, edge, dead, lim, k0, st, pb);
+    if (edge) odd = clean_v<D>(vr, dead, w.causal && a.Tq > 1) || odd;
+    output_step<D, NQ>(vr, pb, st);
+    if (more) {
       load_v(k0 + 128);
       entries_v(k0 + 256);
     }
   }
 
   // ---- the 4 waves' (m, l, o) into one: waves 2, 3 hand theirs to 0, 1, then 1 to 0
-  float* sm = reinterpret_cast<float*>(smem);      // [4][16 NQ]
-  float* sl = sm + 4 * 16 * NQ;                    // [4][16 NQ]
+  float* sm = reinterpret_cast<float*>(smem);              // [4][16 NQ]
+  float* sl = sm + 4 * 16 * NQ;                            // [4][16 NQ]
   f32x4* so = reinterpret_cast<f32x4*>(sl + 4 * 16 * NQ);  // [2][NQ * NE][64 lanes]
   float M[NQ], L[NQ];
+  if (grp == 0) {
 #pragma unroll
-  for (int n = 0; n < NQ; ++n) {
-    l[n] += __shfl_xor(l[n], 16, 64);
-    l[n] += __shfl_xor(l[n], 32, 64);
-    if (grp == 0) {
-      sm[wave * 16 * NQ + 16 * n + col] = m[n];
-      sl[wave * 16 * NQ + 16 * n + col] = l[n];
+    for (int n = 0; n < NQ; ++n) {
+      sm[wave * 16 * NQ + 16 * n + col] = st.m[n];
+      sl[wave * 16 * NQ + 16 * n + col] = st.l[n][0];
     }
   }
-  __syncthreads();
+  odd = __syncthreads_or(odd);
 #pragma unroll
   for (int n = 0; n < NQ; ++n) {
     float mw[4];
 #pragma unroll
-    for (int w = 0; w < 4; ++w) mw[w] = sm[w * 16 * NQ + 16 * n + col];
+    for (int v = 0; v < 4; ++v) mw[v] = sm[v * 16 * NQ + 16 * n + col];
     M[n] = fmaxf(fmaxf(mw[0], mw[1]), fmaxf(mw[2], mw[3]));
     L[n] = 0.f;
 #pragma unroll
-    for (int w = 0; w < 4; ++w)
-      L[n] += mw[w] == -INFINITY ? 0.f : sl[w * 16 * NQ + 16 * n + col] * __builtin_amdgcn_exp2f(mw[w] - M[n]);
-    const float r = m[n] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[n] - M[n]);
+    for (int v = 0; v < 4; ++v)
+      L[n] += mw[v] == -INFINITY ? 0.f : sl[v * 16 * NQ + 16 * n + col] * __builtin_amdgcn_exp2f(mw[v] - M[n]);
+    const float r = st.m[n] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(st.m[n] - M[n]);
 #pragma unroll
-    for (int e = 0; e < NE; ++e)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) o[n][e][i] *= r;
+    for (int e = 0; e < NE; ++e) st.o[n][e] *= r;
   }
   if (wave >= 2) {
 #pragma unroll
     for (int n = 0; n < NQ; ++n)
 #pragma unroll
-      for (int e = 0; e < NE; ++e) so[((wave - 2) * NQ * NE + n * NE + e) * 64 + lane] = o[n][e];
+      for (int e = 0; e < NE; ++e) so[((wave - 2) * NQ * NE + n * NE + e) * 64 + lane] = st.o[n][e];
   }
   __syncthreads();
   if (wave < 2) {
 #pragma unroll
     for (int n = 0; n < NQ; ++n)
 #pragma unroll
-      for (int e = 0; e < NE; ++e) o[n][e] += so[(wave * NQ * NE + n * NE + e) * 64 + lane];
+      for (int e = 0; e < NE; ++e) st.o[n][e] += so[(wave * NQ * NE + n * NE + e) * 64 + lane];
   }
   __syncthreads();
   if (wave == 1) {
 #pragma unroll
     for (int n = 0; n < NQ; ++n)
 #pragma unroll
-      for (int e = 0; e < NE; ++e) so[(n * NE + e) * 64 + lane] = o[n][e];
+      for (int e = 0; e < NE; ++e) so[(n * NE + e) * 64 + lane] = st.o[n][e];
   }
   __syncthreads();
   if (wave != 0) return;
@@ -384,134 +480,289 @@ __device__ __forceinline__ void attn_item(const PAttnArgs& a, const Seg& sg, con
   for (int n = 0; n < NQ; ++n) {
     const int r = r0 + 16 * n + col;
     if (r >= rows) continue;
-    const int t = r / a.gq, head = kvh * a.gq + r - t * a.gq;
-    const long row = (tok0 + t) * a.Hq + head;
-    float x[4 * NE];  // d = (D/4) grp + NE i + e
 #pragma unroll
-    for (int e = 0; e < NE; ++e) {
-      o[n][e] += so[(n * NE + e) * 64 + lane];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) x[NE * i + e] = o[n][e][i];
-    }
-    if (a.direct) {
-      const float inv = L[n] > 0.f || L[n] != L[n] ? 1.0f / L[n] : 0.f;  // no key seen: zeros
-      bf16* op = a.out + (tok0 + t) * a.ldo + (long)head * D + (D / 4) * grp;
-#pragma unroll
-      for (int b = 0; b < NE / 2; ++b) {
-        bf16x8 y;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) y[j] = (bf16)(x[8 * b + j] * inv);
-        *reinterpret_cast<bf16x8*>(op + 8 * b) = y;
-      }
-      if (a.lse && grp == 0) a.lse[row] = M[n] == -INFINITY ? -INFINITY : (M[n] + log2f(L[n])) * 0.69314718055994531f;
-    } else {
-      float* op = a.ws + ((long)part * a.R + row) * D + (D / 4) * grp;
-#pragma unroll
-      for (int b = 0; b < NE; ++b) *reinterpret_cast<f32x4*>(op + 4 * b) = f32x4{x[4 * b], x[4 * b + 1], x[4 * b + 2], x[4 * b + 3]};
-      if (grp == 0) {
-        float* ml = a.ws + (long)(a.pre.ns + a.own.ns) * a.R * D + ((long)part * a.R + row) * 2;
-        *reinterpret_cast<float2*>(ml) = make_float2(M[n], L[n]);
-      }
-    }
+    for (int e = 0; e < NE; ++e) st.o[n][e] += so[(n * NE + e) * 64 + lane];
+    store_row<D>(a, w, r, M[n], L[n], st.o[n]);
+    if (odd) add_nonfinite<D>(a, w, r);
   }
 }
 
-template <int D, int NQP, int NQO>
+constexpr int kRing = 4;
+template <int N>
+__device__ __forceinline__ void wait_vm() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
+// 16 B a lane from global memory to LDS at the wave's base + 16 * lane (m0: the base)
+__device__ __forceinline__ void dma16(const void* g, const char* lds) {
+  const unsigned m = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)LDS_PTR(const char, lds));
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(m), "v"(g) : "memory");
+}
+
+template <int D, int NQ>
+__device__ __forceinline__ void attn_stream(const PAttnArgs& a, Item w, char* smem) {
+  constexpr int KK = D / 32, NE = D / 16, CH = D / 8, TILE = 32 * D * 2, PER = 2 * D / 64;  // PER: DMA pieces a wave and tile
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, grp = lane >> 4;
+  const int rows = w.ntok * a.gq, rw = w.mt * 64 * NQ, r0 = rw + wave * 16 * NQ;
+  const int shift = w.shift, mask = (1 << shift) - 1;
+  unsigned char* badb = reinterpret_cast<unsigned char*>(smem + kRing * 2 * TILE);  // [kRing][4]: 8 keys a wave, 0 or 255
+  bf16x8 qf[NQ][KK];
+  int lim[NQ];
+  load_rows<D, NQ>(a, w, r0, qf, lim);
+  auto tok_of = [&](int r) { return row_token(a, min(r, rows - 1)); };
+  const int free_end = w.causal ? min(w.ke, w.len - a.Tq + tok_of(r0) + 1) : w.ke;  // seen by every row of the wave
+  const int ke = w.causal ? min(w.ke, w.len - a.Tq + tok_of(rw + 64 * NQ - 1) + 1) : w.ke;
+  const int kw = r0 >= rows ? 0 : w.causal ? min(w.ke, w.len - a.Tq + tok_of(r0 + 16 * NQ - 1) + 1) : w.ke;  // this wave's last
+  const int nt = ke > w.kb ? (ke - w.kb + 31) / 32 : 0;
+  State<D, NQ> st;
+  state_init(st);
+  // the queries are here before the first DMA is counted
+  __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
+#pragma unroll
+  for (int n = 0; n < NQ; ++n)
+#pragma unroll
+    for (int k = 0; k < KK; ++k) asm volatile("" : "+v"(qf[n][k]));
+
+  // LDS rows: slot of key x = x with bits 0 and 2 swapped; chunk c of a slot lies at c ^ swz(slot)
+  auto slot_of = [](int x) { return (x & ~5) | (x & 1) << 2 | (x >> 2 & 1); };
+  auto swz = [](int slot) { return D == 64 ? slot >> 1 & 7 : slot & 15; };
+  typedef const int __attribute__((address_space(4))) cint;
+  auto entry = [&](int t) {  // the page of this wave's 8 keys of tile t
+    const int key = min(w.kb + 32 * min(t, nt - 1) + 8 * wave, w.len - 1);
+    return ((cint*)(uintptr_t)w.tab)[__builtin_amdgcn_readfirstlane(key >> shift)];
+  };
+  auto issue = [&](int t, int e) {
+    char* base = smem + (t % kRing) * 2 * TILE;
+    const bool ok = (unsigned)e < (unsigned)w.n_pages;
+    const long page = ok ? (long)e * w.ps : 0L;
+    if (lane == 0) badb[(t % kRing) * 4 + wave] = ok ? 0 : 255;
+#pragma unroll
+    for (int i = 0; i < PER / 2; ++i) {
+      const int slot = 8 * wave + (64 / CH) * i + lane / CH, key = slot_of(slot), ch = (lane % CH) ^ swz(slot);
+      const long off = page + (long)((w.kb + 32 * t + key) & mask) * w.ss + 8 * ch;
+      dma16(w.k + off, base + (8 * wave + (64 / CH) * i) * D * 2);
+      dma16(w.v + off, base + TILE + (8 * wave + (64 / CH) * i) * D * 2);
+    }
+  };
+  int e0 = 0, e1 = 0, e2 = 0, en = 0;
+  if (nt > 0) { e0 = entry(0); e1 = entry(1); e2 = entry(2); en = entry(3); }
+  if (nt > 0) issue(0, e0);
+  if (nt > 1) issue(1, e1);
+  if (nt > 2) issue(2, e2);
+  bool odd = false;
+  for (int t = 0; t < nt; ++t) {
+    const int k0 = w.kb + 32 * t;
+    if (nt - 1 - t >= 2) wait_vm<2 * PER>();
+    else if (nt - 1 - t == 1) wait_vm<PER>();
+    else wait_vm<0>();
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // this wave has read the slot that is filled next
+    __builtin_amdgcn_s_barrier();
+    if (t + 3 < nt) {
+      issue(t + 3, en);
+      en = entry(t + 4);
+    }
+    if (k0 >= kw) continue;
+    const char* Kl = smem + (t % kRing) * 2 * TILE;
+    const char* Vl = Kl + TILE;
+    const unsigned bads = *reinterpret_cast<const unsigned*>(badb + (t % kRing) * 4);
+    bf16x8 kf[2][KK];
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      const int slot = slot_of(16 * s + col);
+#pragma unroll
+      for (int k = 0; k < KK; ++k) kf[s][k] = *reinterpret_cast<const bf16x8*>(Kl + slot * D * 2 + ((4 * k + grp) ^ swz(slot)) * 16);
+    }
+    f32x4 s[NQ][2];
+    bf16x8 pb[NQ];
+    unsigned vr[8][NE / 2];
+    scores<D, NQ>(kf, qf, s);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int slot = slot_of(16 * (j >> 2) + 4 * grp + (j & 3));
+      if constexpr (NE == 4) {
+        const u32x2 x = *reinterpret_cast<const u32x2*>(Vl + slot * D * 2 + ((col >> 1) ^ swz(slot)) * 16 + (col & 1) * 8);
+        vr[j][0] = x[0]; vr[j][1] = x[1];
+      } else {
+        const u32x4 x = *reinterpret_cast<const u32x4*>(Vl + slot * D * 2 + (col ^ swz(slot)) * 16);
+#pragma unroll
+        for (int i = 0; i < NE / 2; ++i) vr[j][i] = x[i];
+      }
+    }
+    const bool edge = k0 + 32 > free_end || __builtin_amdgcn_readfirstlane(bads) != 0;
+    unsigned dead = 0;
+    if (edge) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int x = 16 * (j >> 2) + 4 * grp + (j & 3);
+        dead |= (k0 + x >= w.len || (bads >> x & 1) ? 1u : 0u) << j;
+      }
+    }
+    softmax_step<D, NQ>(s, a.c, edge, dead, lim, k0, st, pb);
+    if (edge) odd = clean_v<D>(vr, dead, w.causal && a.Tq > 1) || odd;
+    output_step<D, NQ>(vr, pb, st);
+  }
+  odd = __any(odd);
+#pragma unroll
+  for (int n = 0; n < NQ; ++n) {
+    const int r = r0 + 16 * n + col;
+    if (r >= rows) continue;
+    store_row<D>(a, w, r, st.m[n], st.l[n][0], st.o[n]);
+    if (odd) add_nonfinite<D>(a, w, r);
+  }
+}
+
+// kinds of a workgroup: direct with 16 or 32 rows, streamed with 64 or 128
+enum { kD16 = 0, kD32 = 1, kS64 = 2, kS128 = 3 };
+constexpr int kKindRows[4] = {16, 32, 64, 128};
+template <int D, int KIND>
+__device__ __forceinline__ void attn_kind(const PAttnArgs& a, const Item& w, char* smem) {
+  if constexpr (KIND == kD16) attn_direct<D, 1>(a, w, smem);
+  else if constexpr (KIND == kD32) attn_direct<D, 2>(a, w, smem);
+  else if constexpr (KIND == kS64) attn_stream<D, 1>(a, w, smem);
+  else attn_stream<D, 2>(a, w, smem);
+}
+constexpr int kind_lds(int D, int kind) {
+  return kind >= kS64 ? kRing * 2 * 32 * D * 2 + 4 * kRing : 2 * 4 * 16 * (kind + 1) * 4 + 2 * (kind + 1) * (D / 16) * 64 * 16;
+}
+
+template <int D, int KP, int KO>
 __global__ __launch_bounds__(256, 2) void prefix_attn_kernel(PAttnArgs a) {
-  constexpr int NQ = NQP > NQO ? NQP : NQO;
-  __shared__ __attribute__((aligned(16))) char smem[2 * 4 * 16 * NQ * 4 + 2 * NQ * (D / 16) * 64 * 16];
+  constexpr int LDS = kind_lds(D, KP) > kind_lds(D, KO) ? kind_lds(D, KP) : kind_lds(D, KO);
+  __shared__ __attribute__((aligned(16))) char smem[LDS];
   long b = blockIdx.x;
-  if (b < a.n_pre) {  // [row tile][group][kv head][range]
-    const int sp = (int)(b % a.pre.ns);
+  const bool pre = b < a.n_pre;
+  Item w;
+  long seq;
+  if (pre) {  // [group][kv head][range][row tile]; 8 neighbours stay 8 apart, so the row tiles of a range share an XCD's L2
+    const long x = b & 7, y = b >> 3;
+    w.mt = (int)(y % a.mt_pre);
+    b = (y / a.mt_pre) * 8 + x;
+    w.part = (int)(b % a.pre.ns);
     b /= a.pre.ns;
-    const int kvh = (int)(b % a.Hkv);
-    b /= a.Hkv;
-    const long ng = a.n_pre / ((long)a.pre.ns * a.Hkv * a.mt_pre);
-    const long g = b % ng;
-    const int mt = (int)(b / ng);
-    const int len = seg_len(a.pre, g), ks = split_keys(len, a.pre.ns), kb = sp * ks;
-    if (kb >= len) return;
-    attn_item<D, NQP>(a, a.pre, a.pre.tab + g * a.pre.ldt, false, len, kb, min(len, kb + ks), kvh, g * a.W * a.Tq,
-                      a.W * a.Tq, mt, sp, smem);
+    w.kvh = (int)(b % a.Hkv);
+    seq = b / a.Hkv;
+    if (seq >= a.groups) return;  // the grid is padded to a multiple of 8
+    w.tok0 = seq * a.W * a.Tq;
+    w.ntok = a.W * a.Tq;
+    w.len = seg_len(a.pre, seq);
   } else {  // [sequence][row tile][kv head][range]
     b -= a.n_pre;
-    const int sp = (int)(b % a.own.ns);
+    w.part = (int)(b % a.own.ns);
     b /= a.own.ns;
-    const int kvh = (int)(b % a.Hkv);
+    w.kvh = (int)(b % a.Hkv);
     b /= a.Hkv;
-    const int mt = (int)(b % a.mt_own);
-    const long n = b / a.mt_own;
-    const int len = seg_len(a.own, n), ks = split_keys(len, a.own.ns), kb = sp * ks;
-    if (kb >= len && !(a.direct && sp == 0)) return;
-    attn_item<D, NQO>(a, a.own, a.own.tab + n * a.own.ldt, true, len, kb, min(len, kb + ks), kvh, n * a.Tq, a.Tq, mt,
-                      a.pre.ns + sp, smem);
+    w.mt = (int)(b % a.mt_own);
+    seq = b / a.mt_own;
+    w.tok0 = seq * a.Tq;
+    w.ntok = a.Tq;
+    w.len = seg_len(a.own, seq);
+  }
+  const int ks = split_keys(w.len, pre ? a.pre.ns : a.own.ns);
+  w.kb = w.part * ks;
+  if (w.kb >= w.len && !a.direct) return;
+  w.ke = min(w.len, w.kb + ks);
+  w.causal = !pre;
+  w.k = (pre ? a.pre.p.k : a.own.p.k) + w.kvh * (pre ? a.pre.p.hs : a.own.p.hs);
+  w.v = (pre ? a.pre.p.v : a.own.p.v) + w.kvh * (pre ? a.pre.p.hs : a.own.p.hs);
+  w.ps = pre ? a.pre.p.ps : a.own.p.ps;
+  w.ss = pre ? a.pre.p.ss : a.own.p.ss;
+  w.n_pages = pre ? a.pre.p.n_pages : a.own.p.n_pages;
+  w.shift = pre ? a.pre.p.shift : a.own.p.shift;
+  w.tab = pre ? a.pre.tab + seq * a.pre.ldt : a.own.tab + seq * a.own.ldt;
+  if (!pre) w.part += a.pre.ns;
+  if constexpr (KP == KO) {
+    attn_kind<D, KP>(a, w, smem);
+  } else {
+    if (pre) attn_kind<D, KP>(a, w, smem);
+    else attn_kind<D, KO>(a, w, smem);
   }
 }
 
-// joins the parts of a row: D / 4 threads a row, four d a thread
-template <int D>
+// Joins the parts of a row: D / 4 threads, four d each, times PG groups that share the parts out (16 or 8 for rows with
+// many parts, where a row's parts would otherwise be one chain of loads).
+template <int D, int PG>
 __global__ __launch_bounds__(256) void prefix_attn_join_kernel(PAttnArgs a) {
-  constexpr int TPR = D / 4;
-  const long row = ((long)blockIdx.x * 256 + threadIdx.x) / TPR;
-  const int d = (threadIdx.x % TPR) * 4;
-  if (row >= a.R) return;
+  constexpr int TPR = D / 4, RPB = 256 / (TPR * PG), B = 4;
+  __shared__ float sml[PG > 1 ? PG : 1][2];
+  __shared__ __attribute__((aligned(16))) f32x4 so[PG > 1 ? PG : 1][TPR];
+  const int d4 = threadIdx.x % TPR, pg = threadIdx.x / TPR % PG;
+  const long row = (long)blockIdx.x * RPB + threadIdx.x / (TPR * PG);
+  if (row >= a.R) return;  // PG > 1: one row a workgroup
   const long tok = row / a.Hq, n = tok / a.Tq;
   const int pl = seg_len(a.pre, n / a.W), ol = seg_len(a.own, n);
   const int np = pl ? (pl + split_keys(pl, a.pre.ns) - 1) / split_keys(pl, a.pre.ns) : 0;
   const int no = ol ? (ol + split_keys(ol, a.own.ns) - 1) / split_keys(ol, a.own.ns) : 0;
   const float2* ml = reinterpret_cast<const float2*>(a.ws + (long)(a.pre.ns + a.own.ns) * a.R * D) + row;
-  const float* ob = a.ws + row * D + d;
+  const float* ob = a.ws + row * D + 4 * d4;
   float m = -INFINITY, l = 0.f;
   f32x4 o = {0.f, 0.f, 0.f, 0.f};
-  constexpr int B = 4;
-  for (int i0 = 0; i0 < np + no; i0 += B) {
-    float2 x[B];
-    f32x4 y[B];
-#pragma unroll
-    for (int u = 0; u < B; ++u) {
-      const int i = min(i0 + u, np + no - 1), p = i < np ? i : a.pre.ns + i - np;
-      x[u] = ml[(long)p * a.R];
-      y[u] = *reinterpret_cast<const f32x4*>(ob + (long)p * a.R * D);
-      if (i0 + u >= np + no) x[u].x = -INFINITY;
-    }
+  auto add = [&](const float (&xm)[B], const float (&xl)[B], const f32x4 (&y)[B]) {
     float mn = m;
 #pragma unroll
-    for (int u = 0; u < B; ++u) mn = fmaxf(mn, x[u].x);
+    for (int u = 0; u < B; ++u) mn = fmaxf(mn, xm[u]);
     const float r = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
     l *= r;
     o *= r;
 #pragma unroll
     for (int u = 0; u < B; ++u) {
-      if (x[u].x == -INFINITY) continue;  // its o was not computed from any key
-      const float w = __builtin_amdgcn_exp2f(x[u].x - mn);
-      l = __builtin_fmaf(w, x[u].y, l);
+      if (xm[u] == -INFINITY) continue;  // its o was not computed from any key
+      const float w = __builtin_amdgcn_exp2f(xm[u] - mn);
+      l = __builtin_fmaf(w, xl[u], l);
 #pragma unroll
       for (int j = 0; j < 4; ++j) o[j] = __builtin_fmaf(w, y[u][j], o[j]);
     }
     m = mn;
+  };
+  for (int i0 = pg; i0 < np + no; i0 += B * PG) {
+    float xm[B], xl[B];
+    f32x4 y[B];
+#pragma unroll
+    for (int u = 0; u < B; ++u) {
+      const int i = min(i0 + u * PG, np + no - 1), p = i < np ? i : a.pre.ns + i - np;
+      const float2 x = ml[(long)p * a.R];
+      y[u] = *reinterpret_cast<const f32x4*>(ob + (long)p * a.R * D);
+      xm[u] = i0 + u * PG < np + no ? x.x : -INFINITY;
+      xl[u] = x.y;
+    }
+    add(xm, xl, y);
+  }
+  if constexpr (PG > 1) {
+    so[pg][d4] = o;
+    if (d4 == 0) { sml[pg][0] = m; sml[pg][1] = l; }
+    __syncthreads();
+    if (pg) return;
+    m = -INFINITY;
+    l = 0.f;
+    o = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i0 = 0; i0 < PG; i0 += B) {
+      float xm[B], xl[B];
+      f32x4 y[B];
+#pragma unroll
+      for (int u = 0; u < B; ++u) { xm[u] = sml[i0 + u][0]; xl[u] = sml[i0 + u][1]; y[u] = so[i0 + u][d4]; }
+      add(xm, xl, y);
+    }
   }
   const float inv = l > 0.f || l != l ? 1.0f / l : 0.f;
   bf16x4 y;
 #pragma unroll
   for (int j = 0; j < 4; ++j) y[j] = (bf16)(o[j] * inv);
-  *reinterpret_cast<bf16x4*>(a.out + tok * a.ldo + (row - tok * a.Hq) * D + d) = y;
-  if (a.lse && d == 0) a.lse[row] = m == -INFINITY ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
+  *reinterpret_cast<bf16x4*>(a.out + tok * a.ldo + (row - tok * a.Hq) * D + 4 * d4) = y;
+  if (a.lse && d4 == 0) a.lse[row] = m == -INFINITY ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
 }
 
-// Row tiles and key ranges of a call: a rule on sizes and the host's bounds alone, so a captured call replays for any
-// lengths up to them. 16, 32 or (head size 64) 64 rows a workgroup, the fewest that hold all rows that share the keys;
-// as many ranges as give about kTarget workgroups, each of at least 128 keys (one tile a wave).
-constexpr long kTarget = 1024;
-struct PAttnPlan { int nqp, nqo, mtp, mto, nsp, nso; };
+// Row tiles and key ranges of a call: a rule on sizes, page sizes and the host's bounds alone, so a captured call replays
+// for any lengths up to them. As many ranges as give about kTarget workgroups, each of at least 128 keys.
+constexpr long kTarget = 512;
+struct PAttnPlan { int kp, ko, mtp, mto, nsp, nso; };
 static PAttnPlan plan_attn(const slx_prefix_attn_desc* d, int capp, int capo) {
   PAttnPlan p;
-  const int gq = d->Hq / d->own_pool.heads, most = d->own_pool.head_dim == 64 ? 4 : 2;
-  auto tile = [&](long rows) { return rows <= 16 ? 1 : (rows <= 32 || most == 2) ? 2 : 4; };
+  const int gq = d->Hq / d->own_pool.heads;
+  auto kind = [](long rows, int page) { return rows <= 16 ? kD16 : rows <= 32 || page < 8 ? kD32 : rows <= 64 ? kS64 : kS128; };
   const long rp = (long)d->width * d->n_q * gq, ro = (long)d->n_q * gq;
-  p.nqo = tile(ro);
-  p.nqp = capp > 0 ? tile(rp) : p.nqo;
-  p.mtp = (int)((rp + 16 * p.nqp - 1) / (16 * p.nqp));
-  p.mto = (int)((ro + 16 * p.nqo - 1) / (16 * p.nqo));
+  p.ko = kind(ro, d->own_pool.page);
+  p.kp = capp > 0 ? kind(rp, d->prefix_pool.page) : p.ko;
+  if (p.kp == kD32 && p.ko >= kS64) p.ko = kD32;       // fewer kernels: a streamed own part goes with a streamed prefix,
+  if (p.kp == kS128 && p.ko == kS64) p.ko = kS128;     // of the same rows
+  p.mtp = (int)((rp + kKindRows[p.kp] - 1) / kKindRows[p.kp]);
+  p.mto = (int)((ro + kKindRows[p.ko] - 1) / kKindRows[p.ko]);
   const long up = (capp + 127) / 128, uo = (capo + 127) / 128;  // units of 128 keys
   const long ip = (long)d->groups * d->own_pool.heads * p.mtp, io = (long)d->groups * d->width * d->own_pool.heads * p.mto;
   const long per = (ip * up + io * uo + kTarget - 1) / kTarget, u = per > 1 ? per : 1;
@@ -543,6 +794,10 @@ static int check_attn(const slx_prefix_attn_desc* d, int* capp, int* capo) {
   SLX_CHECK_ARG(d->groups >= 0 && d->width > 0 && d->n_q > 0 && d->Hq > 0 && d->Hq % d->own_pool.heads == 0,
                 "slx_prefix_attn: groups >= 0, width, n_q > 0 and Hq a multiple of the pool's heads");
   SLX_CHECK_ARG((double)d->groups * d->width * d->n_q * d->Hq < 2147483648.0, "slx_prefix_attn: too many rows");
+  // row / gq is a multiplication (exact while row * gq < 2^32)
+  SLX_CHECK_ARG((double)d->width * d->n_q * (d->Hq / d->own_pool.heads) * (d->Hq / d->own_pool.heads) < 4294967296.0,
+                "slx_prefix_attn: too many rows");
+  SLX_CHECK_ARG(d->scale > 0.0f && d->scale < INFINITY, "slx_prefix_attn: scale must be positive");
   SLX_CHECK_ARG(d->max_own >= 0 && d->ocols > 0 && d->ldot >= d->ocols, "slx_prefix_attn: max_own >= 0, ldot >= ocols > 0");
   *capo = cap_of(d->max_own, d->ocols, d->own_pool.page);
   *capp = 0;
@@ -560,13 +815,23 @@ static int check_attn(const slx_prefix_attn_desc* d, int* capp, int* capo) {
 template <int D>
 static void launch_attn(const PAttnPlan& p, dim3 grid, hipStream_t st, const PAttnArgs& a) {
 #define SLX_PA(P, O)                                                                                         \
-  if (p.nqp == P && p.nqo == O) {                                                                            \
+  if (p.kp == P && p.ko == O) {                                                                              \
     hipLaunchKernelGGL((prefix_attn_kernel<D, P, O>), grid, dim3(256), 0, st, a);                            \
     return;                                                                                                  \
   }
-  SLX_PA(1, 1) SLX_PA(2, 1) SLX_PA(2, 2)
-  if constexpr (D == 64) { SLX_PA(4, 1) SLX_PA(4, 2) SLX_PA(4, 4) }
+  SLX_PA(kD16, kD16) SLX_PA(kD32, kD16) SLX_PA(kD32, kD32) SLX_PA(kS64, kD16) SLX_PA(kS64, kD32) SLX_PA(kS64, kS64)
+  SLX_PA(kS128, kD16) SLX_PA(kS128, kD32) SLX_PA(kS128, kS128)
 #undef SLX_PA
+}
+template <int D>
+static void launch_join(int parts, hipStream_t st, const PAttnArgs& a) {
+  constexpr int PG = 1024 / D;  // one row a workgroup
+  if (parts > 8) {
+    hipLaunchKernelGGL((prefix_attn_join_kernel<D, PG>), dim3((unsigned)a.R), dim3(256), 0, st, a);
+  } else {
+    constexpr int RPB = 1024 / D;
+    hipLaunchKernelGGL((prefix_attn_join_kernel<D, 1>), dim3((unsigned)((a.R + RPB - 1) / RPB)), dim3(256), 0, st, a);
+  }
 }
 
 }  // namespace slx
@@ -626,8 +891,9 @@ int slx_prefix_attn(const slx_prefix_attn_desc* d, slx_stream_t s) {
   if (p.nsp > 0) a.pre = Seg{view(d->prefix_pool), d->ptab, (long)d->ldpt, d->plen, capp, p.nsp};
   a.W = d->width; a.Tq = d->n_q; a.Hq = d->Hq; a.Hkv = Hkv; a.gq = d->Hq / Hkv;
   a.c = d->scale * 1.44269504088896341f;
-  a.mt_pre = p.mtp; a.mt_own = p.mto;
-  a.n_pre = (long)d->groups * Hkv * p.mtp * p.nsp;
+  a.gmul = a.gq == 1 ? 0u : (unsigned)((1ull << 32) / a.gq + 1);
+  a.mt_pre = p.mtp; a.mt_own = p.mto; a.groups = d->groups;
+  a.n_pre = ((long)d->groups * Hkv * p.nsp + 7) / 8 * 8 * p.mtp;
   a.direct = p.nsp + p.nso == 1;
   a.R = (long)d->groups * d->width * d->n_q * d->Hq;
   a.ws = d->ws;
@@ -640,9 +906,8 @@ int slx_prefix_attn(const slx_prefix_attn_desc* d, slx_stream_t s) {
   else launch_attn<128>(p, dim3((unsigned)blocks), (hipStream_t)s, a);
   SLX_LAUNCH_CHECK("slx_prefix_attn");
   if (!a.direct) {
-    const long jb = (a.R * (D / 4) + 255) / 256;
-    if (D == 64) hipLaunchKernelGGL(prefix_attn_join_kernel<64>, dim3((unsigned)jb), dim3(256), 0, (hipStream_t)s, a);
-    else hipLaunchKernelGGL(prefix_attn_join_kernel<128>, dim3((unsigned)jb), dim3(256), 0, (hipStream_t)s, a);
+    if (D == 64) launch_join<64>(p.nsp + p.nso, (hipStream_t)s, a);
+    else launch_join<128>(p.nsp + p.nso, (hipStream_t)s, a);
     SLX_LAUNCH_CHECK("slx_prefix_attn (join)");
   }
   return 0;

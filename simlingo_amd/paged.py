@@ -16,7 +16,9 @@ positions and tables are read on the device, so a captured call follows their co
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
+import struct
 
 import torch
 
@@ -58,66 +60,88 @@ class BeamReorderDesc(ctypes.Structure):  # slx_beam_reorder_desc
                 ("batch", K.c_int), ("width", K.c_int), ("parent", K.c_vp)]
 
 
-K.register("slx_kv_append", [ctypes.POINTER(KVAppendDesc), K.c_vp])
-K.register("slx_prefix_attn", [ctypes.POINTER(PrefixAttnDesc), K.c_vp])
-K.register("slx_prefix_attn_ws_floats", [ctypes.POINTER(PrefixAttnDesc)], K.c_i64)
-K.register("slx_beam_select", [ctypes.POINTER(BeamSelectDesc), K.c_vp])
-K.register("slx_beam_select_ws_bytes", [ctypes.POINTER(BeamSelectDesc)], K.c_i64)
-K.register("slx_beam_reorder", [ctypes.POINTER(BeamReorderDesc), K.c_vp])
+for _name in ("slx_kv_append", "slx_prefix_attn", "slx_beam_select", "slx_beam_reorder"):
+    K.register(_name, [K.c_vp, K.c_vp])
+K.register("slx_prefix_attn_ws_floats", [K.c_vp], K.c_i64)
+K.register("slx_beam_select_ws_bytes", [K.c_vp], K.c_i64)
 
 MAX_WIDTH = MAX_K = 64      # beam_select, beam_reorder
 MAX_VOCAB = 262144          # beam_select
 
+# The calls below are a token's step many times over, on small tensors: descriptors are packed in one go (native sizes and
+# alignment, the structures' own layout) and a check builds its message only when it fails.
+_POOL = "PPqqqiiii"
+_APPEND = struct.Struct("@" + _POOL + "PqPqPqiiPPiiqPPi0q")
+_ATTN = struct.Struct("@" + _POOL + _POOL + "PqPqPPqPPqPiiiiiiiifPq")
+_SELECT = struct.Struct("@PqiiiiiPPiPPPPiPq")
+_REORDER = struct.Struct("@PPqqqqqqqiiiiP")
+_NO_POOL = (0,) * 9
+_raw_stream, _current = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
 
-def _need(ok, msg):
-    if not ok:
-        raise ValueError(msg)
+
+def _bad(msg):
+    raise ValueError(msg)
 
 
-def _on_device(who, first, *rest):
-    """Every tensor on the current device, where the launch goes."""
-    d = first.device
+def _launch(who, name, desc, first, *rest):
+    """Every tensor on the current device, where the launch goes; then the call on its current stream."""
+    d = first.get_device()
     for t in rest:
-        if t is not None and t.device != d:
-            raise RuntimeError(f"{who}: tensors on {d} and {t.device}")
-    if d.type != "cuda":
+        if t is not None and t.get_device() != d:
+            raise RuntimeError(f"{who}: tensors on {first.device} and {t.device}")
+    if d < 0:
         raise RuntimeError(f"{who}: SimLingo MI355X kernels need device tensors (no CPU fallback)")
-    if d.index != torch.cuda.current_device():
-        raise RuntimeError(f"{who}: tensors on {d}, current device cuda:{torch.cuda.current_device()}")
+    if d != _current():
+        raise RuntimeError(f"{who}: tensors on cuda:{d}, current device cuda:{torch.cuda.current_device()}")
+    rc = getattr(K.lib(), name)(desc() if callable(desc) else desc, _raw_stream(d))
+    if rc:
+        K.check(rc, name)
 
 
-def _i32(who, name, t, shape):
-    _need(t.dtype is I32 and t.shape == shape and t.is_contiguous(), f"{who}: {name} must be contiguous int32 {list(shape)}")
+def _i32(who, name, t, n):
+    if not (t.dtype is I32 and t.dim() == 1 and t.shape[0] == n and t.is_contiguous()):
+        _bad(f"{who}: {name} must be contiguous int32 [{n}]")
 
 
-def _rows(who, name, t, cols):
-    """A bf16 matrix view whose rows are contiguous and 16-B aligned -> its row stride."""
-    _need(t.dtype is BF16 and t.dim() == 2 and t.shape[1] >= cols, f"{who}: {name} must be bf16 [rows, >= {cols}]")
-    s0, s1 = t.stride()
-    _need(s1 == 1 and s0 % 8 == 0 and t.data_ptr() % 16 == 0, f"{who}: rows of {name} must be contiguous and 16-B aligned")
-    return s0
+def _rows(who, name, t, n, cols):
+    """A bf16 matrix view of n rows that are contiguous and 16-B aligned -> its address and row stride."""
+    if t.dtype is not BF16 or t.dim() != 2:
+        _bad(f"{who}: {name} must be a bf16 matrix")
+    (m, c), (s0, s1), p = t.shape, t.stride(), t.data_ptr()
+    if m != n or c < cols:
+        _bad(f"{who}: {name} must have {n} rows of at least {cols}, got {m} x {c}")
+    if s1 != 1 or s0 % 8 or p % 16:
+        _bad(f"{who}: rows of {name} must be contiguous and 16-B aligned")
+    return p, s0
 
 
 def _pool(who, k, v, written=False):
-    """slx_kv_pool of a cache k, v [pages, page, heads, head size]."""
-    _need(k.dtype is BF16 and v.dtype is BF16 and k.dim() == 4, f"{who}: k and v must be bf16 [pages, page, heads, head size]")
-    st, sh = k.stride(), k.shape
-    _need(sh == v.shape and st == v.stride(), f"{who}: k and v must have the same shape and strides")
+    """The fields of slx_kv_pool for a cache k, v [pages, page, heads, head size]."""
+    sh, st = k.shape, k.stride()
+    if k.dtype is not BF16 or v.dtype is not BF16 or len(sh) != 4:
+        _bad(f"{who}: k and v must be bf16 [pages, page, heads, head size]")
+    if sh != v.shape or st != v.stride():
+        _bad(f"{who}: k and v must have the same shape and strides")
     n, page, heads, d = sh
-    _need(n > 0 and page > 0 and page & (page - 1) == 0 and heads > 0 and (d == 64 or d == 128),
-          f"{who}: pages and heads > 0, page a power of two, head size 64 or 128 (got {list(sh)})")
+    s0, s1, s2, s3 = st
+    if not (n > 0 and page > 0 and page & (page - 1) == 0 and heads > 0 and (d == 64 or d == 128)):
+        _bad(f"{who}: pages and heads > 0, page a power of two, head size 64 or 128 (got {list(sh)})")
     kp, vp = k.data_ptr(), v.data_ptr()
-    _need(st[3] == 1 and (st[0] | st[1] | st[2]) % 8 == 0 and (kp | vp) % 16 == 0,
-          f"{who}: heads of k and v must be contiguous and 16-B aligned")
-    if written:
-        _need(all(s or m == 1 for s, m in zip(st, sh)), f"{who}: k and v must not be expanded")
-    return KVPoolDesc(kp, vp, st[0], st[1], st[2], n, page, heads, d)
+    if s3 != 1 or (s0 | s1 | s2) % 8 or (kp | vp) % 16:
+        _bad(f"{who}: heads of k and v must be contiguous and 16-B aligned")
+    if written and not ((s0 or n == 1) and (s1 or page == 1) and (s2 or heads == 1)):
+        _bad(f"{who}: k and v must not be expanded")
+    return kp, vp, s0, s1, s2, n, page, heads, d
 
 
 def _table(who, name, t):
-    _need(t.dtype is I32 and t.dim() == 2 and t.shape[1] > 0 and t.stride(1) == 1, f"{who}: {name} must be int32 [sequences, columns], rows contiguous")
-    # rows of a one-row table may have any stride
-    return max(t.stride(0), t.shape[1])
+    """Address, row stride, rows and columns of a page table."""
+    if t.dtype is not I32 or t.dim() != 2:
+        _bad(f"{who}: {name} must be int32 [sequences, columns]")
+    (n, cols), (s0, s1) = t.shape, t.stride()
+    if cols < 1 or s1 != 1 and cols > 1 or s0 < cols and n > 1:
+        _bad(f"{who}: {name} must have columns, its rows contiguous and apart")
+    return t.data_ptr(), max(s0, cols), n, cols
 
 
 def kv_append(qkv, k, v, table, pos, q_out=None, *, n_heads, cos=None, sin=None, seq=None, rows_per_seq=1):
@@ -129,32 +153,47 @@ def kv_append(qkv, k, v, table, pos, q_out=None, *, n_heads, cos=None, sin=None,
     A row with pos < 0, or one that names no slot (behind the table or the rotation's rows, a sequence or page that there
     is not), is padding: nothing of it is written. Two rows of one call must not name the same slot."""
     who = "kv_append"
-    pool = _pool(who, k, v, written=True)
-    hkv, d = pool.heads, pool.head_dim
-    _need(n_heads >= 0 and (q_out is None or n_heads > 0), f"{who}: n_heads")
+    pool = _pool(who, k, v, True)
+    hkv, d = pool[7], pool[8]
+    if n_heads < 0 or (q_out is not None and n_heads == 0):
+        _bad(f"{who}: n_heads {n_heads}")
     rows = qkv.shape[0]
-    ld = _rows(who, "qkv", qkv, (n_heads + 2 * hkv) * d)
-    ldt = _table(who, "table", table)
-    _need(table.shape[0] > 0 and rows_per_seq > 0, f"{who}: an empty table, or rows_per_seq < 1")
-    _i32(who, "pos", pos, (rows,))
+    x, ldx = _rows(who, "qkv", qkv, rows, (n_heads + 2 * hkv) * d)
+    tab, ldt, n_seq, cols = _table(who, "table", table)
+    if n_seq < 1 or rows_per_seq < 1:
+        _bad(f"{who}: an empty table, or rows_per_seq < 1")
+    _i32(who, "pos", pos, rows)
     if seq is not None:
-        _i32(who, "seq", seq, (rows,))
-    ldq = 0
-    if q_out is not None:
-        ldq = _rows(who, "q_out", q_out, n_heads * d)
-        _need(q_out.shape[0] == rows, f"{who}: q_out has {q_out.shape[0]} rows, qkv {rows}")
-    rope = 0
-    _need((cos is None) == (sin is None), f"{who}: cos and sin go together")
-    if cos is not None:
-        rope = cos.shape[0]
-        for t in (cos, sin):
-            _need(t.dtype is F32 and t.shape == (rope, d // 2) and t.is_contiguous() and rope > 0 and t.data_ptr() % 16 == 0,
-                  f"{who}: cos and sin must be contiguous f32 [positions, {d // 2}]")
-    _on_device(who, qkv, k, v, table, pos, q_out, cos, sin, seq)
-    desc = KVAppendDesc(pool, qkv.data_ptr(), ld, q_out.data_ptr() if q_out is not None else 0, ldq, table.data_ptr(), ldt,
-                        table.shape[0], table.shape[1], seq.data_ptr() if seq is not None else 0, pos.data_ptr(), rows_per_seq,
-                        n_heads, rows, cos.data_ptr() if rope else 0, sin.data_ptr() if rope else 0, rope)
-    K.check(K.lib().slx_kv_append(ctypes.byref(desc), K.stream_ptr()), "slx_kv_append")
+        _i32(who, "seq", seq, rows)
+    q, ldq = _rows(who, "q_out", q_out, rows, n_heads * d) if q_out is not None else (0, 0)
+    c = s = rope = 0
+    if cos is None or sin is None:
+        if cos is not sin:
+            _bad(f"{who}: cos and sin go together")
+    else:
+        rope, c, s = cos.shape[0], cos.data_ptr(), sin.data_ptr()
+        if not (cos.dtype is F32 and sin.dtype is F32 and cos.dim() == 2 and cos.shape[1] == d // 2 and sin.shape == cos.shape and rope > 0
+                and cos.is_contiguous() and sin.is_contiguous() and (c | s) % 16 == 0):
+            _bad(f"{who}: cos and sin must be contiguous f32 [positions, {d // 2}]")
+    desc = _APPEND.pack(*pool, x, ldx, q, ldq, tab, ldt, n_seq, cols, seq.data_ptr() if seq is not None else 0, pos.data_ptr(),
+                        rows_per_seq, n_heads, rows, c, s, rope)
+    _launch(who, "slx_kv_append", desc, qkv, k, v, table, pos, q_out, cos, sin, seq)
+
+
+@functools.lru_cache(maxsize=1024)
+def _attn_ws(ppool, opool, ptab, pmax, omax, pcols, ocols, groups, width, n_q, n_heads):
+    """Floats of workspace for these sizes (the C entry's own rule; no address goes into it)."""
+    need = K.lib().slx_prefix_attn_ws_floats(_ATTN.pack(*_fake(ppool), *_fake(opool), 0, 0, 0, 0, 0, ptab, pcols, ptab, 0, ocols, 0, pmax, omax,
+                                                        pcols, ocols, groups, width, n_q, n_heads, 1.0, 0, 0))
+    if need < 0:
+        K.check(need, "slx_prefix_attn")
+    return need
+
+
+def _fake(pool):
+    """slx_kv_pool's fields from its sizes alone."""
+    n, page, heads, d = pool
+    return (16, 16, 0, 0, 0, n, page, heads, d) if n else _NO_POOL
 
 
 def prefix_attn(q, out=None, *, own, prefix=None, n_heads, n_q=1, scale=None, max_own=None, max_prefix=None, lse=None):
@@ -162,56 +201,57 @@ def prefix_attn(q, out=None, *, own, prefix=None, n_heads, n_q=1, scale=None, ma
     tokens' among them as the last; prefix = (k, v, table [G, columns], lengths [G]): keys that sequences g * N/G ...
     share, before their own. q rows [N * n_q, n_heads * head size], a sequence's tokens together, already rotated; the
     kv heads are the caches'. Token t sees the whole prefix and own keys up to length - n_q + t; a row without any key
-    gives zeros. scale: 1 / sqrt(head size) by default. max_own, max_prefix: bounds of the lengths where they are known
+    gives zeros. scale > 0: 1 / sqrt(head size) by default. max_own, max_prefix: bounds of the lengths where they are known
     to be lower than the tables' columns (longer ones are cut to them); the split of the work goes by them.
     Keys on a page number outside the cache are masked. lse: optional f32 [N * n_q, n_heads], natural log of the softmax
     sum (-inf without keys). Returns out (bf16, like q)."""
     who = "prefix_attn"
     ok, ov, otab, olen = own
     opool = _pool(who, ok, ov)
-    d = opool.head_dim
-    n = otab.shape[0]
-    _need(n_heads > 0 and n_heads % opool.heads == 0, f"{who}: n_heads must be a multiple of the cache's {opool.heads} heads")
-    _need(n_q > 0 and q.dim() == 2 and q.shape[0] == n * n_q, f"{who}: q must have {n} x {n_q} rows")
-    ldq = _rows(who, "q", q, n_heads * d)
-    ldot = _table(who, "own table", otab)
-    _i32(who, "own lengths", olen, (n,))
-    groups = n
-    ppool, ptab, ldpt, plen, pcols, pmax = KVPoolDesc(), None, 0, None, 0, 0
-    pk = pv = None
+    heads, d = opool[7], opool[8]
+    ot, ldot, n, ocols = _table(who, "own table", otab)
+    if n_heads < 1 or n_heads % heads:
+        _bad(f"{who}: n_heads must be a multiple of the cache's {heads} heads")
+    if n_q < 1:
+        _bad(f"{who}: n_q {n_q}")
+    scale = d ** -0.5 if scale is None else scale
+    if not 0 < scale < math.inf:
+        _bad(f"{who}: scale must be positive")
+    rows, cols = n * n_q, n_heads * d
+    x, ldq = _rows(who, "q", q, rows, cols)
+    _i32(who, "own lengths", olen, n)
+    ppool, pk, pv, ptab, plen, pt, ldpt, groups, pcols, pmax, pl = _NO_POOL, None, None, None, None, 0, 0, n, 0, 0, 0
     if prefix is not None:
         pk, pv, ptab, plen = prefix
         ppool = _pool(who, pk, pv)
-        _need(ppool.heads == opool.heads and ppool.head_dim == d, f"{who}: the two caches differ in heads or head size")
-        ldpt = _table(who, "prefix table", ptab)
-        groups, pcols = ptab.shape
-        _i32(who, "prefix lengths", plen, (groups,))
-        _need(groups > 0 and n % groups == 0, f"{who}: {n} sequences do not make {groups} groups of one size")
-        pmax = min(pcols * ppool.page, 2**31 - 1) if max_prefix is None else max_prefix
-    omax = min(otab.shape[1] * opool.page, 2**31 - 1) if max_own is None else max_own
-    _need(omax >= 0 and pmax >= 0, f"{who}: bounds must not be negative")
+        if ppool[7] != heads or ppool[8] != d:
+            _bad(f"{who}: the two caches differ in heads or head size")
+        pt, ldpt, groups, pcols = _table(who, "prefix table", ptab)
+        _i32(who, "prefix lengths", plen, groups)
+        if groups < 1 or n % groups:
+            _bad(f"{who}: {n} sequences do not make {groups} groups of one size")
+        pl = plen.data_ptr()
+        pmax = min(pcols * ppool[6], 2**31 - 1) if max_prefix is None else max_prefix
+    omax = min(ocols * opool[6], 2**31 - 1) if max_own is None else max_own
+    if not (0 <= omax < 2**31 and 0 <= pmax < 2**31):
+        _bad(f"{who}: bounds must be 0 .. 2^31 - 1")
     if out is None:
-        out = torch.empty(q.shape[0], n_heads * d, dtype=BF16, device=q.device)
-    ldo = _rows(who, "out", out, n_heads * d)
-    _need(out.shape[0] == q.shape[0], f"{who}: out has {out.shape[0]} rows, q {q.shape[0]}")
-    if lse is not None:
-        _need(lse.dtype is F32 and lse.shape == (q.shape[0], n_heads) and lse.is_contiguous(),
-              f"{who}: lse must be contiguous f32 [{q.shape[0]}, {n_heads}]")
-    _on_device(who, q, ok, ov, otab, olen, out, pk, pv, ptab, plen, lse)
-    if n == 0:
-        return out
-    desc = PrefixAttnDesc(ppool, opool, q.data_ptr(), ldq, out.data_ptr(), ldo, lse.data_ptr() if lse is not None else 0,
-                          ptab.data_ptr() if ptab is not None else 0, ldpt, plen.data_ptr() if plen is not None else 0,
-                          otab.data_ptr(), ldot, olen.data_ptr(), pmax, omax, pcols, otab.shape[1], groups, n // groups, n_q,
-                          n_heads, 1.0 / math.sqrt(d) if scale is None else scale, 0, 0)
-    lib = K.lib()
-    need = lib.slx_prefix_attn_ws_floats(ctypes.byref(desc))
-    if need < 0:
-        K.check(need, "slx_prefix_attn")
-    if need:
-        ws = torch.empty(need, dtype=F32, device=q.device)  # of this call alone, from the current stream's pool
-        desc.ws, desc.ws_floats = ws.data_ptr(), need
-    K.check(lib.slx_prefix_attn(ctypes.byref(desc), K.stream_ptr()), "slx_prefix_attn")
+        out = torch.empty(rows, cols, dtype=BF16, device=q.device)
+    o, ldo = _rows(who, "out", out, rows, cols)
+    if lse is not None and not (lse.dtype is F32 and lse.shape == (rows, n_heads) and lse.is_contiguous()):
+        _bad(f"{who}: lse must be contiguous f32 [{rows}, {n_heads}]")
+    ws = None
+
+    def desc():  # after the device checks: the workspace is of this call alone, from the current stream's memory
+        nonlocal ws
+        need = _attn_ws(ppool[5:], opool[5:], 16 if pt else 0, pmax, omax, pcols, ocols, groups, n // groups, n_q, n_heads)
+        ws = torch.empty(need, dtype=F32, device=q.device) if need else None
+        return _ATTN.pack(*ppool, *opool, x, ldq, o, ldo, lse.data_ptr() if lse is not None else 0, pt, ldpt, pl, ot, ldot, olen.data_ptr(),
+                          pmax, omax, pcols, ocols, groups, n // groups, n_q, n_heads, scale,
+                          ws.data_ptr() if need else 0, need)
+
+    if n:
+        _launch(who, "slx_prefix_attn", desc, q, ok, ov, otab, olen, out, pk, pv, ptab, plen, lse)
     return out
 
 
@@ -225,41 +265,60 @@ def beam_select(logits, scores, *, width, k=None, finished=None, pad_id=0, eos_i
     `scores` itself if k == width). finished_out [batch, k], with eos_id: finished[parent] or token == eos_id."""
     who = "beam_select"
     k = width if k is None else k
-    _need(0 < width <= MAX_WIDTH and 0 < k <= MAX_K, f"{who}: width and k must be 1 .. {MAX_WIDTH}")
-    _need(logits.dim() == 2 and logits.dtype in (F32, BF16) and logits.stride(1) == 1, f"{who}: logits must be f32 or bf16 [rows, V], rows contiguous")
-    n, vocab = logits.shape
-    _need(0 < vocab <= MAX_VOCAB and n % width == 0 and k <= width * vocab, f"{who}: 1 .. {MAX_VOCAB} logits a row, rows a multiple of width, k <= width * V")
+    if not (0 < width <= MAX_WIDTH and 0 < k <= MAX_K):
+        _bad(f"{who}: width and k must be 1 .. {MAX_WIDTH}")
+    bf = logits.dtype is BF16
+    if logits.dim() != 2 or not (bf or logits.dtype is F32):
+        _bad(f"{who}: logits must be f32 or bf16 [rows, V]")
+    (n, vocab), (ldx, s1) = logits.shape, logits.stride()
+    if s1 != 1 and vocab > 1 or ldx < vocab and n > 1:
+        _bad(f"{who}: rows of logits must be contiguous and apart")
+    if not (0 < vocab <= MAX_VOCAB and n % width == 0 and k <= width * vocab):
+        _bad(f"{who}: 1 .. {MAX_VOCAB} logits a row, rows a multiple of width, k <= width * V")
     b = n // width
-    _need(scores.dtype is F32 and scores.numel() == n and scores.is_contiguous(), f"{who}: scores must be contiguous f32 [{n}]")
+    if not (scores.dtype is F32 and scores.numel() == n and scores.is_contiguous()):
+        _bad(f"{who}: scores must be contiguous f32 [{n}]")
+    sp, fp, fo = scores.data_ptr(), 0, 0
     if finished is not None:
-        _need(finished.dtype in (torch.bool, torch.uint8) and finished.numel() == n and finished.is_contiguous(), f"{who}: finished must be contiguous bool [{n}]")
-        _need(0 <= pad_id < vocab, f"{who}: pad_id outside the vocabulary")
+        if not (finished.dtype in (torch.bool, torch.uint8) and finished.numel() == n and finished.is_contiguous()):
+            _bad(f"{who}: finished must be contiguous bool [{n}]")
+        if not 0 <= pad_id < vocab:
+            _bad(f"{who}: pad_id outside the vocabulary")
+        fp = finished.data_ptr()
     if finished_out is not None:
-        _need(finished_out.dtype in (torch.bool, torch.uint8) and finished_out.numel() == b * k and finished_out.is_contiguous(),
-              f"{who}: finished_out must be contiguous bool [{b}, {k}]")
+        if not (finished_out.dtype in (torch.bool, torch.uint8) and finished_out.numel() == b * k and finished_out.is_contiguous()):
+            _bad(f"{who}: finished_out must be contiguous bool [{b}, {k}]")
+        fo = finished_out.data_ptr()
     if out is None:
-        dev = logits.device
-        out = (torch.empty(b, k, dtype=F32, device=dev), torch.empty(b, k, dtype=I32, device=dev), torch.empty(b, k, dtype=I32, device=dev))
-    else:
-        for t, dt in zip(out, (F32, I32, I32)):
-            _need(t.dtype is dt and t.numel() == b * k and t.is_contiguous(), f"{who}: out must be contiguous f32, int32, int32 [{b}, {k}]")
-    for t, given, what in ((out[0], scores, "scores"), (finished_out, finished, "finished")):
-        _need(t is None or given is None or t.data_ptr() != given.data_ptr() or k == width, f"{who}: {what} in place needs k == width")
-    _on_device(who, logits, scores, finished, finished_out, *out)
-    if b == 0:
-        return out
-    desc = BeamSelectDesc(logits.data_ptr(), max(logits.stride(0), vocab), int(logits.dtype is BF16), b, width, vocab, k, scores.data_ptr(),
-                          finished.data_ptr() if finished is not None else 0, pad_id, out[0].data_ptr(), out[1].data_ptr(),
-                          out[2].data_ptr(), finished_out.data_ptr() if finished_out is not None else 0,
-                          -1 if eos_id is None else eos_id, 0, 0)
-    lib = K.lib()
-    need = lib.slx_beam_select_ws_bytes(ctypes.byref(desc))
+        to = torch.empty(3, b, k, dtype=I32, device=logits.device)
+        out = to[0].view(F32), to[1], to[2]
+    s_out, p_out, t_out = out
+    if not (s_out.dtype is F32 and p_out.dtype is I32 and t_out.dtype is I32 and s_out.numel() == p_out.numel() == t_out.numel() == b * k
+            and s_out.is_contiguous() and p_out.is_contiguous() and t_out.is_contiguous()):
+        _bad(f"{who}: out must be contiguous f32, int32, int32 [{b}, {k}]")
+    so = s_out.data_ptr()
+    if k != width and n and (so == sp or fo and fo == fp):
+        _bad(f"{who}: scores or finished in place need k == width")
+    ws = None
+
+    def desc():
+        nonlocal ws
+        need = _select_ws(b, width, vocab, k)
+        ws = torch.empty(need, dtype=torch.uint8, device=logits.device)  # of this call alone, from the current stream's memory
+        return _SELECT.pack(logits.data_ptr(), max(ldx, vocab), bf, b, width, vocab, k, sp, fp, pad_id if fp else 0, so, p_out.data_ptr(),
+                            t_out.data_ptr(), fo, -1 if eos_id is None else eos_id, ws.data_ptr(), need)
+
+    if b:
+        _launch(who, "slx_beam_select", desc, logits, scores, finished, finished_out, s_out, p_out, t_out)
+    return out
+
+
+@functools.lru_cache(maxsize=1024)
+def _select_ws(b, width, vocab, k):
+    need = K.lib().slx_beam_select_ws_bytes(_SELECT.pack(0, vocab, 0, b, width, vocab, k, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0))
     if need < 0:
         K.check(need, "slx_beam_select")
-    ws = torch.empty(need, dtype=torch.uint8, device=logits.device)  # of this call alone, from the current stream's pool
-    desc.ws, desc.ws_bytes = ws.data_ptr(), need
-    K.check(lib.slx_beam_select(ctypes.byref(desc), K.stream_ptr()), "slx_beam_select")
-    return out
+    return need
 
 
 def _span(t):
@@ -273,37 +332,44 @@ def beam_reorder(x, parent, *, dim=0, out=None):
     strided as long as they make at most two runs of rows. A parent outside 0 .. W - 1 stands for w itself.
     Returns out."""
     who = "beam_reorder"
-    out = x if out is None else out
-    _need(parent.dtype is I32 and parent.dim() == 2 and parent.is_contiguous(), f"{who}: parent must be contiguous int32 [batch, W]")
+    if parent.dtype is not I32 or parent.dim() != 2 or not parent.is_contiguous():
+        _bad(f"{who}: parent must be contiguous int32 [batch, W]")
     b, w = parent.shape
-    _need(0 < w <= MAX_WIDTH, f"{who}: W must be 1 .. {MAX_WIDTH}")
-    _need(-x.dim() <= dim < x.dim() and x.shape == out.shape and x.dtype is out.dtype, f"{who}: dim, or out unlike x")
-    dim %= x.dim()
-    _need(x.shape[dim] == b * w, f"{who}: dimension {dim} of x has {x.shape[dim]} rows, parent {b} x {w}")
-    if x.numel() == 0:
-        return out
-    es, ss, ds = x.element_size(), x.stride(), out.stride()
-    run, outer = 1, []  # a row's contiguous elements; the other dimensions (extent, stride in x, stride in out), inner first
-    for i in range(x.dim() - 1, -1, -1):
-        m = x.shape[i]
+    if not 0 < w <= MAX_WIDTH:
+        _bad(f"{who}: W must be 1 .. {MAX_WIDTH}")
+    if out is None:
+        out = x
+    sh, ss, ds, nd = x.shape, x.stride(), out.stride(), x.dim()
+    if not -nd <= dim < nd or sh != out.shape or x.dtype is not out.dtype:
+        _bad(f"{who}: dim, or out unlike x")
+    dim %= nd
+    if sh[dim] != b * w:
+        _bad(f"{who}: dimension {dim} of x has {sh[dim]} rows, parent {b} x {w}")
+    es, run, outer, empty = x.element_size(), 1, [], False
+    for i in range(nd - 1, -1, -1):  # a row's contiguous elements; the other dimensions (extent, stride in x, in out), inner first
+        m, s, t = sh[i], ss[i], ds[i]
+        empty = empty or m == 0
         if i == dim or m == 1:
             continue
-        if not outer and ss[i] == ds[i] == run:
+        if not outer and s == t == run:
             run *= m
-        elif outer and ss[i] == outer[-1][0] * outer[-1][1] and ds[i] == outer[-1][0] * outer[-1][2]:
+        elif outer and s == outer[-1][0] * outer[-1][1] and t == outer[-1][0] * outer[-1][2]:
             outer[-1] = (outer[-1][0] * m, outer[-1][1], outer[-1][2])
         else:
-            outer.append((m, ss[i], ds[i]))
-    _need(len(outer) <= 2, f"{who}: the state's strides make more than two runs of rows")
-    _need(all(s for m, _, s in outer) and (ds[dim] or b * w == 1), f"{who}: out must not be expanded")
-    same = x.data_ptr() == out.data_ptr()
-    if not same or ss != ds:
+            outer.append((m, s, t))
+    if empty:
+        return out
+    if len(outer) > 2:
+        _bad(f"{who}: the state's strides make more than two runs of rows")
+    if any(not t for _, _, t in outer) or (not ds[dim] and b * w > 1):
+        _bad(f"{who}: out must not be expanded")
+    xp, op = x.data_ptr(), out.data_ptr()
+    if xp != op or ss != ds:
         (a0, a1), (c0, c1) = _span(x), _span(out)
-        _need(a1 <= c0 or c1 <= a0, f"{who}: out overlaps x")
-    _on_device(who, x, out, parent)
-    outer += [(1, 0, 0)] * (2 - len(outer))
-    (n1, s1, d1), (n0, s0, d0) = outer
-    desc = BeamReorderDesc(x.data_ptr(), out.data_ptr(), s0 * es, s1 * es, ss[dim] * es, d0 * es, d1 * es, ds[dim] * es, run * es,
-                           n0, n1, b, w, parent.data_ptr())
-    K.check(K.lib().slx_beam_reorder(ctypes.byref(desc), K.stream_ptr()), "slx_beam_reorder")
+        if a0 < c1 and c0 < a1:
+            _bad(f"{who}: out overlaps x")
+    outer += ((1, 0, 0), (1, 0, 0))
+    (n1, s1, d1), (n0, s0, d0) = outer[:2]
+    desc = _REORDER.pack(xp, op, s0 * es, s1 * es, ss[dim] * es, d0 * es, d1 * es, ds[dim] * es, run * es, n0, n1, b, w, parent.data_ptr())
+    _launch(who, "slx_beam_reorder", desc, x, out, parent)
     return out

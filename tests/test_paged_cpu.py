@@ -70,7 +70,7 @@ def attn_args(**kw):
     dict(own=dict(_2=torch.zeros(4, 3))), dict(own=dict(_2=torch.zeros(4, 0, dtype=I32))), dict(own=dict(_3=torch.zeros(3, dtype=I32))), dict(own=dict(_0=pool(n=3)[0])),
     dict(prefix=dict(_2=torch.zeros(3, 3, dtype=I32), _3=torch.zeros(3, dtype=I32))), dict(prefix=dict(_3=torch.zeros(2, dtype=torch.int64))),
     dict(prefix=dict(_0=pool(heads=1)[0], _1=pool(heads=1)[1])), dict(prefix=dict(_0=pool(d=128)[0], _1=pool(d=128)[1])),
-    dict(max_own=-1), dict(max_prefix=-1), dict(out=torch.zeros(4, 192, dtype=BF16)), dict(out=torch.zeros(5, 256, dtype=BF16)), dict(lse=torch.zeros(4, 3)),
+    dict(max_own=-1), dict(max_prefix=-1), dict(scale=0.0), dict(scale=-1.0), dict(scale=float("nan")), dict(out=torch.zeros(4, 192, dtype=BF16)), dict(out=torch.zeros(5, 256, dtype=BF16)), dict(lse=torch.zeros(4, 3)),
 ], ids=lambda kw: "-".join(kw))
 def test_prefix_attn_refuses(kw):
     with pytest.raises(ValueError, match="prefix_attn"):
@@ -137,7 +137,7 @@ def test_c_entries_refuse():
     pre = dict(prefix_pool=good, ptab=4096, ldpt=64, plen=4096, max_prefix=512, pcols=64)
     for kw, text in ((dict(Hq=3), b"multiple"), (dict(width=0), b"width"), (dict(n_q=0), b"n_q"), (dict(ocols=3), b"ocols"), (dict(max_own=-1), b"max_own"), (dict(q=0), b"null"),
                      (dict(q=4104), b"16-B"), (dict(ldo=12), b"16-B"), ({**pre, "plen": 0}, b"plen"), ({**pre, "ldpt": 3}, b"pcols"), (pre, b"workspace"),
-                     (dict(groups=1 << 20, width=1 << 10, n_q=4), b"too many")):
+                     (dict(groups=1 << 20, width=1 << 10, n_q=4), b"too many"), (dict(scale=0.0), b"scale"), (dict(Hq=1 << 14, width=64), b"too many")):
         refused("slx_prefix_attn", PG.PrefixAttnDesc(**{**at, **kw}), text)
     other = PG.KVPoolDesc.from_buffer_copy(good)
     other.heads = 1

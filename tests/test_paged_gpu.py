@@ -175,6 +175,18 @@ ATTN = [  # heads, kv heads, d, groups, width, n_q, prefixes, page, own lengths,
     (2, 1, 64, 2, 2, 40, [64, 5], 8, [40, 47, 100, 41], 16, "slots"),
     (8, 1, 128, 1, 2, 5, [19], 1, [5, 70], 2, "slots"),
     (16, 1, 64, 1, 2, 3, [200], 128, [3, 4], 32, "slots"),
+    # more rows than a wave holds: tiles shared by the workgroup
+    (14, 2, 64, 1, 8, 1, [1], 8, [1] * 8, 8, "slots"),
+    (14, 2, 64, 2, 7, 1, [127, 300], 8, [5] * 14, 16, "heads"),
+    (14, 2, 64, 1, 40, 1, [161], 64, [2] * 40, 1, "pair"),
+    (32, 8, 128, 1, 12, 1, [419], 8, [9] * 12, 16, "slots"),
+    (32, 8, 128, 2, 19, 1, [33, 290], 32, [3] * 38, 4, "pair"),
+    (8, 2, 128, 1, 2, 21, [77], 16, [21, 150], 8, "heads"),
+    (14, 2, 64, 1, 2, 6, [0], 16, [6, 333], 32, "slots"),
+    (4, 1, 64, 1, 1, 37, None, 0, [300], 16, "slots"),
+    (3, 3, 64, 1, 2, 50, [64], 16, [50, 20], 16, "slots"),
+    (5, 1, 128, 1, 3, 13, [40], 64, [13, 14, 64], 8, "slots"),
+    (16, 1, 128, 1, 2, 20, [9], 2, [25, 40], 64, "slots"),
 ]
 
 
@@ -240,12 +252,41 @@ def test_prefix_attn_masked_values(dev):
     assert torch.isnan(got.view(2, 3, 14, 64)[1, 2, :7, 5]).all() and (got.view(2, 3, 14, 64)[1, 2, 7:, 9] == -float("inf")).all()
 
 
+def test_prefix_attn_masked_values_many_rows(dev):
+    """The same with tiles that a workgroup shares: garbage behind the lengths, non-finite values in keys seen by some rows."""
+    for d, hq, hkv in ((64, 14, 2), (128, 8, 2)):
+        q, own, prefix = case(17, hq, hkv, d, 1, 2, 24, [41], 16, [30, 90], 8)
+        for kv, lens in ((own, [30, 90]), (prefix, [41])):
+            used = torch.zeros(kv[0].shape[:2], dtype=torch.bool)
+            for i, n in enumerate(lens):
+                for j in range(n):
+                    used[kv[2][i, j // kv[0].shape[1]], j % kv[0].shape[1]] = True
+            kv[0][~used] = float("nan")
+            kv[1][~used] = float("nan")
+        clean = check(dev, q, own, prefix, hq, 24).view(2, 24, hq, d)
+        for i, key, head, at, val in ((0, 29, 0, 5, float("nan")), (1, 80, 1, 9, float("inf")), (1, 70, 0, d - 1, -float("inf"))):
+            own[1][own[2][i, key // 8], key % 8, head, at] = val
+        got = run(dev, q, own, prefix, hq, 24)[0].view(2, 24, hq, d)
+        r = hq // hkv
+        bad = torch.zeros_like(got, dtype=torch.bool)
+        for i, key, head, at, val, n in ((0, 29, 0, 5, float("nan"), 30), (1, 80, 1, 9, float("inf"), 90), (1, 70, 0, d - 1, -float("inf"), 90)):
+            part = got[i, key - (n - 24):, head * r:(head + 1) * r, at]
+            assert torch.isnan(part).all() if val != val else (part == val).all()
+            bad[i, key - (n - 24):, head * r:(head + 1) * r, at] = True
+        assert torch.equal(got[~bad], clean[~bad])
+
+
 def test_prefix_attn_bad_pages(dev):
     """Keys on page numbers outside the cache are masked, in both caches and at every page size."""
     for ppage, opage in ((16, 8), (64, 1), (2, 32)):
         q, own, prefix = case(7, 4, 2, 64, 1, 3, 1, [150], ppage, [40, 9, 70], opage)
         own[2][0, 0], own[2][2, -1], prefix[2][0, 1] = -1, own[0].shape[0], 2**31 - 1
         check(dev, q, own, prefix, 4, 1)
+    for d, hq, hkv, n_q in ((64, 14, 2, 1), (128, 8, 2, 20)):
+        q, own, prefix = case(18, hq, hkv, d, 1, 9, n_q, [290], 8, [40] * 9, 8)
+        own[2][0, 0], own[2][2, -1], prefix[2][0, 1], prefix[2][0, 30] = -1, own[0].shape[0], 2**31 - 1, -2**31
+        check(dev, q, own, prefix, hq, n_q)
+    q, own, prefix = case(7, 4, 2, 64, 1, 3, 1, [150], 2, [40, 9, 70], 32)
     own[2].fill_(-1)
     prefix[2].fill_(-7)
     assert not check(dev, q, own, prefix, 4, 1).any()
