@@ -14,17 +14,16 @@ namespace slx {
 
 typedef unsigned long long u64;
 typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
-constexpr int kSelE = 16;                // logits a thread
-constexpr int kSelChunk = 256 * kSelE;   // columns a workgroup
+constexpr int kSelChunk = 4096;          // columns a workgroup at least: 16 a thread
 constexpr int kSelMaxChunks = 64;        // one lane each in the second launch
 constexpr int kSelMaxK = 64, kSelMaxW = 64;
-constexpr int kSelList = 256;            // candidates of a chunk that are ranked at once
+constexpr int kSelList = 256;            // candidates of a chunk, or of a row's lists, that are ranked at once
 
 struct SelArgs {
   const void* x; long ldx;
   const float* score; const unsigned char* fin;
   float* score_out; int *parent, *token; unsigned char* fin_out;
-  int B, W, V, K, C, pad, eos;
+  int B, W, V, K, C, pad, eos;  // C: chunks a row
   float2* ml;  // [B * W][C] (max, sum)
   u64* keys;   // [B * W][C][K], descending; 0 = none
 };
@@ -61,82 +60,81 @@ __device__ __forceinline__ u64 wave_kmax(u64 k) {
   return ((u64)hi << 32) | lo;
 }
 
-template <typename T>
+// E columns a thread: 16, or 32 where the rows make workgroups enough (the threshold and the ranking are per workgroup).
+template <typename T, int E>
 __global__ __launch_bounds__(256) void beam_chunk_kernel(SelArgs a) {
   __shared__ float2 sml[4];
-  __shared__ unsigned stv[4];
+  __shared__ float stv[4];
   __shared__ int scount;
   __shared__ u64 list[kSelList];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int c = blockIdx.x, row = blockIdx.y;
+  constexpr int VEC = 16 / (int)sizeof(T), U = E / VEC, CHUNK = 256 * E;  // 16-B loads, VEC columns each
+  const T* xr = (const T*)a.x + (long)row * a.ldx;
+  const int c0 = c * CHUNK;
+  // a thread's columns rise with e, so those below V come first in its order: n of them
+  auto col = [&](int e) { return c0 + ((e / VEC) * 256 + tid) * VEC + e % VEC; };
+  float v[E];
+  int n = E;
   // rows that have ended, or are out of the search already, are not read
   const float s = a.score[row];
   if ((a.fin && a.fin[row]) || s == -INFINITY || s != s) return;
-  constexpr int VEC = 16 / (int)sizeof(T), U = kSelE / VEC;  // 16-B loads, VEC columns each
-  const T* xr = (const T*)a.x + (long)row * a.ldx;
-  const int c0 = c * kSelChunk;
-  auto col = [&](int e) { return c0 + ((e / VEC) * 256 + tid) * VEC + e % VEC; };
-  float v[kSelE];
-  int n = kSelE;  // this thread's columns (a prefix of its order in a full chunk; all or by column in the last)
-  if (c0 + kSelChunk <= a.V) {
+  if (c0 + CHUNK <= a.V) {
+    T t[U][VEC];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      T t[VEC];
-      __builtin_memcpy(t, xr + c0 + (u * 256 + tid) * VEC, 16);  // rows of odd length: any alignment of T
+    for (int u = 0; u < U; ++u) __builtin_memcpy(t[u], xr + c0 + (u * 256 + tid) * VEC, 16);  // rows of odd length: any alignment of T
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) v[u * VEC + j] = (float)t[j] + 0.f;  // -0 ties with 0
-    }
+    for (int e = 0; e < E; ++e) v[e] = (float)t[e / VEC][e % VEC];
   } else {
     n = 0;
 #pragma unroll
-    for (int e = 0; e < kSelE; ++e) {
+    for (int e = 0; e < E; ++e) {
       const bool in = col(e) < a.V;
-      v[e] = in ? (float)xr[col(e)] + 0.f : -INFINITY;
+      v[e] = in ? (float)xr[col(e)] : -INFINITY;
       n += in;
     }
   }
-  // ordered bits, 0 for what is not there; columns past V have no key
-  unsigned o[kSelE], om = 0;
-  float m = -INFINITY;
+  if (tid == 0) scount = 0;
+  float m = v[0];  // NaN stays out of the maximum, and makes the row's sum NaN, so that the row offers nothing
 #pragma unroll
-  for (int e = 0; e < kSelE; ++e) {
-    o[e] = ord_f(v[e]);
-    m = fmaxf(m, v[e]);
-  }
-  // a thread's columns below V come first in its order, so its n first are the ones that count
-#pragma unroll
-  for (int e = 0; e < kSelE; ++e) om = e < n ? max(om, o[e]) : om;
-  const unsigned top = wave_umax(n ? om : 0u);
-  const float mw = unord_f(wave_umax(ord_f(m)));
+  for (int e = 1; e < E; ++e) m = fmaxf(m, v[e]);
+  const unsigned om = ord_f(m);
+  const float mw = unord_f(wave_umax(om));
   const float ms = mw == -INFINITY ? 0.f : mw;
   float l = 0.f;
 #pragma unroll
-  for (int e = 0; e < kSelE; ++e) l += __expf(v[e] - ms);
+  for (int e = 0; e < E; ++e) l += __expf(v[e] - ms);
   l = warp_sum(l);
 
-  // a threshold with at least K of the chunk's columns at or above it: the lanes' own maxima, halved into from both ends
-  unsigned tv = 0;
+  // a threshold with at least K of the chunk's columns at or above it: among the lanes' own maxima, halved into from both ends
+  float tv = -INFINITY;
+  bool all = true;  // no threshold: every column is a candidate
   if (__popcll(__ballot(n > 0)) >= a.K) {
-    unsigned lo = ~wave_umax(~(n ? om : 0u)), hi = top;  // every lane is >= lo
+    unsigned lo = ~wave_umax(~(n ? om : 0u)), hi = wave_umax(n ? om : 0u);  // every lane with columns is >= lo
     for (int it = 0; it < 12 && lo < hi; ++it) {
       const unsigned mid = lo + (hi - lo) / 2 + 1;
       if (__popcll(__ballot(n > 0 && om >= mid)) >= a.K) lo = mid;
       else hi = mid - 1;
     }
-    tv = lo;
+    tv = unord_f(max(lo, 0x007FFFFFu));  // at least -inf
+    all = lo <= 0x007FFFFFu;
   }
   if (lane == 0) {
     sml[wave] = make_float2(mw, l);
-    stv[wave] = tv;
+    stv[wave] = all ? -INFINITY : tv;
   }
-  if (tid == 0) scount = 0;
   __syncthreads();
-  tv = max(max(stv[0], stv[1]), max(stv[2], stv[3]));
+  tv = fmaxf(fmaxf(stv[0], stv[1]), fmaxf(stv[2], stv[3]));
+  u64 hit = 0;
 #pragma unroll
-  for (int e = 0; e < kSelE; ++e) {
-    if (e < n && o[e] >= tv) {
-      const int at = atomicAdd(&scount, 1);
-      if (at < kSelList) list[at] = key_of(o[e], col(e));
+  for (int e = 0; e < E; ++e) hit |= (u64)(tv == -INFINITY || v[e] >= tv) << e;
+  hit &= n >= 64 ? ~0ull : (1ull << n) - 1;
+  if (hit) {
+    const int at = atomicAdd(&scount, __popcll(hit));
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const int i = at + __popcll(hit & ((1ull << e) - 1));
+      if ((hit >> e & 1) && i < kSelList) list[i] = key_of(ord_f(v[e] + 0.f), col(e));  // -0 ties with 0
     }
   }
   __syncthreads();
@@ -147,8 +145,8 @@ __global__ __launch_bounds__(256) void beam_chunk_kernel(SelArgs a) {
     for (int i = 0; i < a.K; ++i) {
       u64 best = 0;
 #pragma unroll
-      for (int e = 0; e < kSelE; ++e) {
-        const u64 k = key_of(o[e], col(e));
+      for (int e = 0; e < E; ++e) {
+        const u64 k = key_of(ord_f(v[e] + 0.f), col(e));
         if (e < n && k < last && k > best) best = k;
       }
       best = wave_kmax(best);
@@ -166,7 +164,7 @@ __global__ __launch_bounds__(256) void beam_chunk_kernel(SelArgs a) {
     if (k && rank < a.K) out[rank] = k;
   }
   // fewer columns than K (the last chunk): the rest of the list is empty
-  const int have = min(a.V - c0, kSelChunk);
+  const int have = min(a.V - c0, CHUNK);
   if (tid >= have && tid < a.K) out[tid] = 0;
   if (tid == 0) {
     float M = sml[0].x;
@@ -177,6 +175,9 @@ __global__ __launch_bounds__(256) void beam_chunk_kernel(SelArgs a) {
   }
 }
 
+__device__ __forceinline__ u64 lane_u64(u64 v, int lane) {
+  return ((u64)(unsigned)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32) | (unsigned)__builtin_amdgcn_readlane((int)v, lane);
+}
 __device__ __forceinline__ u64 ord_d(double v) {
   const u64 u = (u64)__double_as_longlong(v);
   return (u >> 63) ? ~u : (u | 0x8000000000000000ull);
@@ -187,6 +188,8 @@ __device__ __forceinline__ u64 ord_d(double v) {
 __global__ __launch_bounds__(1024) void beam_pick_kernel(SelArgs a) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   u64* sc = reinterpret_cast<u64*>(smem);             // [W][K] ordered bits of the scores, descending
+  u64* cand = sc + a.W * a.K + (a.W * a.K + 1) / 2;   // [waves][kSelList], and then
+  int* rk = reinterpret_cast<int*>(cand);             // [W][K] ranks over all rows
   int* ti = reinterpret_cast<int*>(sc + a.W * a.K);   // [W][K] tokens; -1 = none
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, nw = blockDim.x >> 6;
   const int b = blockIdx.x, K = a.K;
@@ -198,6 +201,12 @@ __global__ __launch_bounds__(1024) void beam_pick_kernel(SelArgs a) {
     fin_s[w] = a.fin ? a.fin[(long)b * a.W + w] : 0;
   }
   __syncthreads();
+  auto put = [&](int w, int i, u64 k, double s, double M, double lt) {  // i-th best of row w
+    double v = s + (((double)unord_f((unsigned)(k >> 32)) - M) - lt) + 0.0;
+    if (v != v) v = -INFINITY;  // +inf score and a -inf logit
+    sc[w * K + i] = ord_d(v);
+    ti[w * K + i] = k ? key_idx(k) : -1;
+  };
   for (int w = wave; w < a.W; w += nw) {
     const long row = (long)b * a.W + w;
     const float s = sin_s[w];
@@ -213,21 +222,49 @@ __global__ __launch_bounds__(1024) void beam_pick_kernel(SelArgs a) {
       live = t > 0.0 && lt - lt == 0.0 && M - M == 0.0;  // a row of -inf, or with a NaN or +inf, offers nothing
     }
     if (live) {
+      // The row's K best of the chunks' sorted lists, a list a lane. No more than K lists matter, those with the largest
+      // heads, and of them the keys from the K-th largest head on; mostly few more than K.
       const u64* lp = a.keys + (row * a.C + lane) * K;
-      u64 cur = lane < a.C ? lp[0] : 0, nxt = lane < a.C && K > 1 ? lp[1] : 0;
-      int at = 2;
+      u64 head = lane < a.C ? lp[0] : 0, nxt[3];
+#pragma unroll
+      for (int i = 0; i < 3; ++i) nxt[i] = lane < a.C && i + 1 < K ? lp[i + 1] : 0;
+      const int lists = __popcll(__ballot(head != 0)), q = (K + lists - 1) / lists;
+      u64 bar;
+      if (q == 1) {
+        int rank = 0;
+        for (int i = 0; i < a.C; ++i) rank += lane_u64(head, i) > head;
+        const u64 atk = __ballot(rank == K - 1 && head);  // (heads are all different, but for empty lists)
+        bar = lane_u64(head, (int)__ffsll((long long)atk) - 1);
+      } else {  // fewer lists than K: the least of their q-th keys has q keys of each list at or above it
+        const u64 k = lane >= a.C || !head ? ~0ull : q == 2 ? nxt[0] : q == 3 ? nxt[1] : q <= K ? lp[q - 1] : 0;
+        bar = ~wave_kmax(~k);
+        if (!bar) bar = 1;
+      }
+      u64* cl = cand + wave * kSelList;
+      int cnt = 0;
       for (int i = 0; i < K; ++i) {
-        const u64 best = wave_kmax(cur);
-        if (lane == 0) {
-          double v = (double)s + (((double)unord_f((unsigned)(best >> 32)) - M) - lt) + 0.0;
-          if (v != v) v = -INFINITY;  // +inf score and a -inf logit
-          sc[w * K + i] = ord_d(v);
-          ti[w * K + i] = best ? key_idx(best) : -1;
+        const u64 k = i == 0 ? head : i == 1 ? nxt[0] : i == 2 ? nxt[1] : i == 3 ? nxt[2] : head >= bar && lane < a.C ? lp[i] : 0;
+        const u64 in = __ballot(k >= bar);
+        if (!in) break;
+        const int at = cnt + __popcll(in & ((1ull << lane) - 1));
+        if (k >= bar && at < kSelList) cl[at] = k;
+        cnt += __popcll(in);
+      }
+      if (cnt <= kSelList) {
+        for (int j = lane; j < cnt; j += 64) {
+          const u64 mine = cl[j];
+          int r = 0;
+          for (int i = 0; i < cnt; ++i) r += cl[i] > mine;
+          if (r < K) put(w, r, mine, (double)s, M, lt);
         }
-        if (cur == best && best) {
-          cur = nxt;
-          nxt = at < K ? lp[at] : 0;
-          ++at;
+        if (lane >= cnt && lane < K) put(w, lane, 0, (double)s, M, lt);  // fewer columns than K: the rest stays empty
+      } else {  // many equal logits: one by one
+        u64 cur = head;
+        int at = 1;
+        for (int i = 0; i < K; ++i) {
+          const u64 best = wave_kmax(cur);
+          if (lane == 0) put(w, i, best, (double)s, M, lt);
+          if (cur == best && best) { cur = at < K ? lp[at] : 0; ++at; }
         }
       }
     } else {
@@ -245,23 +282,29 @@ __global__ __launch_bounds__(1024) void beam_pick_kernel(SelArgs a) {
       }
     }
   }
+  __syncthreads();  // the candidates are done with: their place holds the ranks
+  for (int i = tid; i < a.W * K; i += blockDim.x) rk[i] = i % K;  // within its own list
+  __syncthreads();
+  // how many of list u come before (v, w * V + t): a thread for each candidate and other list, counts added up
+  for (int p = tid; p < a.W * K * a.W; p += blockDim.x) {
+    const int i = p / a.W, u = p - i * a.W, w = i / K;
+    if (u == w || ti[i] < 0) continue;
+    const u64 v = sc[i];
+    int lo = 0, hi = K;
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      const u64 x = sc[u * K + mid];
+      const bool before = ti[u * K + mid] >= 0 && (x > v || (x == v && u < w));
+      if (before) lo = mid + 1;
+      else hi = mid;
+    }
+    if (lo) atomicAdd(&rk[i], lo);
+  }
   __syncthreads();
   for (int i = tid; i < a.W * K; i += blockDim.x) {
-    const int w = i / K, t = ti[i];
+    const int w = i / K, t = ti[i], rank = rk[i];
     if (t < 0) continue;
     const u64 v = sc[i];
-    int rank = i - w * K;  // within its own list
-    for (int u = 0; u < a.W && rank < K; ++u) {
-      if (u == w) continue;
-      int lo = 0, hi = K;  // how many of list u come before (v, w * V + t)
-      while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        const bool before = ti[u * K + mid] >= 0 && (sc[u * K + mid] > v || (sc[u * K + mid] == v && u < w));
-        if (before) lo = mid + 1;
-        else hi = mid;
-      }
-      rank += lo;
-    }
     if (rank < K) {
       const long o = (long)b * K + rank;
       const u64 u = (v >> 63) ? (v & 0x7FFFFFFFFFFFFFFFull) : ~v;
@@ -334,6 +377,15 @@ static int check_select(const slx_beam_select_desc* d) {
   return 0;
 }
 
+// 8192 columns a workgroup instead of 4096 where that still leaves 512 workgroups
+static bool wide_chunks(const slx_beam_select_desc* d) {
+  return (int64_t)d->batch * d->width * ((d->vocab + 2 * kSelChunk - 1) / (2 * kSelChunk)) >= 512;
+}
+static int chunks_of(const slx_beam_select_desc* d) {
+  const int c = wide_chunks(d) ? 2 * kSelChunk : kSelChunk;
+  return (d->vocab + c - 1) / c;
+}
+
 }  // namespace slx
 
 using namespace slx;
@@ -342,7 +394,7 @@ extern "C" {
 
 int64_t slx_beam_select_ws_bytes(const slx_beam_select_desc* d) {
   if (int rc = check_select(d)) return rc;
-  const int64_t C = (d->vocab + kSelChunk - 1) / kSelChunk;
+  const int64_t C = chunks_of(d);
   return (int64_t)d->batch * d->width * C * (8 + 8 * (int64_t)d->k);
 }
 
@@ -357,15 +409,23 @@ int slx_beam_select(const slx_beam_select_desc* d, slx_stream_t s) {
   a.x = d->logits; a.ldx = d->ldx; a.score = d->score; a.fin = d->finished;
   a.score_out = d->score_out; a.parent = d->parent; a.token = d->token; a.fin_out = d->finished_out;
   a.B = d->batch; a.W = d->width; a.V = d->vocab; a.K = d->k; a.pad = d->pad; a.eos = d->eos;
-  a.C = (d->vocab + kSelChunk - 1) / kSelChunk;
+  a.C = chunks_of(d);
   a.ml = (float2*)d->ws;
   a.keys = (u64*)((char*)d->ws + (int64_t)a.B * a.W * a.C * 8);
   const dim3 grid(a.C, a.B * a.W);
-  if (d->logits_bf16) hipLaunchKernelGGL(beam_chunk_kernel<bf16>, grid, dim3(256), 0, (hipStream_t)s, a);
-  else hipLaunchKernelGGL(beam_chunk_kernel<float>, grid, dim3(256), 0, (hipStream_t)s, a);
+  const bool wide = wide_chunks(d);
+  if (d->logits_bf16 && wide) hipLaunchKernelGGL((beam_chunk_kernel<bf16, 32>), grid, dim3(256), 0, (hipStream_t)s, a);
+  else if (d->logits_bf16) hipLaunchKernelGGL((beam_chunk_kernel<bf16, 16>), grid, dim3(256), 0, (hipStream_t)s, a);
+  else if (wide) hipLaunchKernelGGL((beam_chunk_kernel<float, 32>), grid, dim3(256), 0, (hipStream_t)s, a);
+  else hipLaunchKernelGGL((beam_chunk_kernel<float, 16>), grid, dim3(256), 0, (hipStream_t)s, a);
   SLX_LAUNCH_CHECK("slx_beam_select (chunks)");
   const int nw = a.W < 16 ? a.W : 16;
-  hipLaunchKernelGGL(beam_pick_kernel, dim3(a.B), dim3(64 * nw), (size_t)a.W * a.K * 12, (hipStream_t)s, a);
+  const int wk = a.W * a.K, lds = 8 * (wk + (wk + 1) / 2) + (wk * 4 > nw * kSelList * 8 ? wk * 4 : nw * kSelList * 8);
+  if (lds > 60 * 1024) {
+    hipError_t e = hipFuncSetAttribute((const void*)beam_pick_kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    SLX_CHECK_ARG(e == hipSuccess, "slx_beam_select: %d B of LDS: %s", lds, hipGetErrorString(e));
+  }
+  hipLaunchKernelGGL(beam_pick_kernel, dim3(a.B), dim3(64 * nw), lds, (hipStream_t)s, a);
   SLX_LAUNCH_CHECK("slx_beam_select");
   return 0;
 }

@@ -127,14 +127,14 @@ struct PAttnArgs {
   unsigned gmul;  // r / gq = umulhi(r, gmul) (0: gq == 1)
   float c;        // scale * log2(e) > 0
   int mt_pre, mt_own;
-  long groups, n_pre;  // n_pre: workgroups of the prefix part
+  unsigned groups, n_pre;  // n_pre: workgroups of the prefix part
+  int D;
   int direct;     // one part per row: the workgroups write the output themselves
   long R;         // rows * Hq
   float* ws;      // o [parts][R][D], then (m, l) [parts][R]
 };
 
 __host__ __device__ __forceinline__ int split_keys(int len, int ns) { return ((len + ns - 1) / ns + 127) & ~127; }
-__device__ __forceinline__ int seg_len(const Seg& s, long i) { return s.len ? max(0, min(s.len[i], s.cap)) : 0; }
 __device__ __forceinline__ int row_token(const PAttnArgs& a, int r) { return a.gmul ? (int)__umulhi((unsigned)r, a.gmul) : r; }
 
 // one workgroup's share, uniform
@@ -142,12 +142,27 @@ struct Item {
   const bf16 *k, *v;  // of the kv head
   long ps, ss;
   int n_pages, shift;
-  const int* tab;
-  int len, kb, ke;    // keys of the sequence; this range
+  const int *tab, *lens;
+  int cap, ns, range;
+  int len, kb, ke;    // keys of the sequence; this range (item_range)
   bool causal;
   int kvh, ntok, mt, part;
   long tok0;          // first query token
 };
+
+__device__ __forceinline__ void item_segment(Item& w, const Seg& g, unsigned seq, bool causal) {
+  w.ns = g.ns;
+  w.cap = g.cap;
+  w.causal = causal;
+  w.k = g.p.k + w.kvh * g.p.hs;
+  w.v = g.p.v + w.kvh * g.p.hs;
+  w.ps = g.p.ps;
+  w.ss = g.p.ss;
+  w.n_pages = g.p.n_pages;
+  w.shift = g.p.shift;
+  w.tab = g.tab + seq * g.ldt;
+  w.lens = g.len + seq;
+}
 
 template <int D, int NQ>
 struct State {
@@ -166,9 +181,9 @@ __device__ __forceinline__ void state_init(State<D, NQ>& st) {
   }
 }
 
-// query rows r0 .. of a wave as B operands; lim: the keys each row sees
+// query rows r0 .. of a wave as B operands
 template <int D, int NQ>
-__device__ __forceinline__ void load_rows(const PAttnArgs& a, const Item& w, int r0, bf16x8 (&qf)[NQ][D / 32], int (&lim)[NQ]) {
+__device__ __forceinline__ void load_rows(const PAttnArgs& a, const Item& w, int r0, bf16x8 (&qf)[NQ][D / 32]) {
   const int col = threadIdx.x & 15, grp = (threadIdx.x & 63) >> 4, rows = w.ntok * a.gq;
 #pragma unroll
   for (int n = 0; n < NQ; ++n) {
@@ -176,6 +191,34 @@ __device__ __forceinline__ void load_rows(const PAttnArgs& a, const Item& w, int
     const bf16* qp = a.q + (w.tok0 + t) * a.ldq + (long)(w.kvh * a.gq + r - t * a.gq) * D + 8 * grp;
 #pragma unroll
     for (int k = 0; k < D / 32; ++k) qf[n][k] = *reinterpret_cast<const bf16x8*>(qp + 32 * k);
+  }
+}
+
+// The item's range of keys, from the length on the device, while the queries are on their way. An empty range writes
+// m = -inf for its rows (the join reads every part, and so does not wait for the lengths) and is done: false.
+__device__ __forceinline__ bool item_range(const PAttnArgs& a, Item& w, int tile_rows) {
+  w.len = max(0, min(*w.lens, w.cap));
+  const int ks = split_keys(w.len, w.ns);
+  w.kb = w.range * ks;
+  w.ke = min(w.len, w.kb + ks);
+  if (w.kb < w.len || a.direct) return true;
+  const int r = w.mt * tile_rows + (int)threadIdx.x;
+  if ((int)threadIdx.x < tile_rows && r < w.ntok * a.gq) {
+    const int t = row_token(a, r);
+    const long row = (w.tok0 + t) * a.Hq + w.kvh * a.gq + r - t * a.gq;
+    float* ml = a.ws + (long)(a.pre.ns + a.own.ns) * a.R * a.D + ((long)w.part * a.R + row) * 2;
+    *reinterpret_cast<float2*>(ml) = make_float2(-INFINITY, 0.f);
+  }
+  return false;
+}
+
+// the keys that each of a wave's rows sees
+template <int NQ>
+__device__ __forceinline__ void row_limits(const PAttnArgs& a, const Item& w, int r0, int (&lim)[NQ]) {
+  const int col = threadIdx.x & 15, rows = w.ntok * a.gq;
+#pragma unroll
+  for (int n = 0; n < NQ; ++n) {
+    const int t = row_token(a, min(r0 + 16 * n + col, rows - 1));
     lim[n] = w.causal ? min(w.ke, w.len - a.Tq + t + 1) : w.ke;
   }
 }
@@ -192,19 +235,24 @@ __device__ __forceinline__ void scores(const bf16x8 (&kf)[2][D / 32], const bf16
     }
 }
 
-// Scores to probabilities. `edge`: the tile holds keys that some row does not see (room: how many of the tile's keys each
-// row sees) or that are not there (dead: bit j of the lane's 8 keys).
-template <int D, int NQ>
-__device__ __forceinline__ void softmax_step(f32x4 (&s)[NQ][2], float c, bool edge, unsigned dead, const int (&lim)[NQ], int k0,
-                                             State<D, NQ>& st, bf16x8 (&pb)[NQ]) {
+// Scores of keys that are not there (dead: bit j of the lane's 8 keys) or that a row does not see (lim) to -inf.
+template <int NQ>
+__device__ __forceinline__ void mask_scores(f32x4 (&s)[NQ][2], unsigned dead, const int (&lim)[NQ], int k0) {
   const int grp = (threadIdx.x & 63) >> 4;
 #pragma unroll
   for (int n = 0; n < NQ; ++n) {
-    if (edge) {
+    const int room = lim[n] - k0 - 4 * grp;
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if ((dead >> j & 1) || k0 + 16 * (j >> 2) + 4 * grp + (j & 3) >= lim[n]) s[n][j >> 2][j & 3] = -INFINITY;
-    }
+    for (int j = 0; j < 8; ++j)
+      s[n][j >> 2][j & 3] = (dead >> j & 1) | (16 * (j >> 2) + (j & 3) >= room) ? -INFINITY : s[n][j >> 2][j & 3];
+  }
+}
+
+// Scores to probabilities, with the state rescaled where a row's maximum has moved.
+template <int D, int NQ>
+__device__ __forceinline__ void softmax_step(const f32x4 (&s)[NQ][2], float c, State<D, NQ>& st, bf16x8 (&pb)[NQ]) {
+#pragma unroll
+  for (int n = 0; n < NQ; ++n) {
     float mx = s[n][0][0];
 #pragma unroll
     for (int j = 1; j < 8; ++j) mx = fmaxf(mx, s[n][j >> 2][j & 3]);
@@ -323,12 +371,15 @@ __device__ __forceinline__ void add_nonfinite(const PAttnArgs& a, const Item& w,
 template <int D, int NQ>
 __device__ __forceinline__ void attn_direct(const PAttnArgs& a, Item w, char* smem) {
   constexpr int KK = D / 32, NE = D / 16;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, grp = lane >> 4;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, grp = lane >> 4;
   const int rows = w.ntok * a.gq, r0 = w.mt * 16 * NQ;
   const int shift = w.shift, mask = (1 << shift) - 1;
   bf16x8 qf[NQ][KK];
   int lim[NQ];
-  load_rows<D, NQ>(a, w, r0, qf, lim);
+  load_rows<D, NQ>(a, w, r0, qf);
+  asm volatile("" ::: "memory");  // the queries are requested before the length is waited for
+  if (!item_range(a, w, 16 * NQ)) return;
+  row_limits<NQ>(a, w, r0, lim);
   // the causal edge of an own segment: token t of Tq sees keys <= len - Tq + t
   const int free_end = w.causal ? min(w.ke, w.len - a.Tq + row_token(a, r0) + 1) : w.ke;  // keys below it are seen by every row
   const int ke = w.causal ? min(w.ke, w.len - a.Tq + row_token(a, min(r0 + 16 * NQ, rows) - 1) + 1) : w.ke;
@@ -410,15 +461,17 @@ __device__ __forceinline__ void attn_direct(const PAttnArgs& a, Item w, char* sm
     const bool edge = k0 + 32 > free_end || __any(bad != 0);
     unsigned dead = bad;
     if (edge) {
+      const int left = w.len - k0 - 4 * grp;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) dead |= (k0 + 16 * (j >> 2) + 4 * grp + (j & 3) >= w.len ? 1u : 0u) << j;
+      for (int j = 0; j < 8; ++j) dead |= (16 * (j >> 2) + (j & 3) >= left ? 1u : 0u) << j;
+      mask_scores<NQ>(s, dead, lim, k0);
     }
     const bool more = k0 + 128 < ke;
     if (more) {
       load_k(k0 + 128);
       entries_k(k0 + 256);
     }
-    softmax_step<D, NQ>(s, a.c, edge, dead, lim, k0, st, pb);
+    softmax_step<D, NQ>(s, a.c, st, pb);
     if (edge) odd = clean_v<D>(vr, dead, w.causal && a.Tq > 1) || odd;
     output_step<D, NQ>(vr, pb, st);
     if (more) {
@@ -490,36 +543,34 @@ __device__ __forceinline__ void attn_direct(const PAttnArgs& a, Item w, char* sm
 constexpr int kRing = 4;
 template <int N>
 __device__ __forceinline__ void wait_vm() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
+// this wave's pieces of the oldest tile are in LDS, with up to N younger tiles of PER pieces under way
+template <int N, int PER>
+__device__ __forceinline__ void wait_tiles(int younger) {
+  if (younger >= N) wait_vm<N * PER>();
+  else if constexpr (N > 0) wait_tiles<N - 1, PER>(younger);
+}
 // 16 B a lane from global memory to LDS at the wave's base + 16 * lane (m0: the base)
 __device__ __forceinline__ void dma16(const void* g, const char* lds) {
   const unsigned m = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)LDS_PTR(const char, lds));
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(m), "v"(g) : "memory");
 }
 
+// The keys of one segment into the state of a wave's rows r0 .. (the workgroup's from rw); whether values were sifted out.
+// The LDS is free when it is called, and its last tiles may still be read when it returns.
 template <int D, int NQ>
-__device__ __forceinline__ void attn_stream(const PAttnArgs& a, Item w, char* smem) {
+__device__ __forceinline__ bool stream_keys(const PAttnArgs& a, const Item& w, int rw, int r0, const bf16x8 (&qf)[NQ][D / 32],
+                                            State<D, NQ>& st, char* smem) {
   constexpr int KK = D / 32, NE = D / 16, CH = D / 8, TILE = 32 * D * 2, PER = 2 * D / 64;  // PER: DMA pieces a wave and tile
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, grp = lane >> 4;
-  const int rows = w.ntok * a.gq, rw = w.mt * 64 * NQ, r0 = rw + wave * 16 * NQ;
-  const int shift = w.shift, mask = (1 << shift) - 1;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, grp = lane >> 4;
+  const int rows = w.ntok * a.gq, shift = w.shift, mask = (1 << shift) - 1;
   unsigned char* badb = reinterpret_cast<unsigned char*>(smem + kRing * 2 * TILE);  // [kRing][4]: 8 keys a wave, 0 or 255
-  bf16x8 qf[NQ][KK];
   int lim[NQ];
-  load_rows<D, NQ>(a, w, r0, qf, lim);
+  row_limits<NQ>(a, w, r0, lim);
   auto tok_of = [&](int r) { return row_token(a, min(r, rows - 1)); };
   const int free_end = w.causal ? min(w.ke, w.len - a.Tq + tok_of(r0) + 1) : w.ke;  // seen by every row of the wave
   const int ke = w.causal ? min(w.ke, w.len - a.Tq + tok_of(rw + 64 * NQ - 1) + 1) : w.ke;
   const int kw = r0 >= rows ? 0 : w.causal ? min(w.ke, w.len - a.Tq + tok_of(r0 + 16 * NQ - 1) + 1) : w.ke;  // this wave's last
   const int nt = ke > w.kb ? (ke - w.kb + 31) / 32 : 0;
-  State<D, NQ> st;
-  state_init(st);
-  // the queries are here before the first DMA is counted
-  __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
-#pragma unroll
-  for (int n = 0; n < NQ; ++n)
-#pragma unroll
-    for (int k = 0; k < KK; ++k) asm volatile("" : "+v"(qf[n][k]));
-
   // LDS rows: slot of key x = x with bits 0 and 2 swapped; chunk c of a slot lies at c ^ swz(slot)
   auto slot_of = [](int x) { return (x & ~5) | (x & 1) << 2 | (x >> 2 & 1); };
   auto swz = [](int slot) { return D == 64 ? slot >> 1 & 7 : slot & 15; };
@@ -541,33 +592,42 @@ __device__ __forceinline__ void attn_stream(const PAttnArgs& a, Item w, char* sm
       dma16(w.v + off, base + TILE + (8 * wave + (64 / CH) * i) * D * 2);
     }
   };
-  int e0 = 0, e1 = 0, e2 = 0, en = 0;
-  if (nt > 0) { e0 = entry(0); e1 = entry(1); e2 = entry(2); en = entry(3); }
-  if (nt > 0) issue(0, e0);
-  if (nt > 1) issue(1, e1);
-  if (nt > 2) issue(2, e2);
+  int en = 0;
+  if (nt > 0) {
+    int e[kRing - 1];
+#pragma unroll
+    for (int i = 0; i < kRing - 1; ++i) e[i] = entry(i);
+    en = entry(kRing - 1);
+#pragma unroll
+    for (int i = 0; i < kRing - 1; ++i)
+      if (i < nt) issue(i, e[i]);
+  }
+  int ko[KK], vo[8];  // this lane's operands within a tile
+#pragma unroll
+  for (int k = 0; k < KK; ++k) ko[k] = slot_of(col) * D * 2 + ((4 * k + grp) ^ swz(slot_of(col))) * 16;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const int slot = slot_of(16 * (j >> 2) + 4 * grp + (j & 3));
+    vo[j] = TILE + slot * D * 2 + (NE == 4 ? ((col >> 1) ^ swz(slot)) * 16 + (col & 1) * 8 : (col ^ swz(slot)) * 16);
+  }
   bool odd = false;
   for (int t = 0; t < nt; ++t) {
     const int k0 = w.kb + 32 * t;
-    if (nt - 1 - t >= 2) wait_vm<2 * PER>();
-    else if (nt - 1 - t == 1) wait_vm<PER>();
-    else wait_vm<0>();
+    wait_tiles<kRing - 2, PER>(nt - 1 - t);
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // this wave has read the slot that is filled next
     __builtin_amdgcn_s_barrier();
-    if (t + 3 < nt) {
-      issue(t + 3, en);
-      en = entry(t + 4);
+    if (t + kRing - 1 < nt) {
+      issue(t + kRing - 1, en);
+      en = entry(t + kRing);
     }
     if (k0 >= kw) continue;
-    const char* Kl = smem + (t % kRing) * 2 * TILE;
-    const char* Vl = Kl + TILE;
+    const char* tile = smem + (t % kRing) * 2 * TILE;
     const unsigned bads = *reinterpret_cast<const unsigned*>(badb + (t % kRing) * 4);
     bf16x8 kf[2][KK];
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      const int slot = slot_of(16 * s + col);
-#pragma unroll
-      for (int k = 0; k < KK; ++k) kf[s][k] = *reinterpret_cast<const bf16x8*>(Kl + slot * D * 2 + ((4 * k + grp) ^ swz(slot)) * 16);
+    for (int k = 0; k < KK; ++k) {  // keys 16 apart lie 16 slots apart, under the same swizzle
+      kf[0][k] = *reinterpret_cast<const bf16x8*>(tile + ko[k]);
+      kf[1][k] = *reinterpret_cast<const bf16x8*>(tile + ko[k] + 16 * D * 2);
     }
     f32x4 s[NQ][2];
     bf16x8 pb[NQ];
@@ -575,12 +635,11 @@ __device__ __forceinline__ void attn_stream(const PAttnArgs& a, Item w, char* sm
     scores<D, NQ>(kf, qf, s);
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const int slot = slot_of(16 * (j >> 2) + 4 * grp + (j & 3));
       if constexpr (NE == 4) {
-        const u32x2 x = *reinterpret_cast<const u32x2*>(Vl + slot * D * 2 + ((col >> 1) ^ swz(slot)) * 16 + (col & 1) * 8);
+        const u32x2 x = *reinterpret_cast<const u32x2*>(tile + vo[j]);
         vr[j][0] = x[0]; vr[j][1] = x[1];
       } else {
-        const u32x4 x = *reinterpret_cast<const u32x4*>(Vl + slot * D * 2 + (col ^ swz(slot)) * 16);
+        const u32x4 x = *reinterpret_cast<const u32x4*>(tile + vo[j]);
 #pragma unroll
         for (int i = 0; i < NE / 2; ++i) vr[j][i] = x[i];
       }
@@ -593,19 +652,49 @@ __device__ __forceinline__ void attn_stream(const PAttnArgs& a, Item w, char* sm
         const int x = 16 * (j >> 2) + 4 * grp + (j & 3);
         dead |= (k0 + x >= w.len || (bads >> x & 1) ? 1u : 0u) << j;
       }
+      mask_scores<NQ>(s, dead, lim, k0);
     }
-    softmax_step<D, NQ>(s, a.c, edge, dead, lim, k0, st, pb);
+    softmax_step<D, NQ>(s, a.c, st, pb);
     if (edge) odd = clean_v<D>(vr, dead, w.causal && a.Tq > 1) || odd;
     output_step<D, NQ>(vr, pb, st);
   }
+  return odd;
+}
+
+// the queries are here before the first DMA is counted
+template <int D, int NQ>
+__device__ __forceinline__ void settle_rows(bf16x8 (&qf)[NQ][D / 32]) {
+  __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
+#pragma unroll
+  for (int n = 0; n < NQ; ++n)
+#pragma unroll
+    for (int k = 0; k < D / 32; ++k) asm volatile("" : "+v"(qf[n][k]));
+}
+
+template <int D, int NQ>
+__device__ __forceinline__ void store_stream(const PAttnArgs& a, const Item& w, int r0, bool odd, const State<D, NQ>& st) {
   odd = __any(odd);
 #pragma unroll
   for (int n = 0; n < NQ; ++n) {
-    const int r = r0 + 16 * n + col;
-    if (r >= rows) continue;
+    const int r = r0 + 16 * n + (threadIdx.x & 15);
+    if (r >= w.ntok * a.gq) continue;
     store_row<D>(a, w, r, st.m[n], st.l[n][0], st.o[n]);
     if (odd) add_nonfinite<D>(a, w, r);
   }
+}
+
+template <int D, int NQ>
+__device__ __forceinline__ void attn_stream(const PAttnArgs& a, Item w, char* smem) {
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), rw = w.mt * 64 * NQ, r0 = rw + wave * 16 * NQ;
+  bf16x8 qf[NQ][D / 32];
+  load_rows<D, NQ>(a, w, r0, qf);
+  asm volatile("" ::: "memory");  // the queries are requested before the length is waited for
+  if (!item_range(a, w, 64 * NQ)) return;
+  State<D, NQ> st;
+  state_init(st);
+  settle_rows<D, NQ>(qf);
+  const bool odd = stream_keys<D, NQ>(a, w, rw, r0, qf, st, smem);
+  store_stream<D, NQ>(a, w, r0, odd, st);
 }
 
 // kinds of a workgroup: direct with 16 or 32 rows, streamed with 64 or 128
@@ -626,46 +715,34 @@ template <int D, int KP, int KO>
 __global__ __launch_bounds__(256, 2) void prefix_attn_kernel(PAttnArgs a) {
   constexpr int LDS = kind_lds(D, KP) > kind_lds(D, KO) ? kind_lds(D, KP) : kind_lds(D, KO);
   __shared__ __attribute__((aligned(16))) char smem[LDS];
-  long b = blockIdx.x;
+  unsigned b = blockIdx.x;
   const bool pre = b < a.n_pre;
   Item w;
-  long seq;
+  unsigned seq;
   if (pre) {  // [group][kv head][range][row tile]; 8 neighbours stay 8 apart, so the row tiles of a range share an XCD's L2
-    const long x = b & 7, y = b >> 3;
-    w.mt = (int)(y % a.mt_pre);
-    b = (y / a.mt_pre) * 8 + x;
-    w.part = (int)(b % a.pre.ns);
-    b /= a.pre.ns;
-    w.kvh = (int)(b % a.Hkv);
-    seq = b / a.Hkv;
+    const unsigned x = b & 7, y = b >> 3;
+    w.mt = (int)(y % (unsigned)a.mt_pre);
+    b = (y / (unsigned)a.mt_pre) * 8 + x;
+    w.part = (int)(b % (unsigned)a.pre.ns);
+    b /= (unsigned)a.pre.ns;
+    w.kvh = (int)(b % (unsigned)a.Hkv);
+    seq = b / (unsigned)a.Hkv;
     if (seq >= a.groups) return;  // the grid is padded to a multiple of 8
-    w.tok0 = seq * a.W * a.Tq;
+    w.tok0 = (long)seq * a.W * a.Tq;
     w.ntok = a.W * a.Tq;
-    w.len = seg_len(a.pre, seq);
   } else {  // [sequence][row tile][kv head][range]
     b -= a.n_pre;
-    w.part = (int)(b % a.own.ns);
-    b /= a.own.ns;
-    w.kvh = (int)(b % a.Hkv);
-    b /= a.Hkv;
-    w.mt = (int)(b % a.mt_own);
-    seq = b / a.mt_own;
-    w.tok0 = seq * a.Tq;
+    w.part = (int)(b % (unsigned)a.own.ns);
+    b /= (unsigned)a.own.ns;
+    w.kvh = (int)(b % (unsigned)a.Hkv);
+    b /= (unsigned)a.Hkv;
+    w.mt = (int)(b % (unsigned)a.mt_own);
+    seq = b / (unsigned)a.mt_own;
+    w.tok0 = (long)seq * a.Tq;
     w.ntok = a.Tq;
-    w.len = seg_len(a.own, seq);
   }
-  const int ks = split_keys(w.len, pre ? a.pre.ns : a.own.ns);
-  w.kb = w.part * ks;
-  if (w.kb >= w.len && !a.direct) return;
-  w.ke = min(w.len, w.kb + ks);
-  w.causal = !pre;
-  w.k = (pre ? a.pre.p.k : a.own.p.k) + w.kvh * (pre ? a.pre.p.hs : a.own.p.hs);
-  w.v = (pre ? a.pre.p.v : a.own.p.v) + w.kvh * (pre ? a.pre.p.hs : a.own.p.hs);
-  w.ps = pre ? a.pre.p.ps : a.own.p.ps;
-  w.ss = pre ? a.pre.p.ss : a.own.p.ss;
-  w.n_pages = pre ? a.pre.p.n_pages : a.own.p.n_pages;
-  w.shift = pre ? a.pre.p.shift : a.own.p.shift;
-  w.tab = pre ? a.pre.tab + seq * a.pre.ldt : a.own.tab + seq * a.own.ldt;
+  w.range = w.part;
+  item_segment(w, pre ? a.pre : a.own, seq, !pre);
   if (!pre) w.part += a.pre.ns;
   if constexpr (KP == KO) {
     attn_kind<D, KP>(a, w, smem);
@@ -675,21 +752,49 @@ __global__ __launch_bounds__(256, 2) void prefix_attn_kernel(PAttnArgs a) {
   }
 }
 
-// Joins the parts of a row: D / 4 threads, four d each, times PG groups that share the parts out (16 or 8 for rows with
-// many parts, where a row's parts would otherwise be one chain of loads).
-template <int D, int PG>
+// Many new tokens in many sequences: a workgroup takes 64 or 128 rows of ONE sequence through the prefix and then its own
+// keys, so there are no parts to write and join (the prefix is fetched again for every tile of rows, from L2).
+template <int D, int NQ>
+__global__ __launch_bounds__(256, 2) void prefix_attn_whole_kernel(PAttnArgs a) {
+  __shared__ __attribute__((aligned(16))) char smem[kRing * 2 * 32 * D * 2 + 4 * kRing];
+  unsigned b = blockIdx.x;  // [kv head][sequence][row tile]: neighbours share the prefix
+  Item w;
+  w.mt = (int)(b % (unsigned)a.mt_own);
+  b /= (unsigned)a.mt_own;
+  const unsigned n = a.groups * (unsigned)a.W, seq = b % n;
+  w.kvh = (int)(b / n);
+  w.tok0 = (long)seq * a.Tq;
+  w.ntok = a.Tq;
+  w.range = w.part = 0;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), rw = w.mt * 64 * NQ, r0 = rw + wave * 16 * NQ;
+  bf16x8 qf[NQ][D / 32];
+  load_rows<D, NQ>(a, w, r0, qf);
+  asm volatile("" ::: "memory");  // the queries are requested before the lengths are waited for
+  item_segment(w, a.pre, seq / (unsigned)a.W, false);
+  item_range(a, w, 64 * NQ);
+  State<D, NQ> st;
+  state_init(st);
+  settle_rows<D, NQ>(qf);
+  stream_keys<D, NQ>(a, w, rw, r0, qf, st, smem);
+  item_segment(w, a.own, seq, true);
+  item_range(a, w, 64 * NQ);
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the ring is free when every wave has read the prefix's last tiles
+  __builtin_amdgcn_s_barrier();
+  const bool odd = stream_keys<D, NQ>(a, w, rw, r0, qf, st, smem);
+  store_stream<D, NQ>(a, w, r0, odd, st);
+}
+
+// Joins the parts of a row: D / 4 threads, four d each, times PG groups that share the parts out, B at a time (8 parts at
+// once by one group; or 16 or 8 groups for rows with many parts, whose loads would otherwise be one chain).
+template <int D, int PG, int B>
 __global__ __launch_bounds__(256) void prefix_attn_join_kernel(PAttnArgs a) {
-  constexpr int TPR = D / 4, RPB = 256 / (TPR * PG), B = 4;
+  constexpr int TPR = D / 4, RPB = 256 / (TPR * PG);
   __shared__ float sml[PG > 1 ? PG : 1][2];
   __shared__ __attribute__((aligned(16))) f32x4 so[PG > 1 ? PG : 1][TPR];
-  const int d4 = threadIdx.x % TPR, pg = threadIdx.x / TPR % PG;
+  const int d4 = threadIdx.x % TPR, pg = threadIdx.x / TPR % PG, parts = a.pre.ns + a.own.ns;
   const long row = (long)blockIdx.x * RPB + threadIdx.x / (TPR * PG);
   if (row >= a.R) return;  // PG > 1: one row a workgroup
-  const long tok = row / a.Hq, n = tok / a.Tq;
-  const int pl = seg_len(a.pre, n / a.W), ol = seg_len(a.own, n);
-  const int np = pl ? (pl + split_keys(pl, a.pre.ns) - 1) / split_keys(pl, a.pre.ns) : 0;
-  const int no = ol ? (ol + split_keys(ol, a.own.ns) - 1) / split_keys(ol, a.own.ns) : 0;
-  const float2* ml = reinterpret_cast<const float2*>(a.ws + (long)(a.pre.ns + a.own.ns) * a.R * D) + row;
+  const float2* ml = reinterpret_cast<const float2*>(a.ws + parts * a.R * D) + row;
   const float* ob = a.ws + row * D + 4 * d4;
   float m = -INFINITY, l = 0.f;
   f32x4 o = {0.f, 0.f, 0.f, 0.f};
@@ -710,15 +815,15 @@ __global__ __launch_bounds__(256) void prefix_attn_join_kernel(PAttnArgs a) {
     }
     m = mn;
   };
-  for (int i0 = pg; i0 < np + no; i0 += B * PG) {
+  for (int i0 = pg; i0 < parts; i0 += B * PG) {
     float xm[B], xl[B];
     f32x4 y[B];
 #pragma unroll
     for (int u = 0; u < B; ++u) {
-      const int i = min(i0 + u * PG, np + no - 1), p = i < np ? i : a.pre.ns + i - np;
+      const int p = min(i0 + u * PG, parts - 1);
       const float2 x = ml[(long)p * a.R];
       y[u] = *reinterpret_cast<const f32x4*>(ob + (long)p * a.R * D);
-      xm[u] = i0 + u * PG < np + no ? x.x : -INFINITY;
+      xm[u] = i0 + u * PG < parts ? x.x : -INFINITY;
       xl[u] = x.y;
     }
     add(xm, xl, y);
@@ -740,6 +845,7 @@ __global__ __launch_bounds__(256) void prefix_attn_join_kernel(PAttnArgs a) {
       add(xm, xl, y);
     }
   }
+  const long tok = row / a.Hq;
   const float inv = l > 0.f || l != l ? 1.0f / l : 0.f;
   bf16x4 y;
 #pragma unroll
@@ -749,28 +855,39 @@ __global__ __launch_bounds__(256) void prefix_attn_join_kernel(PAttnArgs a) {
 }
 
 // Row tiles and key ranges of a call: a rule on sizes, page sizes and the host's bounds alone, so a captured call replays
-// for any lengths up to them. As many ranges as give about kTarget workgroups, each of at least 128 keys.
-constexpr long kTarget = 512;
-struct PAttnPlan { int kp, ko, mtp, mto, nsp, nso; };
+// for any lengths up to them. As many ranges as give about kTarget workgroups, each of at least 128 keys; or, where the
+// tiles of 64 rows of single sequences make kWhole workgroups by themselves, the whole rows at once.
+constexpr long kTarget = 768, kWhole = 192;
+struct PAttnPlan { int kp, ko, mtp, mto, nsp, nso, whole; };
 static PAttnPlan plan_attn(const slx_prefix_attn_desc* d, int capp, int capo) {
   PAttnPlan p;
   const int gq = d->Hq / d->own_pool.heads;
   auto kind = [](long rows, int page) { return rows <= 16 ? kD16 : rows <= 32 || page < 8 ? kD32 : rows <= 64 ? kS64 : kS128; };
-  const long rp = (long)d->width * d->n_q * gq, ro = (long)d->n_q * gq;
+  const long rp = (long)d->width * d->n_q * gq, ro = (long)d->n_q * gq, heads = d->own_pool.heads;
+  const long seqs = (long)d->groups * d->width * heads, t64 = (ro + 63) / 64, t128 = (ro + 127) / 128;
+  p.whole = 0;
   p.ko = kind(ro, d->own_pool.page);
   p.kp = capp > 0 ? kind(rp, d->prefix_pool.page) : p.ko;
+  if (capp > 0 && p.kp >= kS64 && p.ko >= kS64 && seqs * t64 >= kWhole) {
+    p.whole = 1;
+    p.ko = p.kp = seqs * t128 >= 2 * kWhole ? kS128 : kS64;
+    p.mto = p.mtp = (int)(p.ko == kS128 ? t128 : t64);
+    p.nsp = p.nso = 1;
+    return p;
+  }
   if (p.kp == kD32 && p.ko >= kS64) p.ko = kD32;       // fewer kernels: a streamed own part goes with a streamed prefix,
   if (p.kp == kS128 && p.ko == kS64) p.ko = kS128;     // of the same rows
   p.mtp = (int)((rp + kKindRows[p.kp] - 1) / kKindRows[p.kp]);
   p.mto = (int)((ro + kKindRows[p.ko] - 1) / kKindRows[p.ko]);
   const long up = (capp + 127) / 128, uo = (capo + 127) / 128;  // units of 128 keys
-  const long ip = (long)d->groups * d->own_pool.heads * p.mtp, io = (long)d->groups * d->width * d->own_pool.heads * p.mto;
+  const long ip = d->groups * heads * p.mtp, io = seqs * p.mto;
   const long per = (ip * up + io * uo + kTarget - 1) / kTarget, u = per > 1 ? per : 1;
   p.nsp = (int)((up + u - 1) / u);
   p.nso = (int)((uo + u - 1) / u);
   if (p.nso < 1) p.nso = 1;
   return p;
 }
+static bool is_direct(const PAttnPlan& p) { return p.whole || p.nsp + p.nso == 1; }
 
 static int check_pool(const slx_kv_pool& p, const char* who) {
   SLX_CHECK_ARG(p.k && p.v && ((uintptr_t)p.k & 15) == 0 && ((uintptr_t)p.v & 15) == 0, "%s: k and v must be 16-B aligned", who);
@@ -814,6 +931,11 @@ static int check_attn(const slx_prefix_attn_desc* d, int* capp, int* capo) {
 
 template <int D>
 static void launch_attn(const PAttnPlan& p, dim3 grid, hipStream_t st, const PAttnArgs& a) {
+  if (p.whole) {
+    if (p.ko == kS128) hipLaunchKernelGGL((prefix_attn_whole_kernel<D, 2>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((prefix_attn_whole_kernel<D, 1>), grid, dim3(256), 0, st, a);
+    return;
+  }
 #define SLX_PA(P, O)                                                                                         \
   if (p.kp == P && p.ko == O) {                                                                              \
     hipLaunchKernelGGL((prefix_attn_kernel<D, P, O>), grid, dim3(256), 0, st, a);                            \
@@ -827,10 +949,10 @@ template <int D>
 static void launch_join(int parts, hipStream_t st, const PAttnArgs& a) {
   constexpr int PG = 1024 / D;  // one row a workgroup
   if (parts > 8) {
-    hipLaunchKernelGGL((prefix_attn_join_kernel<D, PG>), dim3((unsigned)a.R), dim3(256), 0, st, a);
+    hipLaunchKernelGGL((prefix_attn_join_kernel<D, PG, 4>), dim3((unsigned)a.R), dim3(256), 0, st, a);
   } else {
     constexpr int RPB = 1024 / D;
-    hipLaunchKernelGGL((prefix_attn_join_kernel<D, 1>), dim3((unsigned)((a.R + RPB - 1) / RPB)), dim3(256), 0, st, a);
+    hipLaunchKernelGGL((prefix_attn_join_kernel<D, 1, 8>), dim3((unsigned)((a.R + RPB - 1) / RPB)), dim3(256), 0, st, a);
   }
 }
 
@@ -871,7 +993,7 @@ int64_t slx_prefix_attn_ws_floats(const slx_prefix_attn_desc* d) {
   int capp, capo;
   if (int rc = check_attn(d, &capp, &capo)) return rc;
   const PAttnPlan p = plan_attn(d, capp, capo);
-  if (p.nsp + p.nso == 1) return 0;
+  if (is_direct(p)) return 0;
   return (int64_t)(p.nsp + p.nso) * d->groups * d->width * d->n_q * d->Hq * (d->own_pool.head_dim + 2);
 }
 
@@ -893,15 +1015,17 @@ int slx_prefix_attn(const slx_prefix_attn_desc* d, slx_stream_t s) {
   a.c = d->scale * 1.44269504088896341f;
   a.gmul = a.gq == 1 ? 0u : (unsigned)((1ull << 32) / a.gq + 1);
   a.mt_pre = p.mtp; a.mt_own = p.mto; a.groups = d->groups;
-  a.n_pre = ((long)d->groups * Hkv * p.nsp + 7) / 8 * 8 * p.mtp;
-  a.direct = p.nsp + p.nso == 1;
+  const long n_pre = p.whole ? 0 : ((long)d->groups * Hkv * p.nsp + 7) / 8 * 8 * p.mtp;
+  a.D = D;
+  a.direct = is_direct(p);
   a.R = (long)d->groups * d->width * d->n_q * d->Hq;
   a.ws = d->ws;
   const int64_t need = a.direct ? 0 : (int64_t)(p.nsp + p.nso) * a.R * (D + 2);
   SLX_CHECK_ARG(need == 0 || (d->ws && ((uintptr_t)d->ws & 15) == 0 && d->ws_floats >= need),
                 "slx_prefix_attn: needs a 16-B aligned workspace of %lld floats", (long long)need);
-  const long blocks = a.n_pre + (long)d->groups * d->width * Hkv * p.mto * p.nso;
+  const long blocks = n_pre + (long)d->groups * d->width * Hkv * p.mto * p.nso;
   SLX_CHECK_ARG(blocks < 2147483648L, "slx_prefix_attn: too many rows");
+  a.n_pre = (unsigned)n_pre;
   if (D == 64) launch_attn<64>(p, dim3((unsigned)blocks), (hipStream_t)s, a);
   else launch_attn<128>(p, dim3((unsigned)blocks), (hipStream_t)s, a);
   SLX_LAUNCH_CHECK("slx_prefix_attn");

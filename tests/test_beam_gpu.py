@@ -24,7 +24,8 @@ def check(dev, logits, scores, width, k, finished=None, pad=0, exact_order=False
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("b,w,k,v", [(1, 1, 1, 1), (1, 1, 5, 5), (1, 4, 4, 151655), (2, 3, 6, 256), (3, 8, 16, 4097), (1, 16, 32, 8191), (2, 5, 64, 300),
-                                     (1, 64, 64, 4096), (1, 2, 3, 262144), (5, 1, 2, 12289), (2, 64, 7, 65)])
+                                     (1, 64, 64, 4096), (1, 2, 3, 262144), (5, 1, 2, 12289), (2, 64, 7, 65),
+                                     (4, 16, 32, 66001), (8, 8, 64, 151655), (64, 8, 3, 5001)])
 def test_beam_select(dev, b, w, k, v, dtype):
     g = gen(b + w + k + v)
     logits = (torch.randn(b * w, v, generator=g) * 3).to(dtype)
@@ -61,6 +62,8 @@ def test_ties_take_the_lowest(dev):
         g = gen(3)
         row = torch.randn(1, 20000, generator=g).to(dtype)
         check(dev, row.expand(8, -1).contiguous(), torch.full((8,), -1.25), 8, 16, exact_order=True)  # beams alike: the first ones'
+        many = torch.randint(0, 3, (64, 66000), generator=g).to(dtype)  # the form with 8192 columns a workgroup
+        check(dev, many, torch.zeros(64), 16, 40, exact_order=True)
         few = torch.randint(0, 3, (3, 5000), generator=g).to(dtype)
         check(dev, few, torch.zeros(3), 1, 40, exact_order=True)
         up = torch.arange(5000, dtype=F32).view(1, -1).div(64).to(dtype)  # rising: every thread's last is its largest
