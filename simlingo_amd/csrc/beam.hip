@@ -77,8 +77,9 @@ __global__ __launch_bounds__(256) void beam_chunk_kernel(SelArgs a) {
   float v[E];
   int n = E;
   // rows that have ended, or are out of the search already, are not read
+  const unsigned char ended = a.fin ? a.fin[row] : 0;  // both on their way before either is looked at
   const float s = a.score[row];
-  if ((a.fin && a.fin[row]) || s == -INFINITY || s != s) return;
+  if (ended || s == -INFINITY || s != s) return;
   if (c0 + CHUNK <= a.V) {
     T t[U][VEC];
 #pragma unroll
@@ -106,35 +107,38 @@ __global__ __launch_bounds__(256) void beam_chunk_kernel(SelArgs a) {
   for (int e = 0; e < E; ++e) l += __expf(v[e] - ms);
   l = warp_sum(l);
 
-  // a threshold with at least K of the chunk's columns at or above it: among the lanes' own maxima, halved into from both ends
+  // a threshold with at least K of the chunk's columns at or above it: among the lanes' own maxima, halved into from both
+  // ends until few more than K lanes are left (-inf: none, every column is a candidate)
   float tv = -INFINITY;
-  bool all = true;  // no threshold: every column is a candidate
   if (__popcll(__ballot(n > 0)) >= a.K) {
     unsigned lo = ~wave_umax(~(n ? om : 0u)), hi = wave_umax(n ? om : 0u);  // every lane with columns is >= lo
     for (int it = 0; it < 12 && lo < hi; ++it) {
       const unsigned mid = lo + (hi - lo) / 2 + 1;
-      if (__popcll(__ballot(n > 0 && om >= mid)) >= a.K) lo = mid;
+      const int above = __popcll(__ballot(n > 0 && om >= mid));
+      if (above >= a.K) lo = mid;
       else hi = mid - 1;
+      if (above >= a.K && above <= a.K + 2) break;
     }
-    tv = unord_f(max(lo, 0x007FFFFFu));  // at least -inf
-    all = lo <= 0x007FFFFFu;
+    if (lo > 0x007FFFFFu) tv = unord_f(lo);
   }
   if (lane == 0) {
     sml[wave] = make_float2(mw, l);
-    stv[wave] = all ? -INFINITY : tv;
+    stv[wave] = tv;
+  }
+  if (n < E) {  // columns behind V: above no threshold
+#pragma unroll
+    for (int e = 0; e < E; ++e) v[e] = e < n ? v[e] : NAN;
   }
   __syncthreads();
   tv = fmaxf(fmaxf(stv[0], stv[1]), fmaxf(stv[2], stv[3]));
-  u64 hit = 0;
 #pragma unroll
-  for (int e = 0; e < E; ++e) hit |= (u64)(tv == -INFINITY || v[e] >= tv) << e;
-  hit &= n >= 64 ? ~0ull : (1ull << n) - 1;
-  if (hit) {
-    const int at = atomicAdd(&scount, __popcll(hit));
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const int i = at + __popcll(hit & ((1ull << e) - 1));
-      if ((hit >> e & 1) && i < kSelList) list[i] = key_of(ord_f(v[e] + 0.f), col(e));  // -0 ties with 0
+  for (int e = 0; e < E; ++e) {
+    const bool h = v[e] >= tv;
+    if (__any(h)) {
+      if (h) {
+        const int at = atomicAdd(&scount, 1);
+        if (at < kSelList) list[at] = key_of(ord_f(v[e] + 0.f), col(e));  // -0 ties with 0
+      }
     }
   }
   __syncthreads();
@@ -147,7 +151,7 @@ __global__ __launch_bounds__(256) void beam_chunk_kernel(SelArgs a) {
 #pragma unroll
       for (int e = 0; e < E; ++e) {
         const u64 k = key_of(ord_f(v[e] + 0.f), col(e));
-        if (e < n && k < last && k > best) best = k;
+        if (v[e] == v[e] && k < last && k > best) best = k;
       }
       best = wave_kmax(best);
       if (lane == 0) list[wave * a.K + i] = best;
@@ -160,6 +164,7 @@ __global__ __launch_bounds__(256) void beam_chunk_kernel(SelArgs a) {
   if (tid < cnt) {  // every key is its own: the rank is the number of greater ones
     const u64 k = list[tid];
     int rank = 0;
+#pragma unroll 8
     for (int i = 0; i < cnt; ++i) rank += list[i] > k;
     if (k && rank < a.K) out[rank] = k;
   }
@@ -194,13 +199,7 @@ __global__ __launch_bounds__(1024) void beam_pick_kernel(SelArgs a) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, nw = blockDim.x >> 6;
   const int b = blockIdx.x, K = a.K;
   const u64 ninf = ord_d(-INFINITY);
-  __shared__ float sin_s[kSelMaxW];
   __shared__ unsigned char fin_s[kSelMaxW];
-  for (int w = tid; w < a.W; w += blockDim.x) {
-    sin_s[w] = a.score[(long)b * a.W + w];
-    fin_s[w] = a.fin ? a.fin[(long)b * a.W + w] : 0;
-  }
-  __syncthreads();
   auto put = [&](int w, int i, u64 k, double s, double M, double lt) {  // i-th best of row w
     double v = s + (((double)unord_f((unsigned)(k >> 32)) - M) - lt) + 0.0;
     if (v != v) v = -INFINITY;  // +inf score and a -inf logit
@@ -209,14 +208,23 @@ __global__ __launch_bounds__(1024) void beam_pick_kernel(SelArgs a) {
   };
   for (int w = wave; w < a.W; w += nw) {
     const long row = (long)b * a.W + w;
-    const float s = sin_s[w];
-    const bool fin = fin_s[w] != 0;
+    // everything that the row may need is requested at once; of a row that is out, nothing but the score has been written
+    const u64* lp = a.keys + (row * a.C + min(lane, a.C - 1)) * K;
+    const unsigned char ended = a.fin ? a.fin[row] : 0;
+    const float s = a.score[row];
+    const float2 x = a.ml[row * a.C + min(lane, a.C - 1)];
+    u64 head = lp[0], nxt[3];
+#pragma unroll
+    for (int i = 0; i < 3; ++i) nxt[i] = lp[min(i + 1, K - 1)];
+    const bool fin = ended != 0;
+    if (lane == 0) fin_s[w] = fin;
     double M = 0.0, lt = 0.0;  // the row's maximum, and the log of its sum of e^{x - M}: apart, since M may be huge
     bool live = !fin && !(s == -INFINITY || s != s);
     if (live) {
-      const float2 x = lane < a.C ? a.ml[row * a.C + lane] : make_float2(-INFINITY, 0.f);
-      M = (double)unord_f(wave_umax(ord_f(x.x)));
-      double t = lane < a.C ? (x.x == -INFINITY && x.y == 0.f ? 0.0 : (double)x.y * exp((double)x.x - M)) : 0.0;
+      const float Mf = unord_f(wave_umax(lane < a.C ? ord_f(x.x) : 0u));
+      M = (double)Mf;
+      // a chunk's weight in 32 bits, like the terms it sums; their sum and its log in 64
+      double t = lane < a.C && !(x.x == -INFINITY && x.y == 0.f) ? (double)(x.y * __expf(x.x - Mf)) : 0.0;
       for (int k = 32; k > 0; k >>= 1) t += __shfl_xor(t, k, 64);
       lt = log(t);
       live = t > 0.0 && lt - lt == 0.0 && M - M == 0.0;  // a row of -inf, or with a NaN or +inf, offers nothing
@@ -224,14 +232,14 @@ __global__ __launch_bounds__(1024) void beam_pick_kernel(SelArgs a) {
     if (live) {
       // The row's K best of the chunks' sorted lists, a list a lane. No more than K lists matter, those with the largest
       // heads, and of them the keys from the K-th largest head on; mostly few more than K.
-      const u64* lp = a.keys + (row * a.C + lane) * K;
-      u64 head = lane < a.C ? lp[0] : 0, nxt[3];
+      if (lane >= a.C) head = 0;
 #pragma unroll
-      for (int i = 0; i < 3; ++i) nxt[i] = lane < a.C && i + 1 < K ? lp[i + 1] : 0;
+      for (int i = 0; i < 3; ++i) nxt[i] = lane < a.C && i + 1 < K ? nxt[i] : 0;
       const int lists = __popcll(__ballot(head != 0)), q = (K + lists - 1) / lists;
       u64 bar;
       if (q == 1) {
         int rank = 0;
+#pragma unroll 4
         for (int i = 0; i < a.C; ++i) rank += lane_u64(head, i) > head;
         const u64 atk = __ballot(rank == K - 1 && head);  // (heads are all different, but for empty lists)
         bar = lane_u64(head, (int)__ffsll((long long)atk) - 1);
@@ -254,6 +262,7 @@ __global__ __launch_bounds__(1024) void beam_pick_kernel(SelArgs a) {
         for (int j = lane; j < cnt; j += 64) {
           const u64 mine = cl[j];
           int r = 0;
+#pragma unroll 8
           for (int i = 0; i < cnt; ++i) r += cl[i] > mine;
           if (r < K) put(w, r, mine, (double)s, M, lt);
         }
