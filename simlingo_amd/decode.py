@@ -32,6 +32,7 @@ import numpy as np
 import torch
 
 from . import kernels as K
+from . import paged as PG
 
 BF16, F32 = torch.bfloat16, torch.float32
 # the attention split over keys (Hkv x 8 workgroups) with its partials merged by the O GEMV's prologue
@@ -297,6 +298,106 @@ class GreedyDecoder:
         K.call("slx_wp_loss_fwd", K.P(sd_[0][0]), K.P(lab_s), 1, ns, cfg.speed_dims, 0, K.P(speed), K.P(dummy),
                K.stream_ptr())
         return route[0], speed[0]
+
+
+class BeamDecoder(GreedyDecoder):
+    """Beam search over the same weights and prompt cache: `generate` returns the best of `num_beams` continuations by the sum
+    of their tokens' log probabilities (an ended beam keeps its score and stays among them until the end).
+
+    The prompt runs once; its rows of the cache are the prefix that the beams share (slx_prefix_attn), and each beam's own
+    keys are a table of single slots, so a step reorders the table and no keys (slx_beam_reorder). One step is the batched
+    kernels over num_beams rows, slx_kv_append and slx_prefix_attn per layer, then slx_beam_select over the whole vocabulary.
+    Stands in for LLM.greedy_sample (simlingo_training/models/language_model/llm.py:178-250) wherever a decoder is taken
+    (infer_example); num_beams 1 is that loop."""
+
+    def __init__(self, engine, num_beams: int = 4, **kw):
+        if not 1 <= num_beams <= PG.MAX_WIDTH:
+            raise ValueError(f"num_beams must be 1 .. {PG.MAX_WIDTH}")
+        super().__init__(engine, use_graph=False, **kw)
+        cfg, dev, W = self.cfg, self.dev, int(num_beams)
+        self.num_beams = W
+        n, hk = max(self.max_new, 1), cfg.llm_kv_heads
+        page = self.max_len & -self.max_len  # the largest power of two that divides the cache: its rows as pages
+        pages = lambda c, at: c.as_strided((self.max_len // page, page, hk, 64), (page * self.nqkv, self.nqkv, 64, 1), at)  # noqa: E731
+        self._prefix = [(pages(c, self.qn), pages(c, self.qn + self.kn)) for c in self.cache]
+        self._ptab = torch.arange(self.max_len // page, dtype=torch.int32, device=dev).view(1, -1)
+        self._plen = torch.zeros(1, dtype=torch.int32, device=dev)
+        # slot j * W + w: token j of beam w
+        self._own = [torch.zeros(2, n * W, 1, hk, 64, dtype=BF16, device=dev) for _ in range(cfg.llm_layers)]
+        self._slots = torch.arange(n * W, dtype=torch.int32, device=dev).view(n, W).t().contiguous()
+
+    def _beam_step(self, tokens, j, S0, table, pos, lens):
+        """Token j of every beam through the layers -> logits [W, V] f32."""
+        eng, cfg, W = self.eng, self.cfg, tokens.numel()
+        d, F, Hq, s = cfg.llm_dim, cfg.llm_ffn, cfg.llm_heads, K.stream_ptr()
+        X = eng._e(W, d, dtype=F32)
+        K.call("slx_gather_rows_b2f", K.P(eng.W["llm.embed"]), d, K.P(tokens), W, d, K.P(X), d, s)
+        cos, sin = self.cos[S0:], self.sin[S0:]
+        for i in range(cfg.llm_layers):
+            p, Wm = f"llm.{i}.", self.Wm[i]
+            h, _ = eng._norm(X, eng.P[p + "ln1"], None, W, d, cfg.rms_eps, rms=True)
+            qkv = eng._e(W, self.nqkv)
+            K.mm(h, Wm["qkv_w"], qkv, bias=eng.P[p + "qkv_b"])
+            k, v = self._own[i]
+            PG.kv_append(qkv, k, v, table, pos, qkv[:, :self.qn], n_heads=Hq, cos=cos, sin=sin)
+            o = PG.prefix_attn(qkv[:, :self.qn], own=(k, v, table, lens), prefix=(*self._prefix[i], self._ptab, self._plen),
+                               n_heads=Hq, max_own=j + 1, max_prefix=S0)
+            Xm = eng._e(W, d, dtype=F32)
+            K.mm(o, Wm["o_w"], Xm, epi=K.EPI_RESID_LS, resid=X, ldr=d, ls=self.ones_d)
+            h2, _ = eng._norm(Xm, eng.P[p + "ln2"], None, W, d, cfg.rms_eps, rms=True)
+            gu, act, X = eng._e(W, 2 * F), eng._e(W, F), eng._e(W, d, dtype=F32)
+            K.mm(h2, Wm["gate_up_w"], gu)
+            K.call("slx_swiglu_fwd", K.P(gu), gu.stride(0), K.P(act), act.stride(0), W, F, s)
+            K.mm(act, Wm["down_w"], X, epi=K.EPI_RESID_LS, resid=Xm, ldr=d, ls=self.ones_d)
+        return self._logits(X)
+
+    def _logits(self, X):
+        eng, cfg = self.eng, self.cfg
+        h, _ = eng._norm(X, eng.P["llm.norm"], None, X.shape[0], cfg.llm_dim, cfg.rms_eps, rms=True)
+        out = eng._e(X.shape[0], eng.Vp, dtype=F32)
+        K.mm(h, eng.W["llm.lm_head"][: cfg.vocab], out)
+        return out[:, : cfg.vocab]
+
+    def search(self, prefix: torch.Tensor, max_new_tokens: int | None = None):
+        """-> (token ids [num_beams, n] int64, scores [num_beams] f32), best first, on the CPU; a beam that has ended is
+        filled with the end token."""
+        cfg, dev, W = self.cfg, self.dev, self.num_beams
+        n_max = self.max_new if max_new_tokens is None else min(int(max_new_tokens), self.max_new)
+        S0 = prefix.shape[0]
+        if S0 + n_max > self.max_len:
+            raise ValueError(f"prompt {S0} + {n_max} new tokens exceeds the cache ({self.max_len} rows)")
+        if n_max <= 0:
+            return torch.zeros(W, 0, dtype=torch.long), torch.zeros(W)
+        if W > cfg.vocab:
+            raise ValueError(f"{W} beams over {cfg.vocab} tokens")
+        pad = self.eos if 0 <= self.eos < cfg.vocab else 0
+        Xl = self._llm_batched(prefix, self.cache)
+        self._plen.fill_(S0)
+        table, pos, lens = self._slots.clone(), torch.zeros(W, dtype=torch.int32, device=dev), torch.ones(W, dtype=torch.int32, device=dev)
+        history = torch.full((W, n_max), pad, dtype=torch.int32, device=dev)
+        done = torch.zeros(W, dtype=torch.bool, device=dev)
+        scores, _, token = PG.beam_select(self._logits(Xl[S0 - 1:]), torch.zeros(1, device=dev), width=1, k=W, eos_id=self.eos,
+                                          finished_out=done)
+        history[:, 0] = token[0]
+        parent = torch.empty(1, W, dtype=torch.int32, device=dev)
+        for j in range(n_max - 1):
+            if j % self.check_every == 0 and bool(done.all()):
+                break
+            logits = self._beam_step(token.view(-1), j, S0, table, pos, lens)
+            PG.beam_select(logits, scores, width=W, finished=done, pad_id=pad, eos_id=self.eos, out=(scores, parent, token),
+                           finished_out=done)
+            PG.beam_reorder(table[:, :j + 1], parent)
+            PG.beam_reorder(history[:, :j + 1], parent)
+            history[:, j + 1] = token[0]
+            pos += 1
+            lens += 1
+        return history.long().cpu(), scores.view(-1).cpu()
+
+    def generate(self, prefix: torch.Tensor, max_new_tokens: int | None = None) -> torch.Tensor:
+        """The best beam's ids (int64, CPU), up to and with the end token if it was produced."""
+        t = self.search(prefix, max_new_tokens)[0][0]
+        end = (t == self.eos).nonzero()
+        return t[: int(end[0]) + 1] if end.numel() else t
 
 
 def infer_example(engine, decoder: GreedyDecoder, example, max_new_tokens: int | None = None):

@@ -83,8 +83,8 @@ def _bad(msg):
     raise ValueError(msg)
 
 
-def _launch(who, name, desc, first, *rest):
-    """Every tensor on the current device, where the launch goes; then the call on its current stream."""
+def _device(who, first, *rest):
+    """The device of every tensor given (None: not given), which has to be the current one, where the launch goes."""
     d = first.get_device()
     for t in rest:
         if t is not None and t.get_device() != d:
@@ -93,9 +93,7 @@ def _launch(who, name, desc, first, *rest):
         raise RuntimeError(f"{who}: SimLingo MI355X kernels need device tensors (no CPU fallback)")
     if d != _current():
         raise RuntimeError(f"{who}: tensors on cuda:{d}, current device cuda:{torch.cuda.current_device()}")
-    rc = getattr(K.lib(), name)(desc() if callable(desc) else desc, _raw_stream(d))
-    if rc:
-        K.check(rc, name)
+    return d
 
 
 def _i32(who, name, t, n):
@@ -177,12 +175,16 @@ def kv_append(qkv, k, v, table, pos, q_out=None, *, n_heads, cos=None, sin=None,
             _bad(f"{who}: cos and sin must be contiguous f32 [positions, {d // 2}]")
     desc = _APPEND.pack(*pool, x, ldx, q, ldq, tab, ldt, n_seq, cols, seq.data_ptr() if seq is not None else 0, pos.data_ptr(),
                         rows_per_seq, n_heads, rows, c, s, rope)
-    _launch(who, "slx_kv_append", desc, qkv, k, v, table, pos, q_out, cos, sin, seq)
+    dev = _device(who, qkv, k, v, table, pos, q_out, cos, sin, seq)
+    rc = K.lib().slx_kv_append(desc, _raw_stream(dev))
+    if rc:
+        K.check(rc, "slx_kv_append")
 
 
 @functools.lru_cache(maxsize=1024)
-def _attn_ws(ppool, opool, ptab, pmax, omax, pcols, ocols, groups, width, n_q, n_heads):
+def _attn_ws(ppool, opool, has_prefix, pmax, omax, pcols, ocols, groups, width, n_q, n_heads):
     """Floats of workspace for these sizes (the C entry's own rule; no address goes into it)."""
+    ptab = 16 if has_prefix else 0
     need = K.lib().slx_prefix_attn_ws_floats(_ATTN.pack(*_fake(ppool), *_fake(opool), 0, 0, 0, 0, 0, ptab, pcols, ptab, 0, ocols, 0, pmax, omax,
                                                         pcols, ocols, groups, width, n_q, n_heads, 1.0, 0, 0))
     if need < 0:
@@ -240,18 +242,17 @@ def prefix_attn(q, out=None, *, own, prefix=None, n_heads, n_q=1, scale=None, ma
     o, ldo = _rows(who, "out", out, rows, cols)
     if lse is not None and not (lse.dtype is F32 and lse.shape == (rows, n_heads) and lse.is_contiguous()):
         _bad(f"{who}: lse must be contiguous f32 [{rows}, {n_heads}]")
-    ws = None
-
-    def desc():  # after the device checks: the workspace is of this call alone, from the current stream's memory
-        nonlocal ws
-        need = _attn_ws(ppool[5:], opool[5:], 16 if pt else 0, pmax, omax, pcols, ocols, groups, n // groups, n_q, n_heads)
-        ws = torch.empty(need, dtype=F32, device=q.device) if need else None
-        return _ATTN.pack(*ppool, *opool, x, ldq, o, ldo, lse.data_ptr() if lse is not None else 0, pt, ldpt, pl, ot, ldot, olen.data_ptr(),
-                          pmax, omax, pcols, ocols, groups, n // groups, n_q, n_heads, scale,
-                          ws.data_ptr() if need else 0, need)
-
-    if n:
-        _launch(who, "slx_prefix_attn", desc, q, ok, ov, otab, olen, out, pk, pv, ptab, plen, lse)
+    dev = _device(who, q, ok, ov, otab, olen, out, pk, pv, ptab, plen, lse)
+    if not n:
+        return out
+    width = n // groups
+    need = _attn_ws(ppool[5:], opool[5:], pt != 0, pmax, omax, pcols, ocols, groups, width, n_q, n_heads)
+    ws = torch.empty(need, dtype=F32, device=q.device) if need else None  # of this call alone, from the current stream's memory
+    desc = _ATTN.pack(*ppool, *opool, x, ldq, o, ldo, lse.data_ptr() if lse is not None else 0, pt, ldpt, pl, ot, ldot, olen.data_ptr(),
+                      pmax, omax, pcols, ocols, groups, width, n_q, n_heads, scale, ws.data_ptr() if need else 0, need)
+    rc = K.lib().slx_prefix_attn(desc, _raw_stream(dev))
+    if rc:
+        K.check(rc, "slx_prefix_attn")
     return out
 
 
@@ -290,8 +291,8 @@ def beam_select(logits, scores, *, width, k=None, finished=None, pad_id=0, eos_i
             _bad(f"{who}: finished_out must be contiguous bool [{b}, {k}]")
         fo = finished_out.data_ptr()
     if out is None:
-        to = torch.empty(3, b, k, dtype=I32, device=logits.device)
-        out = to[0].view(F32), to[1], to[2]
+        s_out, (p_out, t_out) = torch.empty(b, k, dtype=F32, device=logits.device), torch.empty(2, b, k, dtype=I32, device=logits.device).unbind()
+        out = s_out, p_out, t_out
     s_out, p_out, t_out = out
     if not (s_out.dtype is F32 and p_out.dtype is I32 and t_out.dtype is I32 and s_out.numel() == p_out.numel() == t_out.numel() == b * k
             and s_out.is_contiguous() and p_out.is_contiguous() and t_out.is_contiguous()):
@@ -299,17 +300,16 @@ def beam_select(logits, scores, *, width, k=None, finished=None, pad_id=0, eos_i
     so = s_out.data_ptr()
     if k != width and n and (so == sp or fo and fo == fp):
         _bad(f"{who}: scores or finished in place need k == width")
-    ws = None
-
-    def desc():
-        nonlocal ws
-        need = _select_ws(b, width, vocab, k)
-        ws = torch.empty(need, dtype=torch.uint8, device=logits.device)  # of this call alone, from the current stream's memory
-        return _SELECT.pack(logits.data_ptr(), max(ldx, vocab), bf, b, width, vocab, k, sp, fp, pad_id if fp else 0, so, p_out.data_ptr(),
-                            t_out.data_ptr(), fo, -1 if eos_id is None else eos_id, ws.data_ptr(), need)
-
-    if b:
-        _launch(who, "slx_beam_select", desc, logits, scores, finished, finished_out, s_out, p_out, t_out)
+    dev = _device(who, logits, scores, s_out, p_out, t_out, finished, finished_out)
+    if not b:
+        return out
+    need = _select_ws(b, width, vocab, k)
+    ws = torch.empty(need, dtype=torch.uint8, device=logits.device)  # of this call alone, from the current stream's memory
+    rc = K.lib().slx_beam_select(_SELECT.pack(logits.data_ptr(), max(ldx, vocab), bf, b, width, vocab, k, sp, fp, pad_id if fp else 0, so,
+                                              p_out.data_ptr(), t_out.data_ptr(), fo, -1 if eos_id is None else eos_id, ws.data_ptr(), need),
+                                 _raw_stream(dev))
+    if rc:
+        K.check(rc, "slx_beam_select")
     return out
 
 
@@ -371,5 +371,7 @@ def beam_reorder(x, parent, *, dim=0, out=None):
     outer += ((1, 0, 0), (1, 0, 0))
     (n1, s1, d1), (n0, s0, d0) = outer[:2]
     desc = _REORDER.pack(xp, op, s0 * es, s1 * es, ss[dim] * es, d0 * es, d1 * es, ds[dim] * es, run * es, n0, n1, b, w, parent.data_ptr())
-    _launch(who, "slx_beam_reorder", desc, x, out, parent)
+    rc = K.lib().slx_beam_reorder(desc, _raw_stream(_device(who, x, out, parent)))
+    if rc:
+        K.check(rc, "slx_beam_reorder")
     return out
