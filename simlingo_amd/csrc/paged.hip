@@ -108,7 +108,7 @@ __global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs a) {
 //     (K's next tile is requested once the scores have used the last, V's after the output has), the waves' states are
 //     merged through LDS at the end. Few rows: the bytes in flight count, and no wave waits for another.
 //   streamed (more rows): 64 or 128 rows, 16 or 32 a wave, so the keys are fetched once for all of them: tiles of 32 keys
-//     arrive by LDS-DMA in a ring of 4, one barrier a tile. Rows of K and V lie in LDS with their 16-B chunks XOR-ed by
+//     arrive by LDS-DMA in a ring, one barrier a step. Rows of K and V lie in LDS with their 16-B chunks XOR-ed by
 //     the slot (and slots with bits 0 and 2 swapped), which keeps both operands' reads free of bank conflicts. One page
 //     number a wave and tile (scalar load), so pages of at least 8 slots; smaller ones take the direct form.
 struct Seg {
@@ -248,14 +248,14 @@ __device__ __forceinline__ void mask_scores(f32x4 (&s)[NQ][2], unsigned dead, co
   }
 }
 
-// Scores to probabilities, with the state rescaled where a row's maximum has moved.
-template <int D, int NQ>
-__device__ __forceinline__ void softmax_step(const f32x4 (&s)[NQ][2], float c, State<D, NQ>& st, bf16x8 (&pb)[NQ]) {
+// Scores of T tiles to probabilities, with the state rescaled where a row's maximum has moved.
+template <int D, int NQ, int T>
+__device__ __forceinline__ void softmax_step(const f32x4 (&s)[T][NQ][2], float c, State<D, NQ>& st, bf16x8 (&pb)[T][NQ]) {
 #pragma unroll
   for (int n = 0; n < NQ; ++n) {
-    float mx = s[n][0][0];
+    float mx = s[0][n][0][0];
 #pragma unroll
-    for (int j = 1; j < 8; ++j) mx = fmaxf(mx, s[n][j >> 2][j & 3]);
+    for (int j = 1; j < 8 * T; ++j) mx = fmaxf(mx, s[j >> 3][n][j >> 2 & 1][j & 3]);
     mx *= c;
     // the running maximum moves only when a score passes it by 2^8 (exact all the same: it cancels in o / l)
     if (__any(mx > st.m[n] + 8.0f)) {
@@ -272,7 +272,9 @@ __device__ __forceinline__ void softmax_step(const f32x4 (&s)[NQ][2], float c, S
     // P in bf16 for the MFMA (half a step, 2^-8 of each term at most, as the output itself is rounded); l sums the same
     // rounded values, so what is left is the terms' own scatter
 #pragma unroll
-    for (int j = 0; j < 8; ++j) pb[n][j] = (bf16)__builtin_amdgcn_exp2f(__builtin_fmaf(s[n][j >> 2][j & 3], c, -mu));
+    for (int u = 0; u < T; ++u)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) pb[u][n][j] = (bf16)__builtin_amdgcn_exp2f(__builtin_fmaf(s[u][n][j >> 2][j & 3], c, -mu));
   }
 }
 
@@ -455,25 +457,25 @@ __device__ __forceinline__ void attn_direct(const PAttnArgs& a, Item w, char* sm
     entries_v(k0 + 128);
   }
   for (; k0 < ke; k0 += 128) {
-    f32x4 s[NQ][2];
-    bf16x8 pb[NQ];
-    scores<D, NQ>(kf, qf, s);
+    f32x4 s[1][NQ][2];
+    bf16x8 pb[1][NQ];
+    scores<D, NQ>(kf, qf, s[0]);
     const bool edge = k0 + 32 > free_end || __any(bad != 0);
     unsigned dead = bad;
     if (edge) {
       const int left = w.len - k0 - 4 * grp;
 #pragma unroll
       for (int j = 0; j < 8; ++j) dead |= (16 * (j >> 2) + (j & 3) >= left ? 1u : 0u) << j;
-      mask_scores<NQ>(s, dead, lim, k0);
+      mask_scores<NQ>(s[0], dead, lim, k0);
     }
     const bool more = k0 + 128 < ke;
     if (more) {
       load_k(k0 + 128);
       entries_k(k0 + 256);
     }
-    softmax_step<D, NQ>(s, a.c, st, pb);
+    softmax_step<D, NQ, 1>(s, a.c, st, pb);
     if (edge) odd = clean_v<D>(vr, dead, w.causal && a.Tq > 1) || odd;
-    output_step<D, NQ>(vr, pb, st);
+    output_step<D, NQ>(vr, pb[0], st);
     if (more) {
       load_v(k0 + 128);
       entries_v(k0 + 256);
@@ -540,7 +542,6 @@ __device__ __forceinline__ void attn_direct(const PAttnArgs& a, Item w, char* sm
   }
 }
 
-constexpr int kRing = 4;
 template <int N>
 __device__ __forceinline__ void wait_vm() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
 // this wave's pieces of the oldest tile are in LDS, with up to N younger tiles of PER pieces under way
@@ -549,57 +550,74 @@ __device__ __forceinline__ void wait_tiles(int younger) {
   if (younger >= N) wait_vm<N * PER>();
   else if constexpr (N > 0) wait_tiles<N - 1, PER>(younger);
 }
-// 16 B a lane from global memory to LDS at the wave's base + 16 * lane (m0: the base)
-__device__ __forceinline__ void dma16(const void* g, const char* lds) {
-  const unsigned m = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)LDS_PTR(const char, lds));
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(m), "v"(g) : "memory");
+// 16 B a lane from base + off (bytes) to LDS at lds + 16 * lane
+__device__ __forceinline__ void dma16(const void* base, unsigned off, unsigned lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base) : "memory");
 }
+// tiles of 32 keys a step of the ring: two of 64-element heads, so that one wave has independent products to run
+constexpr int ring_tiles(int D) { return D == 64 ? 2 : 1; }
+constexpr int ring_slots(int D) { return D == 64 ? 3 : 4; }
+constexpr int ring_lds(int D) { return ring_slots(D) * (ring_tiles(D) * 2 * 32 * D * 2 + 4 * ring_tiles(D)); }
 
 // The keys of one segment into the state of a wave's rows r0 .. (the workgroup's from rw); whether values were sifted out.
 // The LDS is free when it is called, and its last tiles may still be read when it returns.
 template <int D, int NQ>
 __device__ __forceinline__ bool stream_keys(const PAttnArgs& a, const Item& w, int rw, int r0, const bf16x8 (&qf)[NQ][D / 32],
                                             State<D, NQ>& st, char* smem) {
-  constexpr int KK = D / 32, NE = D / 16, CH = D / 8, TILE = 32 * D * 2, PER = 2 * D / 64;  // PER: DMA pieces a wave and tile
+  constexpr int KK = D / 32, NE = D / 16, CH = D / 8, TILE = 32 * D * 2, T = ring_tiles(D), SLOTS = ring_slots(D), STEP = 32 * T;
+  constexpr int PER = T * 2 * D / 64;  // DMA pieces a wave and step
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, grp = lane >> 4;
   const int rows = w.ntok * a.gq, shift = w.shift, mask = (1 << shift) - 1;
-  unsigned char* badb = reinterpret_cast<unsigned char*>(smem + kRing * 2 * TILE);  // [kRing][4]: 8 keys a wave, 0 or 255
+  unsigned char* badb = reinterpret_cast<unsigned char*>(smem + SLOTS * T * 2 * TILE);  // [SLOTS][T][4]: 8 keys a wave, 0 or 255
+  const unsigned lds0 = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)LDS_PTR(char, smem));
   int lim[NQ];
   row_limits<NQ>(a, w, r0, lim);
   auto tok_of = [&](int r) { return row_token(a, min(r, rows - 1)); };
   const int free_end = w.causal ? min(w.ke, w.len - a.Tq + tok_of(r0) + 1) : w.ke;  // seen by every row of the wave
   const int ke = w.causal ? min(w.ke, w.len - a.Tq + tok_of(rw + 64 * NQ - 1) + 1) : w.ke;
   const int kw = r0 >= rows ? 0 : w.causal ? min(w.ke, w.len - a.Tq + tok_of(r0 + 16 * NQ - 1) + 1) : w.ke;  // this wave's last
-  const int nt = ke > w.kb ? (ke - w.kb + 31) / 32 : 0;
+  const int nt = ke > w.kb ? (ke - w.kb + STEP - 1) / STEP : 0;
   // LDS rows: slot of key x = x with bits 0 and 2 swapped; chunk c of a slot lies at c ^ swz(slot)
   auto slot_of = [](int x) { return (x & ~5) | (x & 1) << 2 | (x >> 2 & 1); };
   auto swz = [](int slot) { return D == 64 ? slot >> 1 & 7 : slot & 15; };
   typedef const int __attribute__((address_space(4))) cint;
-  auto entry = [&](int t) {  // the page of this wave's 8 keys of tile t
-    const int key = min(w.kb + 32 * min(t, nt - 1) + 8 * wave, w.len - 1);
+  auto entry = [&](int t, int u) {  // the page of this wave's 8 keys of tile u of step t
+    const int key = min(w.kb + STEP * min(t, nt - 1) + 32 * u + 8 * wave, w.len - 1);
     return ((cint*)(uintptr_t)w.tab)[__builtin_amdgcn_readfirstlane(key >> shift)];
   };
-  auto issue = [&](int t, int e) {
-    char* base = smem + (t % kRing) * 2 * TILE;
-    const bool ok = (unsigned)e < (unsigned)w.n_pages;
-    const long page = ok ? (long)e * w.ps : 0L;
-    if (lane == 0) badb[(t % kRing) * 4 + wave] = ok ? 0 : 255;
+  // A piece is 1 KiB: the wave's 8 keys lie on one page, so its address is a scalar and the lane's place among them.
+  unsigned off[PER / (2 * T)];
 #pragma unroll
-    for (int i = 0; i < PER / 2; ++i) {
-      const int slot = 8 * wave + (64 / CH) * i + lane / CH, key = slot_of(slot), ch = (lane % CH) ^ swz(slot);
-      const long off = page + (long)((w.kb + 32 * t + key) & mask) * w.ss + 8 * ch;
-      dma16(w.k + off, base + (8 * wave + (64 / CH) * i) * D * 2);
-      dma16(w.v + off, base + TILE + (8 * wave + (64 / CH) * i) * D * 2);
+  for (int i = 0; i < PER / (2 * T); ++i) {
+    const int slot = 8 * wave + (64 / CH) * i + lane / CH;
+    off[i] = 2u * ((unsigned)(slot_of(slot) & 7) * (unsigned)w.ss + 8u * (unsigned)((lane % CH) ^ swz(slot)));
+  }
+  auto issue = [&](int t, const int (&e)[T]) {
+#pragma unroll
+    for (int u = 0; u < T; ++u) {
+      const int at = (t % SLOTS) * T + u;
+      const bool ok = (unsigned)e[u] < (unsigned)w.n_pages;
+      const long from = (ok ? (long)e[u] * w.ps : 0L) + (long)((w.kb + STEP * t + 32 * u + 8 * wave) & mask) * w.ss;
+      if (lane == 0) badb[at * 4 + wave] = ok ? 0 : 255;
+#pragma unroll
+      for (int i = 0; i < PER / (2 * T); ++i) {
+        const unsigned to = lds0 + at * 2 * TILE + (8 * wave + (64 / CH) * i) * D * 2;
+        dma16(w.k + from, off[i], to);
+        dma16(w.v + from, off[i], to + TILE);
+      }
     }
   };
-  int en = 0;
+  int en[T];
   if (nt > 0) {
-    int e[kRing - 1];
+    int e[SLOTS - 1][T];
 #pragma unroll
-    for (int i = 0; i < kRing - 1; ++i) e[i] = entry(i);
-    en = entry(kRing - 1);
+    for (int i = 0; i < SLOTS - 1; ++i)
 #pragma unroll
-    for (int i = 0; i < kRing - 1; ++i)
+      for (int u = 0; u < T; ++u) e[i][u] = entry(i, u);
+#pragma unroll
+    for (int u = 0; u < T; ++u) en[u] = entry(SLOTS - 1, u);
+#pragma unroll
+    for (int i = 0; i < SLOTS - 1; ++i)
       if (i < nt) issue(i, e[i]);
   }
   int ko[KK], vo[8];  // this lane's operands within a tile
@@ -612,51 +630,69 @@ __device__ __forceinline__ bool stream_keys(const PAttnArgs& a, const Item& w, i
   }
   bool odd = false;
   for (int t = 0; t < nt; ++t) {
-    const int k0 = w.kb + 32 * t;
-    wait_tiles<kRing - 2, PER>(nt - 1 - t);
+    const int k0 = w.kb + STEP * t;
+    wait_tiles<SLOTS - 2, PER>(nt - 1 - t);
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // this wave has read the slot that is filled next
     __builtin_amdgcn_s_barrier();
-    if (t + kRing - 1 < nt) {
-      issue(t + kRing - 1, en);
-      en = entry(t + kRing);
+    if (t + SLOTS - 1 < nt) {
+      issue(t + SLOTS - 1, en);
+#pragma unroll
+      for (int u = 0; u < T; ++u) en[u] = entry(t + SLOTS, u);
     }
     if (k0 >= kw) continue;
-    const char* tile = smem + (t % kRing) * 2 * TILE;
-    const unsigned bads = *reinterpret_cast<const unsigned*>(badb + (t % kRing) * 4);
-    bf16x8 kf[2][KK];
+    f32x4 s[T][NQ][2];
+    bf16x8 pb[T][NQ];
+    unsigned vr[T][8][NE / 2], bads[T], dead[T];
 #pragma unroll
-    for (int k = 0; k < KK; ++k) {  // keys 16 apart lie 16 slots apart, under the same swizzle
-      kf[0][k] = *reinterpret_cast<const bf16x8*>(tile + ko[k]);
-      kf[1][k] = *reinterpret_cast<const bf16x8*>(tile + ko[k] + 16 * D * 2);
-    }
-    f32x4 s[NQ][2];
-    bf16x8 pb[NQ];
-    unsigned vr[8][NE / 2];
-    scores<D, NQ>(kf, qf, s);
+    for (int u = 0; u < T; ++u) {
+      const char* tile = smem + ((t % SLOTS) * T + u) * 2 * TILE;
+      bads[u] = *reinterpret_cast<const unsigned*>(badb + ((t % SLOTS) * T + u) * 4);
+      bf16x8 kf[2][KK];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      if constexpr (NE == 4) {
-        const u32x2 x = *reinterpret_cast<const u32x2*>(tile + vo[j]);
-        vr[j][0] = x[0]; vr[j][1] = x[1];
-      } else {
-        const u32x4 x = *reinterpret_cast<const u32x4*>(tile + vo[j]);
-#pragma unroll
-        for (int i = 0; i < NE / 2; ++i) vr[j][i] = x[i];
+      for (int k = 0; k < KK; ++k) {  // keys 16 apart lie 16 slots apart, under the same swizzle
+        kf[0][k] = *reinterpret_cast<const bf16x8*>(tile + ko[k]);
+        kf[1][k] = *reinterpret_cast<const bf16x8*>(tile + ko[k] + 16 * D * 2);
       }
+      scores<D, NQ>(kf, qf, s[u]);
     }
-    const bool edge = k0 + 32 > free_end || __builtin_amdgcn_readfirstlane(bads) != 0;
-    unsigned dead = 0;
-    if (edge) {
+#pragma unroll
+    for (int u = 0; u < T; ++u) {
+      const char* tile = smem + ((t % SLOTS) * T + u) * 2 * TILE;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const int x = 16 * (j >> 2) + 4 * grp + (j & 3);
-        dead |= (k0 + x >= w.len || (bads >> x & 1) ? 1u : 0u) << j;
+        if constexpr (NE == 4) {
+          const u32x2 x = *reinterpret_cast<const u32x2*>(tile + vo[j]);
+          vr[u][j][0] = x[0]; vr[u][j][1] = x[1];
+        } else {
+          const u32x4 x = *reinterpret_cast<const u32x4*>(tile + vo[j]);
+#pragma unroll
+          for (int i = 0; i < NE / 2; ++i) vr[u][j][i] = x[i];
+        }
       }
-      mask_scores<NQ>(s, dead, lim, k0);
     }
-    softmax_step<D, NQ>(s, a.c, st, pb);
-    if (edge) odd = clean_v<D>(vr, dead, w.causal && a.Tq > 1) || odd;
-    output_step<D, NQ>(vr, pb, st);
+    unsigned any_bad = 0;
+#pragma unroll
+    for (int u = 0; u < T; ++u) any_bad |= bads[u];
+    const bool edge = k0 + STEP > free_end || __builtin_amdgcn_readfirstlane(any_bad) != 0;
+    if (edge) {
+#pragma unroll
+      for (int u = 0; u < T; ++u) {
+        dead[u] = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const int x = 16 * (j >> 2) + 4 * grp + (j & 3);
+          dead[u] |= (k0 + 32 * u + x >= w.len || (bads[u] >> x & 1) ? 1u : 0u) << j;
+        }
+        mask_scores<NQ>(s[u], dead[u], lim, k0 + 32 * u);
+      }
+    }
+    softmax_step<D, NQ, T>(s, a.c, st, pb);
+    if (edge) {
+#pragma unroll
+      for (int u = 0; u < T; ++u) odd = clean_v<D>(vr[u], dead[u], w.causal && a.Tq > 1) || odd;
+    }
+#pragma unroll
+    for (int u = 0; u < T; ++u) output_step<D, NQ>(vr[u], pb[u], st);
   }
   return odd;
 }
@@ -708,7 +744,7 @@ __device__ __forceinline__ void attn_kind(const PAttnArgs& a, const Item& w, cha
   else attn_stream<D, 2>(a, w, smem);
 }
 constexpr int kind_lds(int D, int kind) {
-  return kind >= kS64 ? kRing * 2 * 32 * D * 2 + 4 * kRing : 2 * 4 * 16 * (kind + 1) * 4 + 2 * (kind + 1) * (D / 16) * 64 * 16;
+  return kind >= kS64 ? ring_lds(D) : 2 * 4 * 16 * (kind + 1) * 4 + 2 * (kind + 1) * (D / 16) * 64 * 16;
 }
 
 template <int D, int KP, int KO>
@@ -756,7 +792,7 @@ __global__ __launch_bounds__(256, 2) void prefix_attn_kernel(PAttnArgs a) {
 // keys, so there are no parts to write and join (the prefix is fetched again for every tile of rows, from L2).
 template <int D, int NQ>
 __global__ __launch_bounds__(256, 2) void prefix_attn_whole_kernel(PAttnArgs a) {
-  __shared__ __attribute__((aligned(16))) char smem[kRing * 2 * 32 * D * 2 + 4 * kRing];
+  __shared__ __attribute__((aligned(16))) char smem[ring_lds(D)];
   unsigned b = blockIdx.x;  // [kv head][sequence][row tile]: neighbours share the prefix
   Item w;
   w.mt = (int)(b % (unsigned)a.mt_own);
@@ -862,12 +898,16 @@ struct PAttnPlan { int kp, ko, mtp, mto, nsp, nso, whole; };
 static PAttnPlan plan_attn(const slx_prefix_attn_desc* d, int capp, int capo) {
   PAttnPlan p;
   const int gq = d->Hq / d->own_pool.heads;
-  auto kind = [](long rows, int page) { return rows <= 16 ? kD16 : rows <= 32 || page < 8 ? kD32 : rows <= 64 ? kS64 : kS128; };
+  auto kind = [](long rows, const slx_kv_pool& pool) {
+    // streamed tiles: one page number for 8 keys, whose offsets on the page fit 32 bits
+    const bool streams = pool.page >= 8 && pool.slot_stride < (1 << 27);
+    return rows <= 16 ? kD16 : rows <= 32 || !streams ? kD32 : rows <= 64 ? kS64 : kS128;
+  };
   const long rp = (long)d->width * d->n_q * gq, ro = (long)d->n_q * gq, heads = d->own_pool.heads;
   const long seqs = (long)d->groups * d->width * heads, t64 = (ro + 63) / 64, t128 = (ro + 127) / 128;
   p.whole = 0;
-  p.ko = kind(ro, d->own_pool.page);
-  p.kp = capp > 0 ? kind(rp, d->prefix_pool.page) : p.ko;
+  p.ko = kind(ro, d->own_pool);
+  p.kp = capp > 0 ? kind(rp, d->prefix_pool) : p.ko;
   if (capp > 0 && p.kp >= kS64 && p.ko >= kS64 && seqs * t64 >= kWhole) {
     p.whole = 1;
     p.ko = p.kp = seqs * t128 >= 2 * kWhole ? kS128 : kS64;

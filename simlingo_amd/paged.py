@@ -97,35 +97,35 @@ def _device(who, first, *rest):
 
 
 def _i32(who, name, t, n):
-    if not (t.dtype is I32 and t.dim() == 1 and t.shape[0] == n and t.is_contiguous()):
+    if t.dtype is not I32 or t.numel() != n or t.dim() != 1 or not t.is_contiguous():
         _bad(f"{who}: {name} must be contiguous int32 [{n}]")
 
 
 def _rows(who, name, t, n, cols):
     """A bf16 matrix view of n rows that are contiguous and 16-B aligned -> its address and row stride."""
-    if t.dtype is not BF16 or t.dim() != 2:
+    sh, st, p = t.shape, t.stride(), t.data_ptr()
+    if t.dtype is not BF16 or len(sh) != 2:
         _bad(f"{who}: {name} must be a bf16 matrix")
-    (m, c), (s0, s1), p = t.shape, t.stride(), t.data_ptr()
-    if m != n or c < cols:
-        _bad(f"{who}: {name} must have {n} rows of at least {cols}, got {m} x {c}")
-    if s1 != 1 or s0 % 8 or p % 16:
+    if sh[0] != n or sh[1] < cols:
+        _bad(f"{who}: {name} must have {n} rows of at least {cols}, got {list(sh)}")
+    s0, s1 = st
+    if s1 != 1 or (s0 * 2 | p) & 15:
         _bad(f"{who}: rows of {name} must be contiguous and 16-B aligned")
     return p, s0
 
 
 def _pool(who, k, v, written=False):
     """The fields of slx_kv_pool for a cache k, v [pages, page, heads, head size]."""
-    sh, st = k.shape, k.stride()
+    sh, st, kp, vp = k.shape, k.stride(), k.data_ptr(), v.data_ptr()
     if k.dtype is not BF16 or v.dtype is not BF16 or len(sh) != 4:
         _bad(f"{who}: k and v must be bf16 [pages, page, heads, head size]")
     if sh != v.shape or st != v.stride():
         _bad(f"{who}: k and v must have the same shape and strides")
     n, page, heads, d = sh
     s0, s1, s2, s3 = st
-    if not (n > 0 and page > 0 and page & (page - 1) == 0 and heads > 0 and (d == 64 or d == 128)):
+    if n < 1 or page < 1 or page & (page - 1) or heads < 1 or d != 64 and d != 128:
         _bad(f"{who}: pages and heads > 0, page a power of two, head size 64 or 128 (got {list(sh)})")
-    kp, vp = k.data_ptr(), v.data_ptr()
-    if s3 != 1 or (s0 | s1 | s2) % 8 or (kp | vp) % 16:
+    if s3 != 1 or ((s0 | s1 | s2) * 2 | kp | vp) & 15:
         _bad(f"{who}: heads of k and v must be contiguous and 16-B aligned")
     if written and not ((s0 or n == 1) and (s1 or page == 1) and (s2 or heads == 1)):
         _bad(f"{who}: k and v must not be expanded")
@@ -134,12 +134,14 @@ def _pool(who, k, v, written=False):
 
 def _table(who, name, t):
     """Address, row stride, rows and columns of a page table."""
-    if t.dtype is not I32 or t.dim() != 2:
+    sh, st = t.shape, t.stride()
+    if t.dtype is not I32 or len(sh) != 2:
         _bad(f"{who}: {name} must be int32 [sequences, columns]")
-    (n, cols), (s0, s1) = t.shape, t.stride()
+    n, cols = sh
+    s0, s1 = st
     if cols < 1 or s1 != 1 and cols > 1 or s0 < cols and n > 1:
         _bad(f"{who}: {name} must have columns, its rows contiguous and apart")
-    return t.data_ptr(), max(s0, cols), n, cols
+    return t.data_ptr(), s0 if s0 > cols else cols, n, cols
 
 
 def kv_append(qkv, k, v, table, pos, q_out=None, *, n_heads, cos=None, sin=None, seq=None, rows_per_seq=1):
@@ -169,9 +171,10 @@ def kv_append(qkv, k, v, table, pos, q_out=None, *, n_heads, cos=None, sin=None,
         if cos is not sin:
             _bad(f"{who}: cos and sin go together")
     else:
-        rope, c, s = cos.shape[0], cos.data_ptr(), sin.data_ptr()
-        if not (cos.dtype is F32 and sin.dtype is F32 and cos.dim() == 2 and cos.shape[1] == d // 2 and sin.shape == cos.shape and rope > 0
-                and cos.is_contiguous() and sin.is_contiguous() and (c | s) % 16 == 0):
+        sh, c, s = cos.shape, cos.data_ptr(), sin.data_ptr()
+        rope = sh[0]
+        if not (cos.dtype is F32 and sin.dtype is F32 and sh == sin.shape and len(sh) == 2 and sh[1] == d // 2 and rope > 0
+                and cos.is_contiguous() and sin.is_contiguous() and not (c | s) & 15):
             _bad(f"{who}: cos and sin must be contiguous f32 [positions, {d // 2}]")
     desc = _APPEND.pack(*pool, x, ldx, q, ldq, tab, ldt, n_seq, cols, seq.data_ptr() if seq is not None else 0, pos.data_ptr(),
                         rows_per_seq, n_heads, rows, c, s, rope)
