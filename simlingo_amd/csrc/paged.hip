@@ -561,11 +561,13 @@ constexpr int ring_lds(int D) { return ring_slots(D) * (ring_tiles(D) * 2 * 32 *
 
 // The keys of one segment into the state of a wave's rows r0 .. (the workgroup's from rw); whether values were sifted out.
 // The LDS is free when it is called, and its last tiles may still be read when it returns.
-template <int D, int NQ>
+template <int D, int NQ, bool TEAM>
 __device__ __forceinline__ bool stream_keys(const PAttnArgs& a, const Item& w, int rw, int r0, const bf16x8 (&qf)[NQ][D / 32],
                                             State<D, NQ>& st, char* smem) {
   constexpr int KK = D / 32, NE = D / 16, CH = D / 8, TILE = 32 * D * 2, T = ring_tiles(D), SLOTS = ring_slots(D), STEP = 32 * T;
   constexpr int PER = T * 2 * D / 64;  // DMA pieces a wave and step
+  constexpr int RW = (TEAM ? 32 : 64) * NQ, UW = TEAM ? 1 : T;  // rows of the workgroup; tiles of a step that a wave takes
+  static_assert(!TEAM || T == 2, "one tile of a step for each team");
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, grp = lane >> 4;
   const int rows = w.ntok * a.gq, shift = w.shift, mask = (1 << shift) - 1;
   unsigned char* badb = reinterpret_cast<unsigned char*>(smem + SLOTS * T * 2 * TILE);  // [SLOTS][T][4]: 8 keys a wave, 0 or 255
@@ -574,7 +576,7 @@ __device__ __forceinline__ bool stream_keys(const PAttnArgs& a, const Item& w, i
   row_limits<NQ>(a, w, r0, lim);
   auto tok_of = [&](int r) { return row_token(a, min(r, rows - 1)); };
   const int free_end = w.causal ? min(w.ke, w.len - a.Tq + tok_of(r0) + 1) : w.ke;  // seen by every row of the wave
-  const int ke = w.causal ? min(w.ke, w.len - a.Tq + tok_of(rw + 64 * NQ - 1) + 1) : w.ke;
+  const int ke = w.causal ? min(w.ke, w.len - a.Tq + tok_of(rw + RW - 1) + 1) : w.ke;
   const int kw = r0 >= rows ? 0 : w.causal ? min(w.ke, w.len - a.Tq + tok_of(r0 + 16 * NQ - 1) + 1) : w.ke;  // this wave's last
   const int nt = ke > w.kb ? (ke - w.kb + STEP - 1) / STEP : 0;
   // LDS rows: slot of key x = x with bits 0 and 2 swapped; chunk c of a slot lies at c ^ swz(slot)
@@ -639,60 +641,62 @@ __device__ __forceinline__ bool stream_keys(const PAttnArgs& a, const Item& w, i
 #pragma unroll
       for (int u = 0; u < T; ++u) en[u] = entry(t + SLOTS, u);
     }
-    if (k0 >= kw) continue;
-    f32x4 s[T][NQ][2];
-    bf16x8 pb[T][NQ];
-    unsigned vr[T][8][NE / 2], bads[T], dead[T];
+    const int u0 = TEAM ? wave >> 1 : 0;
+    if (k0 + 32 * u0 >= kw) continue;
+    f32x4 s[UW][NQ][2];
+    bf16x8 pb[UW][NQ];
+    unsigned vr[UW][8][NE / 2], bads[UW], dead[UW];
 #pragma unroll
-    for (int u = 0; u < T; ++u) {
-      const char* tile = smem + ((t % SLOTS) * T + u) * 2 * TILE;
-      bads[u] = *reinterpret_cast<const unsigned*>(badb + ((t % SLOTS) * T + u) * 4);
+    for (int v = 0; v < UW; ++v) {
+      const char* tile = smem + ((t % SLOTS) * T + u0 + v) * 2 * TILE;
+      bads[v] = *reinterpret_cast<const unsigned*>(badb + ((t % SLOTS) * T + u0 + v) * 4);
       bf16x8 kf[2][KK];
 #pragma unroll
       for (int k = 0; k < KK; ++k) {  // keys 16 apart lie 16 slots apart, under the same swizzle
         kf[0][k] = *reinterpret_cast<const bf16x8*>(tile + ko[k]);
         kf[1][k] = *reinterpret_cast<const bf16x8*>(tile + ko[k] + 16 * D * 2);
       }
-      scores<D, NQ>(kf, qf, s[u]);
+      scores<D, NQ>(kf, qf, s[v]);
     }
 #pragma unroll
-    for (int u = 0; u < T; ++u) {
-      const char* tile = smem + ((t % SLOTS) * T + u) * 2 * TILE;
+    for (int v = 0; v < UW; ++v) {
+      const char* tile = smem + ((t % SLOTS) * T + u0 + v) * 2 * TILE;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         if constexpr (NE == 4) {
           const u32x2 x = *reinterpret_cast<const u32x2*>(tile + vo[j]);
-          vr[u][j][0] = x[0]; vr[u][j][1] = x[1];
+          vr[v][j][0] = x[0]; vr[v][j][1] = x[1];
         } else {
           const u32x4 x = *reinterpret_cast<const u32x4*>(tile + vo[j]);
 #pragma unroll
-          for (int i = 0; i < NE / 2; ++i) vr[u][j][i] = x[i];
+          for (int i = 0; i < NE / 2; ++i) vr[v][j][i] = x[i];
         }
       }
     }
     unsigned any_bad = 0;
 #pragma unroll
-    for (int u = 0; u < T; ++u) any_bad |= bads[u];
-    const bool edge = k0 + STEP > free_end || __builtin_amdgcn_readfirstlane(any_bad) != 0;
+    for (int v = 0; v < UW; ++v) any_bad |= bads[v];
+    const bool edge = k0 + 32 * (u0 + UW) > free_end || __builtin_amdgcn_readfirstlane(any_bad) != 0;
     if (edge) {
 #pragma unroll
-      for (int u = 0; u < T; ++u) {
-        dead[u] = 0;
+      for (int v = 0; v < UW; ++v) {
+        const int kv = k0 + 32 * (u0 + v);
+        dead[v] = 0;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           const int x = 16 * (j >> 2) + 4 * grp + (j & 3);
-          dead[u] |= (k0 + 32 * u + x >= w.len || (bads[u] >> x & 1) ? 1u : 0u) << j;
+          dead[v] |= (kv + x >= w.len || (bads[v] >> x & 1) ? 1u : 0u) << j;
         }
-        mask_scores<NQ>(s[u], dead[u], lim, k0 + 32 * u);
+        mask_scores<NQ>(s[v], dead[v], lim, kv);
       }
     }
-    softmax_step<D, NQ, T>(s, a.c, st, pb);
+    softmax_step<D, NQ, UW>(s, a.c, st, pb);
     if (edge) {
 #pragma unroll
-      for (int u = 0; u < T; ++u) odd = clean_v<D>(vr[u], dead[u], w.causal && a.Tq > 1) || odd;
+      for (int v = 0; v < UW; ++v) odd = clean_v<D>(vr[v], dead[v], w.causal && a.Tq > 1) || odd;
     }
 #pragma unroll
-    for (int u = 0; u < T; ++u) output_step<D, NQ>(vr[u], pb[u], st);
+    for (int v = 0; v < UW; ++v) output_step<D, NQ>(vr[v], pb[v], st);
   }
   return odd;
 }
@@ -707,30 +711,76 @@ __device__ __forceinline__ void settle_rows(bf16x8 (&qf)[NQ][D / 32]) {
     for (int k = 0; k < D / 32; ++k) asm volatile("" : "+v"(qf[n][k]));
 }
 
-template <int D, int NQ>
-__device__ __forceinline__ void store_stream(const PAttnArgs& a, const Item& w, int r0, bool odd, const State<D, NQ>& st) {
+// What a streamed workgroup of 64 or 128 rows is: 16 rows a wave (128-element heads) or 32; and for 64 rows of 64-element
+// heads two teams of two waves, each with 32 rows a wave and one tile of every step (an operand read from LDS serves 32 rows
+// instead of 16), joined at the end.
+template <int D, int RW>
+struct Stream {
+  static constexpr bool team = D == 64 && RW == 64;
+  static constexpr int NQ = team ? 2 : RW / 64;
+};
+
+template <int D, int RW>
+__device__ __forceinline__ void store_stream(const PAttnArgs& a, const Item& w, int r0, bool odd, State<D, Stream<D, RW>::NQ>& st,
+                                             char* smem) {
+  constexpr int NQ = Stream<D, RW>::NQ, NE = D / 16;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15;
   odd = __any(odd);
+  if constexpr (Stream<D, RW>::team) {
+    f32x4* so = reinterpret_cast<f32x4*>(smem) + (wave & 1) * NQ * (NE + 1) * 64;  // [rows' wave][NQ][NE + 1][lane]
+    __syncthreads();
+    if (wave >= 2) {
+#pragma unroll
+      for (int n = 0; n < NQ; ++n) {
+#pragma unroll
+        for (int e = 0; e < NE; ++e) so[(n * (NE + 1) + e) * 64 + lane] = st.o[n][e];
+        so[(n * (NE + 1) + NE) * 64 + lane] = f32x4{st.m[n], st.l[n][0], odd ? 1.f : 0.f, 0.f};
+      }
+    }
+    __syncthreads();
+    if (wave >= 2) return;
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+      const f32x4 x = so[(n * (NE + 1) + NE) * 64 + lane];
+      const float M = fmaxf(st.m[n], x[0]);
+      const float r0_ = st.m[n] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(st.m[n] - M);
+      const float r1_ = x[0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(x[0] - M);
+      st.l[n][0] = st.l[n][0] * r0_ + x[1] * r1_;
+      st.m[n] = M;
+      odd = odd || x[2] != 0.f;
+#pragma unroll
+      for (int e = 0; e < NE; ++e) st.o[n][e] = st.o[n][e] * r0_ + so[(n * (NE + 1) + e) * 64 + lane] * r1_;
+    }
+    odd = __any(odd);
+  }
 #pragma unroll
   for (int n = 0; n < NQ; ++n) {
-    const int r = r0 + 16 * n + (threadIdx.x & 15);
+    const int r = r0 + 16 * n + col;
     if (r >= w.ntok * a.gq) continue;
     store_row<D>(a, w, r, st.m[n], st.l[n][0], st.o[n]);
     if (odd) add_nonfinite<D>(a, w, r);
   }
 }
 
-template <int D, int NQ>
+template <int D, int RW>
+__device__ __forceinline__ int wave_row(int rw) {  // a wave's first row
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  return rw + (Stream<D, RW>::team ? wave & 1 : wave) * 16 * Stream<D, RW>::NQ;
+}
+
+template <int D, int RW>
 __device__ __forceinline__ void attn_stream(const PAttnArgs& a, Item w, char* smem) {
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), rw = w.mt * 64 * NQ, r0 = rw + wave * 16 * NQ;
+  constexpr int NQ = Stream<D, RW>::NQ;
+  const int rw = w.mt * RW, r0 = wave_row<D, RW>(rw);
   bf16x8 qf[NQ][D / 32];
   load_rows<D, NQ>(a, w, r0, qf);
   asm volatile("" ::: "memory");  // the queries are requested before the length is waited for
-  if (!item_range(a, w, 64 * NQ)) return;
+  if (!item_range(a, w, RW)) return;
   State<D, NQ> st;
   state_init(st);
   settle_rows<D, NQ>(qf);
-  const bool odd = stream_keys<D, NQ>(a, w, rw, r0, qf, st, smem);
-  store_stream<D, NQ>(a, w, r0, odd, st);
+  const bool odd = stream_keys<D, NQ, Stream<D, RW>::team>(a, w, rw, r0, qf, st, smem);
+  store_stream<D, RW>(a, w, r0, odd, st, smem);
 }
 
 // kinds of a workgroup: direct with 16 or 32 rows, streamed with 64 or 128
@@ -740,8 +790,8 @@ template <int D, int KIND>
 __device__ __forceinline__ void attn_kind(const PAttnArgs& a, const Item& w, char* smem) {
   if constexpr (KIND == kD16) attn_direct<D, 1>(a, w, smem);
   else if constexpr (KIND == kD32) attn_direct<D, 2>(a, w, smem);
-  else if constexpr (KIND == kS64) attn_stream<D, 1>(a, w, smem);
-  else attn_stream<D, 2>(a, w, smem);
+  else if constexpr (KIND == kS64) attn_stream<D, 64>(a, w, smem);
+  else attn_stream<D, 128>(a, w, smem);
 }
 constexpr int kind_lds(int D, int kind) {
   return kind >= kS64 ? ring_lds(D) : 2 * 4 * 16 * (kind + 1) * 4 + 2 * (kind + 1) * (D / 16) * 64 * 16;
@@ -790,7 +840,7 @@ __global__ __launch_bounds__(256, 2) void prefix_attn_kernel(PAttnArgs a) {
 
 // Many new tokens in many sequences: a workgroup takes 64 or 128 rows of ONE sequence through the prefix and then its own
 // keys, so there are no parts to write and join (the prefix is fetched again for every tile of rows, from L2).
-template <int D, int NQ>
+template <int D, int RW>
 __global__ __launch_bounds__(256, 2) void prefix_attn_whole_kernel(PAttnArgs a) {
   __shared__ __attribute__((aligned(16))) char smem[ring_lds(D)];
   unsigned b = blockIdx.x;  // [kv head][sequence][row tile]: neighbours share the prefix
@@ -802,22 +852,23 @@ __global__ __launch_bounds__(256, 2) void prefix_attn_whole_kernel(PAttnArgs a) 
   w.tok0 = (long)seq * a.Tq;
   w.ntok = a.Tq;
   w.range = w.part = 0;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), rw = w.mt * 64 * NQ, r0 = rw + wave * 16 * NQ;
+  constexpr int NQ = Stream<D, RW>::NQ;
+  const int rw = w.mt * RW, r0 = wave_row<D, RW>(rw);
   bf16x8 qf[NQ][D / 32];
   load_rows<D, NQ>(a, w, r0, qf);
   asm volatile("" ::: "memory");  // the queries are requested before the lengths are waited for
   item_segment(w, a.pre, seq / (unsigned)a.W, false);
-  item_range(a, w, 64 * NQ);
+  item_range(a, w, RW);
   State<D, NQ> st;
   state_init(st);
   settle_rows<D, NQ>(qf);
-  stream_keys<D, NQ>(a, w, rw, r0, qf, st, smem);
+  stream_keys<D, NQ, Stream<D, RW>::team>(a, w, rw, r0, qf, st, smem);
   item_segment(w, a.own, seq, true);
-  item_range(a, w, 64 * NQ);
+  item_range(a, w, RW);
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the ring is free when every wave has read the prefix's last tiles
   __builtin_amdgcn_s_barrier();
-  const bool odd = stream_keys<D, NQ>(a, w, rw, r0, qf, st, smem);
-  store_stream<D, NQ>(a, w, r0, odd, st);
+  const bool odd = stream_keys<D, NQ, Stream<D, RW>::team>(a, w, rw, r0, qf, st, smem);
+  store_stream<D, RW>(a, w, r0, odd, st, smem);
 }
 
 // Joins the parts of a row: D / 4 threads, four d each, times PG groups that share the parts out, B at a time (8 parts at
@@ -972,8 +1023,8 @@ static int check_attn(const slx_prefix_attn_desc* d, int* capp, int* capo) {
 template <int D>
 static void launch_attn(const PAttnPlan& p, dim3 grid, hipStream_t st, const PAttnArgs& a) {
   if (p.whole) {
-    if (p.ko == kS128) hipLaunchKernelGGL((prefix_attn_whole_kernel<D, 2>), grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((prefix_attn_whole_kernel<D, 1>), grid, dim3(256), 0, st, a);
+    if (p.ko == kS128) hipLaunchKernelGGL((prefix_attn_whole_kernel<D, 128>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((prefix_attn_whole_kernel<D, 64>), grid, dim3(256), 0, st, a);
     return;
   }
 #define SLX_PA(P, O)                                                                                         \
