@@ -1,4 +1,4 @@
-"""In-tree build of libslx_hip.so (gfx950) with hipcc — no cmake, no JIT cache.
+"""In-tree build of libslx_hip.so (gfx950) with hipcc, and of the binding _paged.so with g++ — no cmake, no JIT cache.
 
 `python -m simlingo_amd.build` compiles every csrc/*.hip to an object (in parallel, incremental
 on mtime) and links the shared library next to the sources, so it travels with the repo snapshot
@@ -48,12 +48,32 @@ def _compile(src: Path, extra: list[str]) -> Path:
     return obj
 
 
+def _build_bind():
+    """simlingo_amd/_paged.so: the Python entry of the paged decode operators, host code against torch's headers."""
+    src, out = CSRC / "paged_bind.cpp", HERE / "_paged.so"
+    if not _needs(out, [src, INCLUDE / "slx.h"]):
+        return
+    import sysconfig
+
+    import torch
+    root = Path(torch.__file__).resolve().parent
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-shared", "-fPIC", "-Wall", "-Werror=return-type",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-isystem", str(root / "include"),
+           f"-I{sysconfig.get_paths()['include']}", f"-I{INCLUDE}", str(src), "-o", str(out), f"-L{root / 'lib'}", "-lc10", "-ltorch_cpu",
+           "-ltorch_python"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"{src.name}: {r.stdout}\n{r.stderr}")
+
+
 def build(verbose: bool = True, jobs: int | None = None, extra: list[str] | None = None) -> Path:
     BUILD_DIR.mkdir(exist_ok=True)
     srcs = sorted(CSRC.glob("*.hip"))
     jobs = jobs or min(8, os.cpu_count() or 4)
     with cf.ThreadPoolExecutor(jobs) as ex:
+        bind = ex.submit(_build_bind)
         objs = list(ex.map(lambda s: _compile(s, extra or []), srcs))
+        bind.result()
     if _needs(OUT, objs):
         # hipBLASLt: slx_gemm_lt (csrc/blaslt.hip), the vendor library for the plain GEMMs it runs faster
         cmd = [HIPCC, "-shared", "-fPIC", f"--offload-arch={ARCH}", *map(str, objs), "-lhipblaslt", "-o", str(OUT)]
@@ -61,7 +81,7 @@ def build(verbose: bool = True, jobs: int | None = None, extra: list[str] | None
         if r.returncode != 0:
             raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
     if verbose:
-        print(f"[slx] built {OUT} ({len(srcs)} sources)")
+        print(f"[slx] built {OUT} ({len(srcs)} sources) and {HERE / '_paged.so'}")
     return OUT
 
 
