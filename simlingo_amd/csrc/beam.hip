@@ -17,7 +17,7 @@ typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 constexpr int kSelChunk = 4096;          // columns a workgroup at least: 16 a thread
 constexpr int kSelMaxChunks = 64;        // one lane each in the second launch
 constexpr int kSelMaxK = 64, kSelMaxW = 64;
-constexpr int kSelList = 256;            // candidates of a chunk, or of a row's lists, that are ranked at once
+constexpr int kSelList = 256;            // candidates of a chunk (64 a wave), or of a row's lists, that are ranked at once
 
 struct SelArgs {
   const void* x; long ldx;
@@ -53,6 +53,14 @@ __device__ __forceinline__ unsigned wave_umax(unsigned x) {
   const unsigned c = (unsigned)__builtin_amdgcn_readlane((int)x, 32), d = (unsigned)__builtin_amdgcn_readlane((int)x, 48);
   return max(max(a, b), max(c, d));
 }
+__device__ __forceinline__ float wave_fsum(float x) {
+  x += __uint_as_float(dpp_u<0xB1>(__float_as_uint(x)));
+  x += __uint_as_float(dpp_u<0x4E>(__float_as_uint(x)));
+  x += __uint_as_float(dpp_u<0x141>(__float_as_uint(x)));
+  x += __uint_as_float(dpp_u<0x140>(__float_as_uint(x)));
+  const auto rl = [&](int l) { return __uint_as_float((unsigned)__builtin_amdgcn_readlane(__float_as_int(x), l)); };
+  return (rl(0) + rl(16)) + (rl(32) + rl(48));
+}
 // the largest key over the wave (uniform): high words first, then the low words of the lanes that hold that high word
 __device__ __forceinline__ u64 wave_kmax(u64 k) {
   const unsigned hi = wave_umax((unsigned)(k >> 32));
@@ -64,9 +72,9 @@ __device__ __forceinline__ u64 wave_kmax(u64 k) {
 template <typename T, int E>
 __global__ __launch_bounds__(256) void beam_chunk_kernel(SelArgs a) {
   __shared__ float2 sml[4];
-  __shared__ float stv[4];
-  __shared__ int scount;
-  __shared__ u64 list[kSelList];
+  __shared__ unsigned smax[256];
+  __shared__ int scount[4];
+  __shared__ u64 list[kSelList];  // 64 a wave
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int c = blockIdx.x, row = blockIdx.y;
   constexpr int VEC = 16 / (int)sizeof(T), U = E / VEC, CHUNK = 256 * E;  // 16-B loads, VEC columns each
@@ -95,7 +103,6 @@ __global__ __launch_bounds__(256) void beam_chunk_kernel(SelArgs a) {
       n += in;
     }
   }
-  if (tid == 0) scount = 0;
   float m = v[0];  // NaN stays out of the maximum, and makes the row's sum NaN, so that the row offers nothing
 #pragma unroll
   for (int e = 1; e < E; ++e) m = fmaxf(m, v[e]);
@@ -105,46 +112,67 @@ __global__ __launch_bounds__(256) void beam_chunk_kernel(SelArgs a) {
   float l = 0.f;
 #pragma unroll
   for (int e = 0; e < E; ++e) l += __expf(v[e] - ms);
-  l = warp_sum(l);
+  l = wave_fsum(l);
 
-  // a threshold with at least K of the chunk's columns at or above it: among the lanes' own maxima, halved into from both
-  // ends until few more than K lanes are left (-inf: none, every column is a candidate)
-  float tv = -INFINITY;
-  if (__popcll(__ballot(n > 0)) >= a.K) {
-    unsigned lo = ~wave_umax(~(n ? om : 0u)), hi = wave_umax(n ? om : 0u);  // every lane with columns is >= lo
-    for (int it = 0; it < 12 && lo < hi; ++it) {
-      const unsigned mid = lo + (hi - lo) / 2 + 1;
-      const int above = __popcll(__ballot(n > 0 && om >= mid));
-      if (above >= a.K) lo = mid;
-      else hi = mid - 1;
-      if (above >= a.K && above <= a.K + 2) break;
-    }
-    if (lo > 0x007FFFFFu) tv = unord_f(lo);
-  }
-  if (lane == 0) {
-    sml[wave] = make_float2(mw, l);
-    stv[wave] = tv;
-  }
+  // a threshold with at least K of the chunk's columns at or above it: the K-th largest of the 256 threads' own maxima, halved
+  // into from both ends until few more than K are left (-inf: fewer threads than K, or -inf itself)
+  smax[tid] = n ? om : 0u;
+  if (lane == 0) sml[wave] = make_float2(mw, l);
   if (n < E) {  // columns behind V: above no threshold
 #pragma unroll
     for (int e = 0; e < E; ++e) v[e] = e < n ? v[e] : NAN;
   }
   __syncthreads();
-  tv = fmaxf(fmaxf(stv[0], stv[1]), fmaxf(stv[2], stv[3]));
+  float tv = -INFINITY;
+  {
+    unsigned x[4], mx = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x[i] = smax[64 * i + lane];
+      mx = max(mx, x[i]);
+    }
+    auto above = [&](unsigned t) {
+      int k = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) k += __popcll(__ballot(x[i] >= t));
+      return k;
+    };
+    unsigned lo = 0x007FFFFFu, hi = wave_umax(mx);  // -inf
+    if (above(lo + 1) >= a.K) {
+      ++lo;
+      const unsigned near = hi - min(hi - lo, 0x02000000u);  // most often within a factor of 16 of the largest
+      if (near > lo && above(near) >= a.K) lo = near;
+      for (int it = 0; it < 20 && lo < hi; ++it) {
+        const unsigned mid = lo + (hi - lo) / 2 + 1;
+        const int k = above(mid);
+        if (k >= a.K) lo = mid;
+        else hi = mid - 1;
+        if (k >= a.K && k <= a.K + 2) break;
+      }
+      tv = unord_f(lo);
+    }
+  }
+  int at = 0;  // this wave's candidates
 #pragma unroll
   for (int e = 0; e < E; ++e) {
     const bool h = v[e] >= tv;
-    if (__any(h)) {
-      if (h) {
-        const int at = atomicAdd(&scount, 1);
-        if (at < kSelList) list[at] = key_of(ord_f(v[e] + 0.f), col(e));  // -0 ties with 0
-      }
+    const u64 in = __ballot(h);
+    if (in) {
+      const int i = at + __popcll(in & ((1ull << lane) - 1));
+      if (h && i < 64) list[64 * wave + i] = key_of(ord_f(v[e] + 0.f), col(e));  // -0 ties with 0
+      at += __popcll(in);
     }
   }
+  if (lane == 0) scount[wave] = at;
   __syncthreads();
-  int cnt = scount;
-  if (cnt > kSelList) {  // many equal logits: each wave draws its K largest keys one by one
-    __syncthreads();
+  int cnt[4];
+  bool over = false;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    cnt[w] = scount[w];
+    over = over || cnt[w] > 64;
+  }
+  if (over) {  // many equal logits: each wave draws its K largest keys one by one
     u64 last = ~0ull;
     for (int i = 0; i < a.K; ++i) {
       u64 best = 0;
@@ -154,18 +182,22 @@ __global__ __launch_bounds__(256) void beam_chunk_kernel(SelArgs a) {
         if (v[e] == v[e] && k < last && k > best) best = k;
       }
       best = wave_kmax(best);
-      if (lane == 0) list[wave * a.K + i] = best;
+      if (lane == 0) list[64 * wave + i] = best;
       last = best;  // 0 once the wave has no more: nothing is below it
     }
-    cnt = 4 * a.K;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) cnt[w] = a.K;
     __syncthreads();
   }
   u64* out = a.keys + ((long)row * a.C + c) * a.K;
-  if (tid < cnt) {  // every key is its own: the rank is the number of greater ones
+  const int mine = wave == 0 ? cnt[0] : wave == 1 ? cnt[1] : wave == 2 ? cnt[2] : cnt[3];
+  if (lane < mine) {  // every key is its own: the rank is the number of greater ones
     const u64 k = list[tid];
     int rank = 0;
-#pragma unroll 8
-    for (int i = 0; i < cnt; ++i) rank += list[i] > k;
+#pragma unroll
+    for (int w = 0; w < 4; ++w)
+#pragma unroll 4
+      for (int i = 0; i < cnt[w]; ++i) rank += list[64 * w + i] > k;
     if (k && rank < a.K) out[rank] = k;
   }
   // fewer columns than K (the last chunk): the rest of the list is empty
