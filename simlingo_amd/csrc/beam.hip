@@ -19,6 +19,8 @@ constexpr int kSelMaxChunks = 64;        // one lane each in the second launch
 constexpr int kSelMaxK = 64, kSelMaxW = 64;
 constexpr int kSelList = 256;            // candidates of a chunk (64 a wave), or of a row's lists, that are ranked at once
 
+constexpr int kSelFew = 512;             // entries of the rows' lists that are ranked at once
+
 struct SelArgs {
   const void* x; long ldx;
   const float* score; const unsigned char* fin;
@@ -68,6 +70,28 @@ __device__ __forceinline__ u64 wave_kmax(u64 k) {
   return ((u64)hi << 32) | lo;
 }
 
+// A value with at least K of the wave's N x 64 values at or above it, given that lo has: halved into between lo and the largest
+// until few more than K are left (all of 20 halvings leave a range of 2^12 of a float's bits; more than K is only more work).
+template <int N>
+__device__ __forceinline__ unsigned kth_below(const unsigned (&x)[N], unsigned lo, unsigned hi, int K) {
+  auto above = [&](unsigned t) {
+    int k = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) k += __popcll(__ballot(x[i] >= t));
+    return k;
+  };
+  const unsigned near = hi - min(hi - lo, 0x02000000u);  // most often within a factor of 16 of the largest
+  if (near > lo && above(near) >= K) lo = near;
+  for (int it = 0; it < 20 && lo < hi; ++it) {
+    const unsigned mid = lo + (hi - lo) / 2 + 1;
+    const int k = above(mid);
+    if (k >= K) lo = mid;
+    else hi = mid - 1;
+    if (k >= K && k <= K + 2) break;
+  }
+  return lo;
+}
+
 // E columns a thread: 16, or 32 where the rows make workgroups enough (the threshold and the ranking are per workgroup).
 template <typename T, int E>
 __global__ __launch_bounds__(256) void beam_chunk_kernel(SelArgs a) {
@@ -80,15 +104,17 @@ __global__ __launch_bounds__(256) void beam_chunk_kernel(SelArgs a) {
   constexpr int VEC = 16 / (int)sizeof(T), U = E / VEC, CHUNK = 256 * E;  // 16-B loads, VEC columns each
   const T* xr = (const T*)a.x + (long)row * a.ldx;
   const int c0 = c * CHUNK;
-  // a thread's columns rise with e, so those below V come first in its order: n of them
-  auto col = [&](int e) { return c0 + ((e / VEC) * 256 + tid) * VEC + e % VEC; };
+  // the last chunk is read element by element and spread over all threads; a thread's columns rise with e, so those below V
+  // come first in its order: n of them
+  const bool full = c0 + CHUNK <= a.V;
+  auto col = [&](int e) { return c0 + (full ? ((e / VEC) * 256 + tid) * VEC + e % VEC : e * 256 + tid); };
   float v[E];
   int n = E;
   // rows that have ended, or are out of the search already, are not read
   const unsigned char ended = a.fin ? a.fin[row] : 0;  // both on their way before either is looked at
   const float s = a.score[row];
   if (ended || s == -INFINITY || s != s) return;
-  if (c0 + CHUNK <= a.V) {
+  if (full) {
     T t[U][VEC];
 #pragma unroll
     for (int u = 0; u < U; ++u) __builtin_memcpy(t[u], xr + c0 + (u * 256 + tid) * VEC, 16);  // rows of odd length: any alignment of T
@@ -131,26 +157,10 @@ __global__ __launch_bounds__(256) void beam_chunk_kernel(SelArgs a) {
       x[i] = smax[64 * i + lane];
       mx = max(mx, x[i]);
     }
-    auto above = [&](unsigned t) {
-      int k = 0;
+    int finite = 0;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) k += __popcll(__ballot(x[i] >= t));
-      return k;
-    };
-    unsigned lo = 0x007FFFFFu, hi = wave_umax(mx);  // -inf
-    if (above(lo + 1) >= a.K) {
-      ++lo;
-      const unsigned near = hi - min(hi - lo, 0x02000000u);  // most often within a factor of 16 of the largest
-      if (near > lo && above(near) >= a.K) lo = near;
-      for (int it = 0; it < 20 && lo < hi; ++it) {
-        const unsigned mid = lo + (hi - lo) / 2 + 1;
-        const int k = above(mid);
-        if (k >= a.K) lo = mid;
-        else hi = mid - 1;
-        if (k >= a.K && k <= a.K + 2) break;
-      }
-      tv = unord_f(lo);
-    }
+    for (int i = 0; i < 4; ++i) finite += __popcll(__ballot(x[i] > 0x007FFFFFu));  // above -inf
+    if (finite >= a.K) tv = unord_f(kth_below(x, 0x00800000u, wave_umax(mx), a.K));
   }
   int at = 0;  // this wave's candidates
 #pragma unroll
@@ -221,17 +231,17 @@ __device__ __forceinline__ u64 ord_d(double v) {
 }
 
 // One workgroup a batch entry, one wave a row: the row's sum, then its k best of the chunks' sorted lists (a lane holds
-// a list's head), then every candidate's rank over all rows' lists by binary search (they are sorted alike).
+// a list's head); at the end one wave merges the rows' lists.
 __global__ __launch_bounds__(1024) void beam_pick_kernel(SelArgs a) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   u64* sc = reinterpret_cast<u64*>(smem);             // [W][K] ordered bits of the scores, descending
-  u64* cand = sc + a.W * a.K + (a.W * a.K + 1) / 2;   // [waves][kSelList], and then
-  int* rk = reinterpret_cast<int*>(cand);             // [W][K] ranks over all rows
+  u64* cand = sc + a.W * a.K + (a.W * a.K + 1) / 2;   // [waves][kSelList]
   int* ti = reinterpret_cast<int*>(sc + a.W * a.K);   // [W][K] tokens; -1 = none
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, nw = blockDim.x >> 6;
   const int b = blockIdx.x, K = a.K;
   const u64 ninf = ord_d(-INFINITY);
   __shared__ unsigned char fin_s[kSelMaxW];
+  __shared__ int ci[kSelFew];
   auto put = [&](int w, int i, u64 k, double s, double M, double lt) {  // i-th best of row w
     double v = s + (((double)unord_f((unsigned)(k >> 32)) - M) - lt) + 0.0;
     if (v != v) v = -INFINITY;  // +inf score and a -inf logit
@@ -255,11 +265,10 @@ __global__ __launch_bounds__(1024) void beam_pick_kernel(SelArgs a) {
     if (live) {
       const float Mf = unord_f(wave_umax(lane < a.C ? ord_f(x.x) : 0u));
       M = (double)Mf;
-      // a chunk's weight in 32 bits, like the terms it sums; their sum and its log in 64
-      double t = lane < a.C && !(x.x == -INFINITY && x.y == 0.f) ? (double)(x.y * __expf(x.x - Mf)) : 0.0;
-      for (int k = 32; k > 0; k >>= 1) t += __shfl_xor(t, k, 64);
-      lt = log(t);
-      live = t > 0.0 && lt - lt == 0.0 && M - M == 0.0;  // a row of -inf, or with a NaN or +inf, offers nothing
+      // the chunks' weights and their sum in 32 bits, like the terms they sum; its log in 64
+      const float t = wave_fsum(lane < a.C && !(x.x == -INFINITY && x.y == 0.f) ? x.y * __expf(x.x - Mf) : 0.f);
+      lt = log((double)t);
+      live = t > 0.f && lt - lt == 0.0 && M - M == 0.0;  // a row of -inf, or with a NaN or +inf, offers nothing
     }
     if (live) {
       // The row's K best of the chunks' sorted lists, a list a lane. No more than K lists matter, those with the largest
@@ -267,34 +276,64 @@ __global__ __launch_bounds__(1024) void beam_pick_kernel(SelArgs a) {
       if (lane >= a.C) head = 0;
 #pragma unroll
       for (int i = 0; i < 3; ++i) nxt[i] = lane < a.C && i + 1 < K ? nxt[i] : 0;
-      const int lists = __popcll(__ballot(head != 0)), q = (K + lists - 1) / lists;
-      u64 bar;
-      if (q == 1) {
-        int rank = 0;
-#pragma unroll 4
-        for (int i = 0; i < a.C; ++i) rank += lane_u64(head, i) > head;
-        const u64 atk = __ballot(rank == K - 1 && head);  // (heads are all different, but for empty lists)
-        bar = lane_u64(head, (int)__ffsll((long long)atk) - 1);
-      } else {  // fewer lists than K: the least of their q-th keys has q keys of each list at or above it
-        const u64 k = lane >= a.C || !head ? ~0ull : q == 2 ? nxt[0] : q == 3 ? nxt[1] : q <= K ? lp[q - 1] : 0;
-        bar = ~wave_kmax(~k);
-        if (!bar) bar = 1;
-      }
       u64* cl = cand + wave * kSelList;
+      u64 k[4] = {head, nxt[0], nxt[1], nxt[2]};
       int cnt = 0;
-      for (int i = 0; i < K; ++i) {
-        const u64 k = i == 0 ? head : i == 1 ? nxt[0] : i == 2 ? nxt[1] : i == 3 ? nxt[2] : head >= bar && lane < a.C ? lp[i] : 0;
-        const u64 in = __ballot(k >= bar);
-        if (!in) break;
-        const int at = cnt + __popcll(in & ((1ull << lane) - 1));
-        if (k >= bar && at < kSelList) cl[at] = k;
-        cnt += __popcll(in);
+      if (a.C * K <= kSelList) {  // all of them
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          k[i] = lane + 64 * i < a.C * K ? (a.keys + row * a.C * K)[lane + 64 * i] : 0;
+          cnt += __popcll(__ballot(k[i] != 0));
+        }
+      } else {
+        const int lists = __popcll(__ballot(head != 0)), q = (K + lists - 1) / lists;
+        u64 bar;
+        if (q == 1) {
+          int rank = 0;
+          for (int i = 0; i < a.C; ++i) rank += lane_u64(head, i) > head;
+          const u64 atk = __ballot(rank == K - 1 && head);  // (heads are all different, but for empty lists)
+          bar = lane_u64(head, (int)__ffsll((long long)atk) - 1);
+        } else {  // fewer lists than K: the least of their q-th keys has q keys of each list at or above it
+          bar = ~wave_kmax(~(lane < a.C && head ? lp[q - 1] : ~0ull));
+          if (!bar) bar = 1;
+        }
+        for (int i = 0; i < K; i += 4) {  // along the lists that reach the bar, four keys at a time
+          u64 in = 0;
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            in = __ballot(k[u] >= bar);
+            const int at = cnt + __popcll(in & ((1ull << lane) - 1));
+            if (k[u] >= bar && at < kSelList) cl[at] = k[u];
+            cnt += __popcll(in);
+          }
+          if (!in) break;
+          const bool on = k[3] >= bar;
+#pragma unroll
+          for (int u = 0; u < 4; ++u) k[u] = on && i + 4 + u < K ? lp[i + 4 + u] : 0;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) k[i] = lane + 64 * i < min(cnt, kSelList) ? cl[lane + 64 * i] : 0;
       }
-      if (cnt <= kSelList) {
+      if (cnt <= kSelList) {  // closer to K, by the K-th largest value among them; then the rank of each
+        unsigned x[4], mx = 0, t = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          x[i] = (unsigned)(k[i] >> 32);
+          mx = max(mx, x[i]);
+        }
+        if (cnt > K + 16) t = kth_below(x, 0, wave_umax(mx), K);
+        cnt = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const bool in = k[i] && x[i] >= t;
+          const u64 m = __ballot(in);
+          if (in) cl[cnt + __popcll(m & ((1ull << lane) - 1))] = k[i];
+          cnt += __popcll(m);
+        }
         for (int j = lane; j < cnt; j += 64) {
           const u64 mine = cl[j];
           int r = 0;
-#pragma unroll 8
+#pragma unroll 4
           for (int i = 0; i < cnt; ++i) r += cl[i] > mine;
           if (r < K) put(w, r, mine, (double)s, M, lt);
         }
@@ -323,36 +362,62 @@ __global__ __launch_bounds__(1024) void beam_pick_kernel(SelArgs a) {
       }
     }
   }
-  __syncthreads();  // the candidates are done with: their place holds the ranks
-  for (int i = tid; i < a.W * K; i += blockDim.x) rk[i] = i % K;  // within its own list
   __syncthreads();
-  // how many of list u come before (v, w * V + t): a thread for each candidate and other list, counts added up
-  for (int p = tid; p < a.W * K * a.W; p += blockDim.x) {
-    const int i = p / a.W, u = p - i * a.W, w = i / K;
-    if (u == w || ti[i] < 0) continue;
-    const u64 v = sc[i];
-    int lo = 0, hi = K;
-    while (lo < hi) {
-      const int mid = (lo + hi) >> 1;
-      const u64 x = sc[u * K + mid];
-      const bool before = ti[u * K + mid] >= 0 && (x > v || (x == v && u < w));
-      if (before) lo = mid + 1;
-      else hi = mid;
+  if (wave != 0) return;
+  auto write = [&](int r, int i, u64 v) {  // the r-th best: entry i of the rows' lists
+    const long o = (long)b * K + r;
+    const u64 u = (v >> 63) ? (v & 0x7FFFFFFFFFFFFFFFull) : ~v;
+    const int w = i / K, t = ti[i];
+    a.score_out[o] = (float)__longlong_as_double((long long)u);
+    a.parent[o] = w;
+    a.token[o] = t;
+    if (a.fin_out) a.fin_out[o] = fin_s[w] || t == a.eos;
+  };
+  if (a.W * K <= kSelFew) {
+    // few entries: those from the K-th largest high word of the scores on, and the rank of each among them; equal scores in
+    // the order of the lists, which is that of w * V + t
+    u64 k[kSelFew / 64];
+    unsigned x[kSelFew / 64], mx = 0, t = 0;
+#pragma unroll
+    for (int i = 0; i < kSelFew / 64; ++i) {
+      const int j = lane + 64 * i;
+      k[i] = j < a.W * K && ti[j] >= 0 ? sc[j] : 0;  // 0: none (-inf has bits)
+      x[i] = (unsigned)(k[i] >> 32);
+      mx = max(mx, x[i]);
     }
-    if (lo) atomicAdd(&rk[i], lo);
+    if (a.W * K > K + 16) t = kth_below(x, 0, wave_umax(mx), K);
+    int cnt = 0;
+#pragma unroll
+    for (int i = 0; i < kSelFew / 64; ++i) {
+      const bool in = k[i] && x[i] >= t;
+      const u64 m = __ballot(in);
+      const int to = cnt + __popcll(m & ((1ull << lane) - 1));
+      if (in) { cand[to] = k[i]; ci[to] = lane + 64 * i; }
+      cnt += __popcll(m);
+    }
+    for (int j = lane; j < cnt; j += 64) {
+      const u64 v = cand[j];
+      int r = 0;
+#pragma unroll 4
+      for (int i = 0; i < cnt; ++i) r += cand[i] > v || (cand[i] == v && i < j);
+      if (r < K) write(r, ci[j], v);
+    }
+    return;
   }
-  __syncthreads();
-  for (int i = tid; i < a.W * K; i += blockDim.x) {
-    const int w = i / K, t = ti[i], rank = rk[i];
-    if (t < 0) continue;
-    const u64 v = sc[i];
-    if (rank < K) {
-      const long o = (long)b * K + rank;
-      const u64 u = (v >> 63) ? (v & 0x7FFFFFFFFFFFFFFFull) : ~v;
-      a.score_out[o] = (float)__longlong_as_double((long long)u);
-      a.parent[o] = w;
-      a.token[o] = t;
-      if (a.fin_out) a.fin_out[o] = fin_s[w] || t == a.eos;
+  // The k best of the rows' sorted lists, a list a lane: k rounds of the wave's largest head (its low word among the lanes
+  // with the largest high word), ties to the lowest row. A list's next entry is read ahead.
+  const int base = min(lane, a.W - 1) * K, end = lane < a.W ? K : 0;
+  u64 cur = end && ti[base] >= 0 ? sc[base] : 0;  // 0: none (-inf has bits)
+  int at = 0;
+  for (int r = 0; r < K; ++r) {
+    const int i = base + min(at + 1, K - 1);
+    const u64 nxt = at + 1 < end && ti[i] >= 0 ? sc[i] : 0;
+    const u64 best = wave_kmax(cur);
+    if (!best) break;
+    if (lane == (int)__ffsll((long long)__ballot(cur == best)) - 1) {
+      write(r, base + at, cur);
+      cur = nxt;
+      ++at;
     }
   }
 }
@@ -461,7 +526,7 @@ int slx_beam_select(const slx_beam_select_desc* d, slx_stream_t s) {
   else hipLaunchKernelGGL((beam_chunk_kernel<float, 16>), grid, dim3(256), 0, (hipStream_t)s, a);
   SLX_LAUNCH_CHECK("slx_beam_select (chunks)");
   const int nw = a.W < 16 ? a.W : 16;
-  const int wk = a.W * a.K, lds = 8 * (wk + (wk + 1) / 2) + (wk * 4 > nw * kSelList * 8 ? wk * 4 : nw * kSelList * 8);
+  const int wk = a.W * a.K, lds = 8 * (wk + (wk + 1) / 2) + nw * kSelList * 8;
   if (lds > 60 * 1024) {
     hipError_t e = hipFuncSetAttribute((const void*)beam_pick_kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
     SLX_CHECK_ARG(e == hipSuccess, "slx_beam_select: %d B of LDS: %s", lds, hipGetErrorString(e));

@@ -25,7 +25,8 @@ def check(dev, logits, scores, width, k, finished=None, pad=0, exact_order=False
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("b,w,k,v", [(1, 1, 1, 1), (1, 1, 5, 5), (1, 4, 4, 151655), (2, 3, 6, 256), (3, 8, 16, 4097), (1, 16, 32, 8191), (2, 5, 64, 300),
                                      (1, 64, 64, 4096), (1, 2, 3, 262144), (5, 1, 2, 12289), (2, 64, 7, 65),
-                                     (4, 16, 32, 66001), (8, 8, 64, 151655), (64, 8, 3, 5001)])
+                                     (4, 16, 32, 66001), (8, 8, 64, 151655), (64, 8, 3, 5001),
+                                     (3, 12, 25, 256), (1, 16, 32, 20011), (2, 16, 64, 70000), (1, 8, 40, 28675)])
 def test_beam_select(dev, b, w, k, v, dtype):
     g = gen(b + w + k + v)
     logits = (torch.randn(b * w, v, generator=g) * 3).to(dtype)
