@@ -18,9 +18,9 @@ for src in "$ROOT"/simlingo_amd/csrc/*.hip; do
   o="$OUT/$(basename "${src%.hip}").o"
   objs+=("$o")
   if [ ! -f "$o" ] || [ "$src" -nt "$o" ]; then
-    # attention.hip issues its LDS DMA by inline asm with SGPR ("s") operands, which device -O0 cannot allocate
+    # attention.hip and paged.hip issue their LDS DMA by inline asm with SGPR ("s") operands, which device -O0 cannot allocate
     extra=()
-    [ "$(basename "$src")" = "attention.hip" ] && extra=(-Xarch_device -O1)
+    case "$(basename "$src")" in attention.hip | paged.hip) extra=(-Xarch_device -O1) ;; esac
     "$CLANG" "${FL[@]}" "${extra[@]}" -c "$src" -o "$o" &
     pids+=($!)
   fi
