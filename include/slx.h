@@ -557,12 +557,12 @@ int64_t slx_prefix_attn_ws_floats(const slx_prefix_attn_desc* d); /* < 0: bad ar
 /* ---- beam search (csrc/beam.hip) ----------------------------------------------------------------------------------
  * Beside the greedy choice of llm.py:145-160. score(b, w, t) = score[b][w] + x[b, w, t] - log sum_t' e^x[b, w, t'];
  * the k best of a batch entry's width * vocab scores in descending order, ties to the lowest w * vocab + t. A row that
- * has finished offers one continuation, `pad`, with its score unchanged. A score that is not a number (a row of -inf, a
- * row with a NaN or +inf logit) counts as -inf. score_out and finished_out may be score and finished when k == width. */
+ * has finished offers one continuation, `pad`, with its score unchanged. A row whose score is not finite, whose logits are
+ * all -inf or that has a NaN or +inf logit is out: its scores count as -inf. score_out and finished_out may be score and finished when k == width. */
 typedef struct slx_beam_select_desc {
   const void* logits; int64_t ldx; int logits_bf16;  /* [batch * width][vocab] f32 or bf16, any alignment of the type  */
   int batch, width, vocab, k;                /* width, k <= 64; vocab <= 262144                                        */
-  const float* score;                        /* [batch * width]; -inf: the beam is out                                 */
+  const float* score;                        /* [batch * width]; not finite: the beam is out                           */
   const unsigned char* finished; int pad;    /* optional [batch * width]                                               */
   float* score_out; int* parent; int* token; /* [batch][k]                                                             */
   unsigned char* finished_out; int eos;      /* optional [batch][k]: finished[parent] or token == eos                  */

@@ -100,7 +100,7 @@ __global__ __launch_bounds__(256) void beam_chunk_kernel(SelArgs a) {
   __shared__ int scount[4];
   __shared__ u64 list[kSelList];  // 64 a wave
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int c = blockIdx.x, row = blockIdx.y;
+  const int row = (int)(blockIdx.x / (unsigned)a.C), c = (int)(blockIdx.x - (unsigned)row * a.C);
   constexpr int VEC = 16 / (int)sizeof(T), U = E / VEC, CHUNK = 256 * E;  // 16-B loads, VEC columns each
   const T* xr = (const T*)a.x + (long)row * a.ldx;
   const int c0 = c * CHUNK;
@@ -113,7 +113,7 @@ __global__ __launch_bounds__(256) void beam_chunk_kernel(SelArgs a) {
   // rows that have ended, or are out of the search already, are not read
   const unsigned char ended = a.fin ? a.fin[row] : 0;  // both on their way before either is looked at
   const float s = a.score[row];
-  if (ended || s == -INFINITY || s != s) return;
+  if (ended || !(fabsf(s) < INFINITY)) return;
   if (full) {
     T t[U][VEC];
 #pragma unroll
@@ -244,7 +244,6 @@ __global__ __launch_bounds__(1024) void beam_pick_kernel(SelArgs a) {
   __shared__ int ci[kSelFew];
   auto put = [&](int w, int i, u64 k, double s, double M, double lt) {  // i-th best of row w
     double v = s + (((double)unord_f((unsigned)(k >> 32)) - M) - lt) + 0.0;
-    if (v != v) v = -INFINITY;  // +inf score and a -inf logit
     sc[w * K + i] = ord_d(v);
     ti[w * K + i] = k ? key_idx(k) : -1;
   };
@@ -261,7 +260,7 @@ __global__ __launch_bounds__(1024) void beam_pick_kernel(SelArgs a) {
     const bool fin = ended != 0;
     if (lane == 0) fin_s[w] = fin;
     double M = 0.0, lt = 0.0;  // the row's maximum, and the log of its sum of e^{x - M}: apart, since M may be huge
-    bool live = !fin && !(s == -INFINITY || s != s);
+    bool live = !fin && fabsf(s) < INFINITY;
     if (live) {
       const float Mf = unord_f(wave_umax(lane < a.C ? ord_f(x.x) : 0u));
       M = (double)Mf;
@@ -349,7 +348,7 @@ __global__ __launch_bounds__(1024) void beam_pick_kernel(SelArgs a) {
       }
     } else {
       // every score is -inf, but the one continuation of a row that has ended: the lowest tokens stand for the rest
-      const bool keep = fin && s == s && s != -INFINITY;
+      const bool keep = fin && fabsf(s) < INFINITY;
       for (int i = lane; i < K; i += 64) {
         int t = i;
         u64 v = ninf;
@@ -474,8 +473,8 @@ static void reorder_launch(const ReorderArgs& a, hipStream_t st) {
 
 static int check_select(const slx_beam_select_desc* d) {
   SLX_CHECK_ARG(d != nullptr, "slx_beam_select: null desc");
-  SLX_CHECK_ARG(d->batch >= 0 && d->batch <= 65535 / kSelMaxW && d->width > 0 && d->width <= kSelMaxW,
-                "slx_beam_select: 0 <= batch <= %d, 0 < width <= %d", 65535 / kSelMaxW, kSelMaxW);
+  SLX_CHECK_ARG(d->batch >= 0 && d->width > 0 && d->width <= kSelMaxW && (int64_t)d->batch * d->width * kSelMaxChunks < 2147483648L,
+                "slx_beam_select: 0 <= batch, 0 < width <= %d, batch * width < 2^25", kSelMaxW);
   SLX_CHECK_ARG(d->vocab > 0 && d->vocab <= kSelChunk * kSelMaxChunks, "slx_beam_select: 0 < vocab <= %d", kSelChunk * kSelMaxChunks);
   SLX_CHECK_ARG(d->k > 0 && d->k <= kSelMaxK && d->k <= (int64_t)d->width * d->vocab, "slx_beam_select: 0 < k <= %d and <= width * vocab", kSelMaxK);
   SLX_CHECK_ARG(d->ldx >= d->vocab, "slx_beam_select: ldx >= vocab");
@@ -518,7 +517,7 @@ int slx_beam_select(const slx_beam_select_desc* d, slx_stream_t s) {
   a.C = chunks_of(d);
   a.ml = (float2*)d->ws;
   a.keys = (u64*)((char*)d->ws + (int64_t)a.B * a.W * a.C * 8);
-  const dim3 grid(a.C, a.B * a.W);
+  const dim3 grid((unsigned)((int64_t)a.C * a.B * a.W));
   const bool wide = wide_chunks(d);
   if (d->logits_bf16 && wide) hipLaunchKernelGGL((beam_chunk_kernel<bf16, 32>), grid, dim3(256), 0, (hipStream_t)s, a);
   else if (d->logits_bf16) hipLaunchKernelGGL((beam_chunk_kernel<bf16, 16>), grid, dim3(256), 0, (hipStream_t)s, a);

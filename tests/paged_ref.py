@@ -100,6 +100,7 @@ def close_attn(got, want, spread):
 def select(logits, scores, width, k, finished=None, pad=0):
     """-> (scores f64, parent, token) by the definition: a stable sort of all width * V scores."""
     n, v = logits.shape
+    scores = torch.where(torch.isfinite(scores), scores, torch.full_like(scores, NEG))
     score = scores.double().view(n, 1) + torch.log_softmax(logits.double(), 1)
     if finished is not None:
         for i in range(n):

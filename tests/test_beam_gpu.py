@@ -100,6 +100,7 @@ def test_dead_and_finished_beams(dev):
     s = -torch.rand(12, generator=g) * 3
     s[1] = s[2] = s[3] = -INF        # the first step: one beam alive
     s[6] = NAN
+    s[5] = INF                       # as good as out
     fin = torch.zeros(12, dtype=torch.bool)
     fin[4] = fin[7] = True
     fin[8:] = True
@@ -112,6 +113,22 @@ def test_dead_and_finished_beams(dev):
     s[:] = -INF
     check(dev, x, s, 4, 6)
     check(dev, x[:, :2].contiguous(), torch.zeros(12), 4, 8, fin, 1)  # fewer continuations than asked for, -inf in order
+
+
+def test_many_batch_entries(dev):
+    g = gen(9)
+    x, s = torch.randn(70000, 40, generator=g), -torch.rand(70000, generator=g)
+    check(dev, x, s, 1, 2)
+
+
+def test_tensors_elsewhere(dev):
+    x, s = torch.randn(4, 40), torch.zeros(4)
+    with pytest.raises(RuntimeError, match="tensors on"):
+        PG.beam_select(x.to(dev), s, width=2)
+    with pytest.raises(RuntimeError, match="tensors on"):
+        PG.beam_reorder(x.to(dev), torch.zeros(2, 2, dtype=I32))
+    with pytest.raises(TypeError, match="must be a tensor"):
+        PG.beam_select(x.to(dev), 0.0, width=2)
 
 
 def test_in_place_and_finished_out(dev):
