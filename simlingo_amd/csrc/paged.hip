@@ -1021,20 +1021,21 @@ static int check_attn(const slx_prefix_attn_desc* d, int* capp, int* capo) {
 }
 
 template <int D>
-static void launch_attn(const PAttnPlan& p, dim3 grid, hipStream_t st, const PAttnArgs& a) {
+static bool launch_attn(const PAttnPlan& p, dim3 grid, hipStream_t st, const PAttnArgs& a) {
   if (p.whole) {
     if (p.ko == kS128) hipLaunchKernelGGL((prefix_attn_whole_kernel<D, 128>), grid, dim3(256), 0, st, a);
     else hipLaunchKernelGGL((prefix_attn_whole_kernel<D, 64>), grid, dim3(256), 0, st, a);
-    return;
+    return true;
   }
 #define SLX_PA(P, O)                                                                                         \
   if (p.kp == P && p.ko == O) {                                                                              \
     hipLaunchKernelGGL((prefix_attn_kernel<D, P, O>), grid, dim3(256), 0, st, a);                            \
-    return;                                                                                                  \
+    return true;                                                                                             \
   }
   SLX_PA(kD16, kD16) SLX_PA(kD32, kD16) SLX_PA(kD32, kD32) SLX_PA(kS64, kD16) SLX_PA(kS64, kD32) SLX_PA(kS64, kS64)
   SLX_PA(kS128, kD16) SLX_PA(kS128, kD32) SLX_PA(kS128, kS128)
 #undef SLX_PA
+  return false;
 }
 template <int D>
 static void launch_join(int parts, hipStream_t st, const PAttnArgs& a) {
@@ -1117,8 +1118,9 @@ int slx_prefix_attn(const slx_prefix_attn_desc* d, slx_stream_t s) {
   const long blocks = n_pre + (long)d->groups * d->width * Hkv * p.mto * p.nso;
   SLX_CHECK_ARG(blocks < 2147483648L, "slx_prefix_attn: too many rows");
   a.n_pre = (unsigned)n_pre;
-  if (D == 64) launch_attn<64>(p, dim3((unsigned)blocks), (hipStream_t)s, a);
-  else launch_attn<128>(p, dim3((unsigned)blocks), (hipStream_t)s, a);
+  const bool known = D == 64 ? launch_attn<64>(p, dim3((unsigned)blocks), (hipStream_t)s, a)
+                             : launch_attn<128>(p, dim3((unsigned)blocks), (hipStream_t)s, a);
+  SLX_CHECK_ARG(known, "slx_prefix_attn: no kernel for row tiles %d and %d", p.kp, p.ko);
   SLX_LAUNCH_CHECK("slx_prefix_attn");
   if (!a.direct) {
     if (D == 64) launch_join<64>(p.nsp + p.nso, (hipStream_t)s, a);

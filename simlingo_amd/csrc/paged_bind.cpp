@@ -77,9 +77,20 @@ Rows rows_of(const char* who, const char* name, const Tensor& t, int64_t n, int6
   NEED(t.scalar_type() == at::kBFloat16 && t.dim() == 2, "%s must be a bf16 matrix", name);
   NEED(t.size(0) == n && t.size(1) >= cols, "%s must have %lld rows of at least %lld, got %lld x %lld", name, (long long)n,
        (long long)cols, (long long)t.size(0), (long long)t.size(1));
-  const int64_t s0 = t.stride(0), s1 = t.stride(1);
+  const int64_t s0 = n > 1 ? t.stride(0) : t.size(1) / 8 * 8, s1 = t.stride(1);  // one row's stride says nothing
   NEED(s1 == 1 && s0 % 8 == 0 && ((uintptr_t)t.data_ptr() & 15) == 0, "rows of %s must be contiguous and 16-B aligned", name);
   return {t.data_ptr(), s0};
+}
+
+// Whether a call that reads x rows and writes y rows (n of them, wx and wy wide) may: apart, other columns of the same rows, or
+// y in x's place.
+bool may_write(const Rows& x, int64_t wx, const Rows& y, int64_t wy, int64_t n) {
+  const int64_t delta = ((const char*)y.p - (const char*)x.p) / 2;  // both 16-B aligned
+  if (n == 0 || delta >= (n - 1) * x.ld + wx || -delta >= (n - 1) * y.ld + wy) return true;
+  if (x.ld != y.ld && n > 1) return false;
+  if (delta == 0) return true;
+  if (n == 1) return false;
+  return delta > 0 ? delta >= wx && delta + wy <= x.ld : -delta >= wy && -delta + wx <= x.ld;
 }
 
 slx_kv_pool pool_of(const char* who, const Tensor& k, const Tensor& v, bool written) {
@@ -93,6 +104,7 @@ slx_kv_pool pool_of(const char* who, const Tensor& k, const Tensor& v, bool writ
        (long long)sh[0], (long long)sh[1], (long long)sh[2], (long long)sh[3]);
   NEED(st[3] == 1 && ((st[0] | st[1] | st[2]) & 7) == 0 && (((uintptr_t)k.data_ptr() | (uintptr_t)v.data_ptr()) & 15) == 0,
        "heads of k and v must be contiguous and 16-B aligned");
+  NEED(!written || k.data_ptr() != v.data_ptr(), "k and v are the same memory");
   NEED(!written || ((st[0] || sh[0] == 1) && (st[1] || sh[1] == 1) && (st[2] || sh[2] == 1)), "k and v must not be expanded");
   slx_kv_pool p;
   p.k = k.data_ptr();
@@ -183,6 +195,7 @@ PyObject* kv_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (seq) d.seq = ints_of(who, "seq", *seq, d.rows);
     if (q) {
       const Rows y = rows_of(who, "q_out", *q, d.rows, heads * hd);
+      NEED(may_write(x, (heads + 2 * hkv) * hd, y, heads * hd, d.rows), "q_out overlaps qkv other than in its own q columns");
       d.q_out = y.p; d.ldq = y.ld;
     }
     NEED(!cs == !sn, "cos and sin go together");
@@ -251,6 +264,7 @@ PyObject* prefix_attn(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (a[1] == Py_None) made = at::empty({rows, cols}, q.options());
     const Tensor& out = a[1] == Py_None ? made : tensor(a[1], who, "out");
     const Rows o = rows_of(who, "out", out, rows, cols);
+    NEED(may_write(x, cols, o, cols, rows), "out overlaps q other than in its place");
     d.out = o.p; d.ldo = o.ld;
     if (lse) {
       NEED(lse->scalar_type() == at::kFloat && lse->dim() == 2 && lse->size(0) == rows && lse->size(1) == heads && lse->is_contiguous(),

@@ -92,7 +92,8 @@ def kv_append(qkv, k, v, table, pos, q_out=None, *, n_heads, cos=None, sin=None,
     qkv's own q columns; without q_out q is not read.
 
     A row with pos < 0, or one that names no slot (behind the table or the rotation's rows, a sequence or page that there
-    is not), is padding: nothing of it is written. Two rows of one call must not name the same slot."""
+    is not), is padding: nothing of it is written. Two rows of one call must not name the same slot, and no other sequence may
+    hold the page of a row written."""
     (_native or _bind()).kv_append(qkv, k, v, table, pos, q_out, n_heads, cos, sin, seq, rows_per_seq)
 
 
@@ -113,8 +114,8 @@ def prefix_attn(q, out=None, *, own, prefix=None, n_heads, n_q=1, scale=None, ma
 def beam_select(logits, scores, *, width, k=None, finished=None, pad_id=0, eos_id=None, out=None, finished_out=None):
     """The k (default: width) best continuations of each batch entry by scores[b, w] + log_softmax(logits[b, w])[t], in
     descending order, ties to the lowest w * V + t. logits [batch * width, V] f32 or bf16, rows contiguous; scores
-    [batch * width] f32 (-inf: the beam is out). finished [batch * width] bool / uint8: such a row offers `pad_id` alone,
-    its score unchanged. A score that is not a number (rows of -inf, rows with a NaN or +inf) counts as -inf.
+    [batch * width] f32 (not finite: the beam is out). finished [batch * width] bool / uint8: such a row offers `pad_id` alone,
+    its score unchanged. The scores of a row that is out, is -inf throughout or holds a NaN or +inf count as -inf.
 
     Returns (scores f32, parent int32, token int32), each [batch, k] (out: the three to write to; the scores may be
     `scores` itself if k == width). finished_out [batch, k], with eos_id: finished[parent] or token == eos_id."""

@@ -106,6 +106,20 @@ def test_beam_reorder_refuses(x, parent, kw):
         PG.beam_reorder(x, parent, **kw)
 
 
+def test_writing_over_what_is_read():
+    """Outputs in the place of the queries, or in other columns of their rows, are taken; anything else that overlaps is not."""
+    buf = torch.zeros(6, 1024, dtype=BF16)
+    for q_out, ok in ((buf[:3, :256], True), (buf[:3, 512:768], True), (buf[3:, :256], True), (buf[:3, 64:320], False), (buf[1:4, :256], False), (buf[:3, 256:512], False)):
+        with pytest.raises(RuntimeError if ok else ValueError, match="no CPU" if ok else "overlaps qkv"):
+            PG.kv_append(**append_args(qkv=buf[:3, :512], q_out=q_out))
+    for out, ok in ((buf[:4, :256], True), (buf[:4, 256:512], True), (buf[1:5, :256], False), (buf[:4, 128:384], False)):
+        with pytest.raises(RuntimeError if ok else ValueError, match="no CPU" if ok else "overlaps q"):
+            PG.prefix_attn(**attn_args(q=buf[:4, :256], out=out))
+    k = pool()[0]
+    with pytest.raises(ValueError, match="same memory"):
+        PG.kv_append(**append_args(k=k, v=k))
+
+
 def test_beam_reorder_refuses_overlap():
     x = torch.zeros(6, 4)
     with pytest.raises(ValueError, match="overlaps"):
@@ -149,7 +163,7 @@ def test_c_entries_refuse():
     refused("slx_prefix_attn", d, b"workspace")
     refused("slx_prefix_attn", None, b"null")
     se = dict(logits=4096, ldx=9, batch=1, width=2, vocab=9, k=2, score=4096, score_out=4096, parent=4096, token=4096, ws=4096, ws_bytes=1 << 20)
-    for kw, text in ((dict(width=65), b"width"), (dict(batch=1 << 20), b"batch"), (dict(vocab=262145, ldx=262145), b"vocab"), (dict(k=65), b"k <="), (dict(k=19), b"k <="), (dict(ldx=8), b"ldx"),
+    for kw, text in ((dict(width=65), b"width"), (dict(batch=1 << 25), b"batch"), (dict(vocab=262145, ldx=262145), b"vocab"), (dict(k=65), b"k <="), (dict(k=19), b"k <="), (dict(ldx=8), b"ldx"),
                      (dict(finished=4096, pad=9), b"pad"), (dict(token=0), b"null"), (dict(ws=0), b"workspace"), (dict(ws_bytes=16), b"workspace"), (dict(ws=4100), b"workspace")):
         refused("slx_beam_select", PG.BeamSelectDesc(**{**se, **kw}), text)
     refused("slx_beam_select", None, b"null")

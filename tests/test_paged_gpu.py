@@ -313,6 +313,31 @@ def test_prefix_attn_strided_rows(dev):
     assert (buf[0] == 5).all() and (buf[7] == 5).all() and (buf[:, :64] == 5).all()
 
 
+def test_prefix_attn_in_the_queries_place(dev):
+    """out = q, in every form: split and joined, direct, whole rows; and out in other columns of q's rows."""
+    for hq, hkv, d, width, n_q, plens, olens in ((14, 2, 64, 5, 1, [300], [5] * 5), (14, 2, 64, 3, 1, None, [90, 1, 3]), (8, 2, 64, 26, 30, [70], [31] * 26),
+                                                 (32, 8, 128, 20, 1, [200], [7] * 20), (6, 2, 128, 2, 40, None, [40, 60])):
+        q, own, prefix = case(19, hq, hkv, d, 1, width, n_q, plens, 16, olens, 8)
+        want = PG.prefix_attn(q.to(dev), own=on(dev, own), prefix=on(dev, prefix), n_heads=hq, n_q=n_q)
+        buf = torch.zeros(q.shape[0], 2 * hq * d, dtype=BF16, device=dev)
+        x = buf[:, :hq * d]
+        x.copy_(q)
+        got = PG.prefix_attn(x, buf[:, hq * d:], own=on(dev, own), prefix=on(dev, prefix), n_heads=hq, n_q=n_q)
+        assert torch.equal(got, want) and torch.equal(x.cpu(), q)
+        assert torch.equal(PG.prefix_attn(x, x, own=on(dev, own), prefix=on(dev, prefix), n_heads=hq, n_q=n_q), want)
+
+
+def test_tensors_elsewhere(dev):
+    q, own, prefix = case(20, 2, 1, 64, 1, 1, 1, [9], 4, [3], 4)
+    for i in range(4):
+        mixed = tuple(x if j == i else to(x, dev) for j, x in enumerate(own))
+        with pytest.raises(RuntimeError, match="tensors on"):
+            PG.prefix_attn(q.to(dev), own=mixed, n_heads=2)
+    k, v = to(own[0], dev), to(own[1], dev)
+    with pytest.raises(RuntimeError, match="tensors on"):
+        PG.kv_append(torch.zeros(1, 256, dtype=BF16, device=dev), k, v, own[2], torch.zeros(1, dtype=I32, device=dev), n_heads=2)
+
+
 def test_prefix_attn_offsets_past_32_bits(dev):
     """Pages more than 2^31 elements apart."""
     heads, d, page = 1, 64, 16
