@@ -278,6 +278,13 @@ __device__ __forceinline__ void softmax_step(const f32x4 (&s)[T][NQ][2], float c
   }
 }
 
+// Rows whose every score is NaN have no maximum but a sum that is NaN: a state like any other from here on, not an empty one.
+template <int D, int NQ>
+__device__ __forceinline__ void keep_nan(State<D, NQ>& st) {
+#pragma unroll
+  for (int n = 0; n < NQ; ++n) st.m[n] = st.l[n][0] != st.l[n][0] && st.m[n] == -INFINITY ? 0.f : st.m[n];
+}
+
 // V of keys that are not there becomes 0 (0 * NaN would reach every row); with `sift`, so do values that are not finite
 // in keys that some row does not see yet -> whether there were any (they are added at the end: add_nonfinite)
 template <int D>
@@ -487,6 +494,7 @@ __device__ __forceinline__ void attn_direct(const PAttnArgs& a, Item w, char* sm
   float* sl = sm + 4 * 16 * NQ;                            // [4][16 NQ]
   f32x4* so = reinterpret_cast<f32x4*>(sl + 4 * 16 * NQ);  // [2][NQ * NE][64 lanes]
   float M[NQ], L[NQ];
+  keep_nan(st);
   if (grp == 0) {
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
@@ -726,6 +734,7 @@ __device__ __forceinline__ void store_stream(const PAttnArgs& a, const Item& w, 
   constexpr int NQ = Stream<D, RW>::NQ, NE = D / 16;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15;
   odd = __any(odd);
+  keep_nan(st);
   if constexpr (Stream<D, RW>::team) {
     f32x4* so = reinterpret_cast<f32x4*>(smem) + (wave & 1) * NQ * (NE + 1) * 64;  // [rows' wave][NQ][NE + 1][lane]
     __syncthreads();

@@ -276,6 +276,26 @@ def test_prefix_attn_masked_values_many_rows(dev):
         assert torch.equal(got[~bad], clean[~bad])
 
 
+def test_prefix_attn_nan_reaches_the_output(dev):
+    """A query that is NaN, and a sequence whose only key is: NaN in those rows and no others, in one part or split, few rows or many."""
+    nan = float("nan")
+    for hq, hkv, d, width, n_q, plens, olens in ((14, 2, 64, 2, 1, None, [1, 40]), (14, 2, 64, 2, 1, [300], [1, 140]), (14, 2, 64, 6, 1, [300], [5] * 6),
+                                                 (14, 2, 64, 20, 1, [300], [1] * 20), (32, 8, 128, 20, 1, [200], [7] * 20), (8, 2, 64, 26, 30, [70], [31] * 26),
+                                                 (8, 2, 128, 26, 30, [70], [31] * 26), (6, 2, 64, 2, 40, None, [40, 60])):
+        q, own, prefix = case(23, hq, hkv, d, 1, width, n_q, plens, 16, olens, 8)
+        q[-1, :d] = nan                                       # the last token's first head
+        if olens[0] == 1:
+            own[0][int(own[2][0, 0]), 0, hkv - 1] = nan       # sequence 0's only own key, last kv head
+        out, lse = run(dev, q, own, prefix, hq, n_q)
+        out = out.view(-1, hq, d)
+        want = torch.zeros(out.shape[0], hq, dtype=torch.bool)
+        want[-1, 0] = True
+        if olens[0] == 1:
+            want[0, hq - hq // hkv:] = True
+        assert torch.equal(torch.isnan(out).all(-1), want) and torch.equal(torch.isnan(out).any(-1), want)
+        assert torch.equal(torch.isnan(lse), want)
+
+
 def test_prefix_attn_bad_pages(dev):
     """Keys on page numbers outside the cache are masked, in both caches and at every page size."""
     for ppage, opage in ((16, 8), (64, 1), (2, 32)):
