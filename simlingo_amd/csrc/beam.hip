@@ -70,6 +70,9 @@ __device__ __forceinline__ u64 wave_kmax(u64 k) {
   return ((u64)hi << 32) | lo;
 }
 
+// what one lane of a wave has put into LDS is there for the others (its accesses are in order; the compiler keeps them so)
+__device__ __forceinline__ void wave_fence() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); }
+
 // A value with at least K of the wave's N x 64 values at or above it, given that lo has: halved into between lo and the largest
 // until few more than K are left (all of 20 halvings leave a range of 2^12 of a float's bits; more than K is only more work).
 template <int N>
@@ -310,6 +313,7 @@ __global__ __launch_bounds__(1024) void beam_pick_kernel(SelArgs a) {
 #pragma unroll
           for (int u = 0; u < 4; ++u) k[u] = on && i + 4 + u < K ? lp[i + 4 + u] : 0;
         }
+        wave_fence();
 #pragma unroll
         for (int i = 0; i < 4; ++i) k[i] = lane + 64 * i < min(cnt, kSelList) ? cl[lane + 64 * i] : 0;
       }
@@ -321,6 +325,7 @@ __global__ __launch_bounds__(1024) void beam_pick_kernel(SelArgs a) {
           mx = max(mx, x[i]);
         }
         if (cnt > K + 16) t = kth_below(x, 0, wave_umax(mx), K);
+        wave_fence();
         cnt = 0;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -329,6 +334,7 @@ __global__ __launch_bounds__(1024) void beam_pick_kernel(SelArgs a) {
           if (in) cl[cnt + __popcll(m & ((1ull << lane) - 1))] = k[i];
           cnt += __popcll(m);
         }
+        wave_fence();
         for (int j = lane; j < cnt; j += 64) {
           const u64 mine = cl[j];
           int r = 0;
@@ -394,6 +400,7 @@ __global__ __launch_bounds__(1024) void beam_pick_kernel(SelArgs a) {
       if (in) { cand[to] = k[i]; ci[to] = lane + 64 * i; }
       cnt += __popcll(m);
     }
+    wave_fence();
     for (int j = lane; j < cnt; j += 64) {
       const u64 v = cand[j];
       int r = 0;
