@@ -534,16 +534,16 @@ typedef struct slx_kv_append_desc {
                                                 position >= rope_rows counts as padding                               */
 } slx_kv_append_desc;
 /* rotate_half RoPE of q and k (f32, rounded once), k and v into their slots, in one pass. Two rows of one call must not
- * name the same slot.                                                                                                */
+ * name the same slot; the pool overlaps nothing else.                                                                */
 int slx_kv_append(const slx_kv_append_desc* d, slx_stream_t s);
 typedef struct slx_prefix_attn_desc {
   slx_kv_pool prefix_pool, own_pool;
   const void* q; int64_t ldq;                /* bf16 rows [groups * width * n_q][Hq * head_dim], a sequence's n_q tokens together */
-  void* out; int64_t ldo;                    /* bf16 [rows][Hq * head_dim]                                             */
+  void* out; int64_t ldo;                    /* bf16 [rows][Hq * head_dim]; may be q                                   */
   float* lse;                                /* optional f32 [rows][Hq]: natural log of the softmax sum (-inf: no key) */
   const int* ptab; int64_t ldpt; const int* plen;  /* [groups] prefixes; ptab NULL: none                               */
   const int* otab; int64_t ldot; const int* olen;  /* [groups * width] own keys, the n_q new tokens' last among them   */
-  int max_prefix, max_own;                   /* bounds of plen and olen (longer ones are cut to them)                  */
+  int max_prefix, max_own;                   /* bounds of plen and olen (longer ones are cut to them); <= 2^30         */
   int pcols, ocols;                          /* table columns                                                          */
   int groups, width, n_q, Hq;
   float scale;                               /* > 0                                                                    */
@@ -558,7 +558,8 @@ int64_t slx_prefix_attn_ws_floats(const slx_prefix_attn_desc* d); /* < 0: bad ar
  * Beside the greedy choice of llm.py:145-160. score(b, w, t) = score[b][w] + x[b, w, t] - log sum_t' e^x[b, w, t'];
  * the k best of a batch entry's width * vocab scores in descending order, ties to the lowest w * vocab + t. A row that
  * has finished offers one continuation, `pad`, with its score unchanged. A row whose score is not finite, whose logits are
- * all -inf or that has a NaN or +inf logit is out: its scores count as -inf. score_out and finished_out may be score and finished when k == width. */
+ * all -inf or that has a NaN or +inf logit is out: its scores count as -inf. score_out and finished_out may be score and
+ * finished when k == width; the outputs overlap nothing else.                                                          */
 typedef struct slx_beam_select_desc {
   const void* logits; int64_t ldx; int logits_bf16;  /* [batch * width][vocab] f32 or bf16, any alignment of the type  */
   int batch, width, vocab, k;                /* width, k <= 64; vocab <= 262144                                        */

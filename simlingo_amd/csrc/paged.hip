@@ -558,6 +558,8 @@ __device__ __forceinline__ void wait_tiles(int younger) {
   if (younger >= N) wait_vm<N * PER>();
   else if constexpr (N > 0) wait_tiles<N - 1, PER>(younger);
 }
+// a barrier after this wave's LDS accesses alone, with its DMA still under way; no access moves across it
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 // 16 B a lane from base + off (bytes) to LDS at lds + 16 * lane
 __device__ __forceinline__ void dma16(const void* base, unsigned off, unsigned lds) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base) : "memory");
@@ -642,8 +644,7 @@ __device__ __forceinline__ bool stream_keys(const PAttnArgs& a, const Item& w, i
   for (int t = 0; t < nt; ++t) {
     const int k0 = w.kb + STEP * t;
     wait_tiles<SLOTS - 2, PER>(nt - 1 - t);
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // this wave has read the slot that is filled next
-    __builtin_amdgcn_s_barrier();
+    lds_barrier();  // every wave has read the slot that is filled next
     if (t + SLOTS - 1 < nt) {
       issue(t + SLOTS - 1, en);
 #pragma unroll
@@ -874,8 +875,7 @@ __global__ __launch_bounds__(256, 2) void prefix_attn_whole_kernel(PAttnArgs a) 
   stream_keys<D, NQ, Stream<D, RW>::team>(a, w, rw, r0, qf, st, smem);
   item_segment(w, a.own, seq, true);
   item_range(a, w, RW);
-  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the ring is free when every wave has read the prefix's last tiles
-  __builtin_amdgcn_s_barrier();
+  lds_barrier();  // the ring is free when every wave has read the prefix's last tiles
   const bool odd = stream_keys<D, NQ, Stream<D, RW>::team>(a, w, rw, r0, qf, st, smem);
   store_stream<D, RW>(a, w, r0, odd, st, smem);
 }
@@ -1026,6 +1026,7 @@ static int check_attn(const slx_prefix_attn_desc* d, int* capp, int* capo) {
                   "slx_prefix_attn: a prefix needs plen, max_prefix >= 0, ldpt >= pcols > 0");
     *capp = cap_of(d->max_prefix, d->pcols, d->prefix_pool.page);
   }
+  SLX_CHECK_ARG(*capo <= 1 << 30 && *capp <= 1 << 30, "slx_prefix_attn: max_own and max_prefix (or the tables' columns) must be <= 2^30 keys");
   return 0;
 }
 

@@ -270,6 +270,10 @@ PyObject* prefix_attn(PyObject*, PyObject* const* a, Py_ssize_t n) {
       NEED(lse->scalar_type() == at::kFloat && lse->dim() == 2 && lse->size(0) == rows && lse->size(1) == heads && lse->is_contiguous(),
            "lse must be contiguous f32 [%lld, %lld]", (long long)rows, (long long)heads);
       d.lse = (float*)lse->data_ptr();
+      auto apart = [&](const Rows& r) {
+        return !rows || (char*)(d.lse + rows * heads) <= (char*)r.p || (char*)r.p + 2 * ((rows - 1) * r.ld + cols) <= (char*)d.lse;
+      };
+      NEED(apart(x) && apart(o), "lse overlaps q or out");
     }
     const slx_stream_t s = stream_of(who, {&q, &ok, &ov, &otab, &olen, &out, pk, pv, ptab, plen, lse});
     if (ot.n) {
@@ -341,7 +345,16 @@ PyObject* beam_select(PyObject*, PyObject* const* a, Py_ssize_t n) {
     d.batch = (int)b; d.width = (int)w; d.vocab = (int)vocab; d.k = (int)k;
     d.score = (const float*)scores.data_ptr();
     d.score_out = (float*)to[0]->data_ptr(); d.parent = (int*)to[1]->data_ptr(); d.token = (int*)to[2]->data_ptr();
-    NEED(k == w || !rows || (d.score_out != d.score && (!d.finished_out || d.finished_out != d.finished)), "scores or finished in place need k == width");
+    // batch entries run apart: what one writes, no other may read or write, but for scores and finished in place
+    const struct { const void* p; int64_t n; } put[4] = {{d.score_out, 4 * b * k}, {d.parent, 4 * b * k}, {d.token, 4 * b * k}, {d.finished_out, b * k}},
+                                               get[2] = {{d.score, 4 * rows}, {d.finished, rows}};
+    auto apart = [](const auto& u, const auto& t) {
+      return !u.p || !t.p || (const char*)u.p + u.n <= (const char*)t.p || (const char*)t.p + t.n <= (const char*)u.p;
+    };
+    for (int i = 0; i < 4; ++i) {
+      for (int j = 0; j < 2; ++j) NEED(apart(put[i], get[j]) || (k == w && i == 3 * j && put[i].p == get[j].p), "scores or finished in place need k == width, and all of it");
+      for (int j = 0; j < i; ++j) NEED(apart(put[i], put[j]), "outputs overlap");
+    }
     const slx_stream_t s = stream_of(who, {&x, &scores, to[0], to[1], to[2], fin, fout});
     if (b) {
       const int64_t need = lib.beam_select_ws_bytes(&d);

@@ -22,7 +22,6 @@ import torch
 from . import kernels as K
 
 
-
 class KVPoolDesc(ctypes.Structure):  # slx_kv_pool
     _fields_ = [("k", K.c_vp), ("v", K.c_vp), ("page_stride", K.c_i64), ("slot_stride", K.c_i64), ("head_stride", K.c_i64),
                 ("n_pages", K.c_int), ("page", K.c_int), ("heads", K.c_int), ("head_dim", K.c_int)]
@@ -92,8 +91,8 @@ def kv_append(qkv, k, v, table, pos, q_out=None, *, n_heads, cos=None, sin=None,
     qkv's own q columns; without q_out q is not read.
 
     A row with pos < 0, or one that names no slot (behind the table or the rotation's rows, a sequence or page that there
-    is not), is padding: nothing of it is written. Two rows of one call must not name the same slot, and no other sequence may
-    hold the page of a row written."""
+    is not), is padding: nothing of it is written. Two rows of one call must not name the same slot. k and v are apart from
+    each other and from qkv and q_out."""
     (_native or _bind()).kv_append(qkv, k, v, table, pos, q_out, n_heads, cos, sin, seq, rows_per_seq)
 
 
@@ -103,9 +102,9 @@ def prefix_attn(q, out=None, *, own, prefix=None, n_heads, n_q=1, scale=None, ma
     share, before their own. q rows [N * n_q, n_heads * head size], a sequence's tokens together, already rotated; the
     kv heads are the caches'. Token t sees the whole prefix and own keys up to length - n_q + t; a row without any key
     gives zeros. scale > 0: 1 / sqrt(head size) by default. max_own, max_prefix: bounds of the lengths where they are known
-    to be lower than the tables' columns (longer ones are cut to them); the split of the work goes by them.
+    to be lower than the tables' columns (longer ones are cut to them), at most 2^30; the split of the work goes by them.
     Keys on a page number outside the cache are masked. lse: optional f32 [N * n_q, n_heads], natural log of the softmax
-    sum (-inf without keys). Returns out (bf16, like q)."""
+    sum (-inf without keys). Returns out (bf16, like q); it may be q itself."""
     ok, ov, otab, olen = own
     pk, pv, ptab, plen = prefix if prefix is not None else (None, None, None, None)
     return (_native or _bind()).prefix_attn(q, out, ok, ov, otab, olen, pk, pv, ptab, plen, n_heads, n_q, scale, max_own, max_prefix, lse)
@@ -118,7 +117,7 @@ def beam_select(logits, scores, *, width, k=None, finished=None, pad_id=0, eos_i
     its score unchanged. The scores of a row that is out, is -inf throughout or holds a NaN or +inf count as -inf.
 
     Returns (scores f32, parent int32, token int32), each [batch, k] (out: the three to write to; the scores may be
-    `scores` itself if k == width). finished_out [batch, k], with eos_id: finished[parent] or token == eos_id."""
+    `scores` itself if k == width, and finished_out `finished`). finished_out [batch, k], with eos_id: finished[parent] or token == eos_id."""
     return (_native or _bind()).beam_select(logits, scores, width, k, finished, pad_id, eos_id, out, finished_out)
 
 

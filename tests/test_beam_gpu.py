@@ -230,3 +230,20 @@ def test_beam_graph(dev):
         rows = (out[1].cpu().long() + torch.tensor([[0], [4]])).view(-1)
         assert torch.equal(table.cpu(), before[rows])
         torch.randn(1000, device=dev).sum().item()
+
+
+def test_widest_in_a_graph(dev):
+    """64 rows, 64 chosen, which takes the most shared memory: captured, and replayed between eager calls."""
+    g = gen(11)
+    x, s = torch.randn(64, 5000, generator=g).to(dev), torch.zeros(64, device=dev)
+    out = (torch.empty(1, 64, device=dev), torch.empty(1, 64, dtype=I32, device=dev), torch.empty(1, 64, dtype=I32, device=dev))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        PG.beam_select(x, s, width=64, out=out)
+    for i in range(3):
+        x.copy_(torch.randn(64, 5000, generator=g))
+        s.copy_(-torch.rand(64, generator=g))
+        graph.replay()
+        R.check_select(out, R.select(x.cpu(), s.cpu(), 64, 64))
+        for a, b in zip(PG.beam_select(x, s, width=64), out):
+            assert torch.equal(a, b)

@@ -118,6 +118,20 @@ def test_writing_over_what_is_read():
     k = pool()[0]
     with pytest.raises(ValueError, match="same memory"):
         PG.kv_append(**append_args(k=k, v=k))
+    with pytest.raises(ValueError, match="lse overlaps"):
+        PG.prefix_attn(**attn_args(q=buf[:4, :256], lse=buf.view(-1)[512:].view(torch.float32)[:16].view(4, 4)))
+
+
+@pytest.mark.parametrize("at,k,ok", (((0, 100, 200, 300), 4, True), ((400, 100, 200, 500), 4, True), ((404, 100, 200, 300), 4, False), ((0, 100, 200, 502), 4, False),
+                                     ((400, 100, 200, 300), 2, False), ((0, 100, 200, 500), 2, False), ((0, 400, 200, 300), 4, False), ((0, 16, 200, 300), 4, False),
+                                     ((0, 32, 64, 96), 4, True), ((0, 32, 64, 92), 4, False)))
+def test_select_outputs_apart(at, k, ok):
+    """scores at byte 400 (8 of 4 B), finished at 500 (8 of 1 B); outputs of 2 x k at the bytes given."""
+    b = torch.zeros(512, dtype=torch.uint8)
+    v = lambda o, t: b[o:o + 2 * k * t.itemsize].view(t).view(2, k)
+    out, fout = (v(at[0], torch.float32), v(at[1], torch.int32), v(at[2], torch.int32)), v(at[3], torch.uint8)
+    with pytest.raises(RuntimeError if ok else ValueError, match="no CPU" if ok else "overlap|in place"):
+        PG.beam_select(torch.zeros(8, 9), b[400:432].view(torch.float32), width=4, k=k, finished=b[500:508], out=out, finished_out=fout)
 
 
 def test_beam_reorder_refuses_overlap():
@@ -159,6 +173,11 @@ def test_c_entries_refuse():
     d = PG.PrefixAttnDesc(**{**at, **pre})
     need = lib.slx_prefix_attn_ws_floats(ctypes.byref(d))
     assert need > 0 and need % (2 * 4 * 66) == 0
+    d.max_own, d.ocols = (1 << 30) + 1, 1 << 30
+    d.ldot = d.ocols
+    refused("slx_prefix_attn", d, b"2^30")
+    assert lib.slx_prefix_attn_ws_floats(ctypes.byref(d)) < 0
+    d.max_own, d.ocols, d.ldot = 16, 2, 2
     d.ws, d.ws_floats = 4096, need - 1
     refused("slx_prefix_attn", d, b"workspace")
     refused("slx_prefix_attn", None, b"null")
