@@ -880,16 +880,16 @@ __global__ __launch_bounds__(256, 2) void prefix_attn_whole_kernel(PAttnArgs a) 
   store_stream<D, RW>(a, w, r0, odd, st, smem);
 }
 
-// Joins the parts of a row: D / 4 threads, four d each, times PG groups that share the parts out, B at a time (8 parts at
-// once by one group; or 16 or 8 groups for rows with many parts, whose loads would otherwise be one chain).
+// Joins the parts of a row: D / 4 threads, four d each, times PG groups that share the parts out, B at a time: up to 8 parts at
+// once by one group, up to 16 by four, more by a whole workgroup, so that the loads of a row make few rounds.
 template <int D, int PG, int B>
 __global__ __launch_bounds__(256) void prefix_attn_join_kernel(PAttnArgs a) {
   constexpr int TPR = D / 4, RPB = 256 / (TPR * PG);
-  __shared__ float sml[PG > 1 ? PG : 1][2];
-  __shared__ __attribute__((aligned(16))) f32x4 so[PG > 1 ? PG : 1][TPR];
-  const int d4 = threadIdx.x % TPR, pg = threadIdx.x / TPR % PG, parts = a.pre.ns + a.own.ns;
-  const long row = (long)blockIdx.x * RPB + threadIdx.x / (TPR * PG);
-  if (row >= a.R) return;  // PG > 1: one row a workgroup
+  __shared__ float sml[RPB][PG][2];
+  __shared__ __attribute__((aligned(16))) f32x4 so[RPB][PG][TPR];
+  const int d4 = threadIdx.x % TPR, pg = threadIdx.x / TPR % PG, rl = threadIdx.x / (TPR * PG), parts = a.pre.ns + a.own.ns;
+  const bool off = (long)blockIdx.x * RPB + rl >= a.R;  // behind the last row: along with it up to the barrier
+  const long row = min((long)blockIdx.x * RPB + rl, a.R - 1);
   const float2* ml = reinterpret_cast<const float2*>(a.ws + parts * a.R * D) + row;
   const float* ob = a.ws + row * D + 4 * d4;
   float m = -INFINITY, l = 0.f;
@@ -925,8 +925,8 @@ __global__ __launch_bounds__(256) void prefix_attn_join_kernel(PAttnArgs a) {
     add(xm, xl, y);
   }
   if constexpr (PG > 1) {
-    so[pg][d4] = o;
-    if (d4 == 0) { sml[pg][0] = m; sml[pg][1] = l; }
+    so[rl][pg][d4] = o;
+    if (d4 == 0) { sml[rl][pg][0] = m; sml[rl][pg][1] = l; }
     __syncthreads();
     if (pg) return;
     m = -INFINITY;
@@ -937,10 +937,11 @@ __global__ __launch_bounds__(256) void prefix_attn_join_kernel(PAttnArgs a) {
       float xm[B], xl[B];
       f32x4 y[B];
 #pragma unroll
-      for (int u = 0; u < B; ++u) { xm[u] = sml[i0 + u][0]; xl[u] = sml[i0 + u][1]; y[u] = so[i0 + u][d4]; }
+      for (int u = 0; u < B; ++u) { xm[u] = sml[rl][i0 + u][0]; xl[u] = sml[rl][i0 + u][1]; y[u] = so[rl][i0 + u][d4]; }
       add(xm, xl, y);
     }
   }
+  if (off) return;
   const long tok = row / a.Hq;
   const float inv = l > 0.f || l != l ? 1.0f / l : 0.f;
   bf16x4 y;
@@ -952,8 +953,11 @@ __global__ __launch_bounds__(256) void prefix_attn_join_kernel(PAttnArgs a) {
 
 // Row tiles and key ranges of a call: a rule on sizes, page sizes and the host's bounds alone, so a captured call replays
 // for any lengths up to them. As many ranges as give about kTarget workgroups, each of at least 128 keys; or, where the
-// tiles of 64 rows of single sequences make kWhole workgroups by themselves, the whole rows at once.
-constexpr long kTarget = 768, kWhole = 192;
+// tiles of 64 rows of single sequences make kWhole workgroups by themselves and there are up to kWholeUnits x 128 keys, the
+// whole rows at once: a tile then runs through its keys alone (1.7 us for 128 of them), but writes no parts. Against parts and
+// join, 14 heads on 2 of 64: 12 sequences of 77 tokens, 640 shared keys: 16.5 us, 24 + 5; 1280: 25, 28 + 5; 8000: 113, 71 + 6.
+// 96 sequences of 4 tokens, 798 shared keys: 17, 18 + 5; 1800: 30, 21 + 5.
+constexpr long kTarget = 768, kWhole = 192, kWholeUnits = 12;
 struct PAttnPlan { int kp, ko, mtp, mto, nsp, nso, whole; };
 static PAttnPlan plan_attn(const slx_prefix_attn_desc* d, int capp, int capo) {
   PAttnPlan p;
@@ -961,14 +965,15 @@ static PAttnPlan plan_attn(const slx_prefix_attn_desc* d, int capp, int capo) {
   auto kind = [](long rows, const slx_kv_pool& pool) {
     // streamed tiles: one page number for 8 keys, whose offsets on the page fit 32 bits
     const bool streams = pool.page >= 8 && pool.slot_stride < (1 << 27);
-    return rows <= 16 ? kD16 : rows <= 32 || !streams ? kD32 : rows <= 64 ? kS64 : kS128;
+    return rows <= 16 ? kD16 : !streams ? kD32 : rows <= 64 ? kS64 : kS128;
   };
   const long rp = (long)d->width * d->n_q * gq, ro = (long)d->n_q * gq, heads = d->own_pool.heads;
   const long seqs = (long)d->groups * d->width * heads, t64 = (ro + 63) / 64, t128 = (ro + 127) / 128;
+  const long up = (capp + 127) / 128, uo = (capo + 127) / 128;  // units of 128 keys
   p.whole = 0;
   p.ko = kind(ro, d->own_pool);
   p.kp = capp > 0 ? kind(rp, d->prefix_pool) : p.ko;
-  if (capp > 0 && p.kp >= kS64 && p.ko >= kS64 && seqs * t64 >= kWhole) {
+  if (capp > 0 && p.kp >= kS64 && p.ko >= kS64 && seqs * t64 >= kWhole && up + uo <= kWholeUnits) {
     p.whole = 1;
     p.ko = p.kp = seqs * t128 >= 2 * kWhole ? kS128 : kS64;
     p.mto = p.mtp = (int)(p.ko == kS128 ? t128 : t64);
@@ -979,7 +984,6 @@ static PAttnPlan plan_attn(const slx_prefix_attn_desc* d, int capp, int capo) {
   if (p.kp == kS128 && p.ko == kS64) p.ko = kS128;     // of the same rows
   p.mtp = (int)((rp + kKindRows[p.kp] - 1) / kKindRows[p.kp]);
   p.mto = (int)((ro + kKindRows[p.ko] - 1) / kKindRows[p.ko]);
-  const long up = (capp + 127) / 128, uo = (capo + 127) / 128;  // units of 128 keys
   const long ip = d->groups * heads * p.mtp, io = seqs * p.mto;
   const long per = (ip * up + io * uo + kTarget - 1) / kTarget, u = per > 1 ? per : 1;
   p.nsp = (int)((up + u - 1) / u);
@@ -1047,15 +1051,16 @@ static bool launch_attn(const PAttnPlan& p, dim3 grid, hipStream_t st, const PAt
 #undef SLX_PA
   return false;
 }
+template <int D, int PG, int B>
+static void launch_join(hipStream_t st, const PAttnArgs& a) {
+  constexpr int RPB = 256 / (D / 4 * PG);
+  hipLaunchKernelGGL((prefix_attn_join_kernel<D, PG, B>), dim3((unsigned)((a.R + RPB - 1) / RPB)), dim3(256), 0, st, a);
+}
 template <int D>
-static void launch_join(int parts, hipStream_t st, const PAttnArgs& a) {
-  constexpr int PG = 1024 / D;  // one row a workgroup
-  if (parts > 8) {
-    hipLaunchKernelGGL((prefix_attn_join_kernel<D, PG, 4>), dim3((unsigned)a.R), dim3(256), 0, st, a);
-  } else {
-    constexpr int RPB = 1024 / D;
-    hipLaunchKernelGGL((prefix_attn_join_kernel<D, 1, 8>), dim3((unsigned)((a.R + RPB - 1) / RPB)), dim3(256), 0, st, a);
-  }
+static void join_parts(int parts, hipStream_t st, const PAttnArgs& a) {
+  if (parts <= 8) launch_join<D, 1, 8>(st, a);
+  else if (parts <= 16) launch_join<D, 4, 4>(st, a);
+  else launch_join<D, 1024 / D, 4>(st, a);
 }
 
 }  // namespace slx
@@ -1133,8 +1138,8 @@ int slx_prefix_attn(const slx_prefix_attn_desc* d, slx_stream_t s) {
   SLX_CHECK_ARG(known, "slx_prefix_attn: no kernel for row tiles %d and %d", p.kp, p.ko);
   SLX_LAUNCH_CHECK("slx_prefix_attn");
   if (!a.direct) {
-    if (D == 64) launch_join<64>(p.nsp + p.nso, (hipStream_t)s, a);
-    else launch_join<128>(p.nsp + p.nso, (hipStream_t)s, a);
+    if (D == 64) join_parts<64>(p.nsp + p.nso, (hipStream_t)s, a);
+    else join_parts<128>(p.nsp + p.nso, (hipStream_t)s, a);
     SLX_LAUNCH_CHECK("slx_prefix_attn (join)");
   }
   return 0;
