@@ -564,21 +564,27 @@ __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(
 __device__ __forceinline__ void dma16(const void* base, unsigned off, unsigned lds) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base) : "memory");
 }
-// tiles of 32 keys a step of the ring: two of 64-element heads, so that one wave has independent products to run
-constexpr int ring_tiles(int D) { return D == 64 ? 2 : 1; }
-constexpr int ring_slots(int D) { return D == 64 ? 3 : 4; }
-constexpr int ring_lds(int D) { return ring_slots(D) * (ring_tiles(D) * 2 * 32 * D * 2 + 4 * ring_tiles(D)); }
+// A streamed workgroup: NW waves over RW rows, 16 NQ rows a wave, and as many teams as that leaves, each of which takes tiles of
+// its own of every step of the ring, T tiles of 32 keys; the teams are joined at the end.
+template <int D, int RW, int NW>
+struct Shape {
+  static constexpr int RWV = D == 64 ? RW / 32 : 4, NQ = RW / 16 / RWV, TEAMS = NW / RWV;
+  static constexpr int T = TEAMS > 1 ? TEAMS : D == 64 ? 2 : 1, UW = T / TEAMS;  // tiles a step, and of them a team's
+  static constexpr int SLOTS = D == 128 && T == 1 ? 4 : 3;
+  static constexpr int LDS = SLOTS * (T * 2 * 32 * D * 2 + 4 * T);
+};
 
 // The keys of one segment into the state of a wave's rows r0 .. (the workgroup's from rw); whether values were sifted out.
 // The LDS is free when it is called, and its last tiles may still be read when it returns.
-template <int D, int NQ, bool TEAM>
-__device__ __forceinline__ bool stream_keys(const PAttnArgs& a, const Item& w, int rw, int r0, const bf16x8 (&qf)[NQ][D / 32],
-                                            State<D, NQ>& st, char* smem) {
-  constexpr int KK = D / 32, NE = D / 16, CH = D / 8, TILE = 32 * D * 2, T = ring_tiles(D), SLOTS = ring_slots(D), STEP = 32 * T;
-  constexpr int PER = T * 2 * D / 64;  // DMA pieces a wave and step
-  constexpr int RW = (TEAM ? 32 : 64) * NQ, UW = TEAM ? 1 : T;  // rows of the workgroup; tiles of a step that a wave takes
-  static_assert(!TEAM || T == 2, "one tile of a step for each team");
+template <int D, int RW, int NW>
+__device__ __forceinline__ bool stream_keys(const PAttnArgs& a, const Item& w, int rw, int r0,
+                                            const bf16x8 (&qf)[Shape<D, RW, NW>::NQ][D / 32], State<D, Shape<D, RW, NW>::NQ>& st, char* smem) {
+  typedef Shape<D, RW, NW> S;
+  constexpr int KK = D / 32, NE = D / 16, CH = D / 8, TILE = 32 * D * 2, T = S::T, SLOTS = S::SLOTS, STEP = 32 * T, NQ = S::NQ, UW = S::UW;
+  constexpr int TI = 4 * T / NW;       // tiles of a step that a wave brings 8 keys of
+  constexpr int PER = TI * 2 * D / 64;  // DMA pieces a wave and step
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, grp = lane >> 4;
+  const int wk = 8 * (wave & 3), wt = wave >> 2;  // its 8 keys of a tile, and which tile of each NW / 4
   const int rows = w.ntok * a.gq, shift = w.shift, mask = (1 << shift) - 1;
   unsigned char* badb = reinterpret_cast<unsigned char*>(smem + SLOTS * T * 2 * TILE);  // [SLOTS][T][4]: 8 keys a wave, 0 or 255
   const unsigned lds0 = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)LDS_PTR(char, smem));
@@ -593,41 +599,41 @@ __device__ __forceinline__ bool stream_keys(const PAttnArgs& a, const Item& w, i
   auto slot_of = [](int x) { return (x & ~5) | (x & 1) << 2 | (x >> 2 & 1); };
   auto swz = [](int slot) { return D == 64 ? slot >> 1 & 7 : slot & 15; };
   typedef const int __attribute__((address_space(4))) cint;
-  auto entry = [&](int t, int u) {  // the page of this wave's 8 keys of tile u of step t
-    const int key = min(w.kb + STEP * min(t, nt - 1) + 32 * u + 8 * wave, w.len - 1);
+  auto entry = [&](int t, int u) {  // the page of this wave's 8 keys of its tile u of step t
+    const int key = min(w.kb + STEP * min(t, nt - 1) + 32 * (u * (NW / 4) + wt) + wk, w.len - 1);
     return ((cint*)(uintptr_t)w.tab)[__builtin_amdgcn_readfirstlane(key >> shift)];
   };
   // A piece is 1 KiB: the wave's 8 keys lie on one page, so its address is a scalar and the lane's place among them.
-  unsigned off[PER / (2 * T)];
+  unsigned off[PER / (2 * TI)];
 #pragma unroll
-  for (int i = 0; i < PER / (2 * T); ++i) {
-    const int slot = 8 * wave + (64 / CH) * i + lane / CH;
+  for (int i = 0; i < PER / (2 * TI); ++i) {
+    const int slot = wk + (64 / CH) * i + lane / CH;
     off[i] = 2u * ((unsigned)(slot_of(slot) & 7) * (unsigned)w.ss + 8u * (unsigned)((lane % CH) ^ swz(slot)));
   }
-  auto issue = [&](int t, const int (&e)[T]) {
+  auto issue = [&](int t, const int (&e)[TI]) {
 #pragma unroll
-    for (int u = 0; u < T; ++u) {
-      const int at = (t % SLOTS) * T + u;
+    for (int u = 0; u < TI; ++u) {
+      const int tile = u * (NW / 4) + wt, at = (t % SLOTS) * T + tile;
       const bool ok = (unsigned)e[u] < (unsigned)w.n_pages;
-      const long from = (ok ? (long)e[u] * w.ps : 0L) + (long)((w.kb + STEP * t + 32 * u + 8 * wave) & mask) * w.ss;
-      if (lane == 0) badb[at * 4 + wave] = ok ? 0 : 255;
+      const long from = (ok ? (long)e[u] * w.ps : 0L) + (long)((w.kb + STEP * t + 32 * tile + wk) & mask) * w.ss;
+      if (lane == 0) badb[at * 4 + (wave & 3)] = ok ? 0 : 255;
 #pragma unroll
-      for (int i = 0; i < PER / (2 * T); ++i) {
-        const unsigned to = lds0 + at * 2 * TILE + (8 * wave + (64 / CH) * i) * D * 2;
+      for (int i = 0; i < PER / (2 * TI); ++i) {
+        const unsigned to = lds0 + at * 2 * TILE + (wk + (64 / CH) * i) * D * 2;
         dma16(w.k + from, off[i], to);
         dma16(w.v + from, off[i], to + TILE);
       }
     }
   };
-  int en[T];
+  int en[TI];
   if (nt > 0) {
-    int e[SLOTS - 1][T];
+    int e[SLOTS - 1][TI];
 #pragma unroll
     for (int i = 0; i < SLOTS - 1; ++i)
 #pragma unroll
-      for (int u = 0; u < T; ++u) e[i][u] = entry(i, u);
+      for (int u = 0; u < TI; ++u) e[i][u] = entry(i, u);
 #pragma unroll
-    for (int u = 0; u < T; ++u) en[u] = entry(SLOTS - 1, u);
+    for (int u = 0; u < TI; ++u) en[u] = entry(SLOTS - 1, u);
 #pragma unroll
     for (int i = 0; i < SLOTS - 1; ++i)
       if (i < nt) issue(i, e[i]);
@@ -648,9 +654,9 @@ __device__ __forceinline__ bool stream_keys(const PAttnArgs& a, const Item& w, i
     if (t + SLOTS - 1 < nt) {
       issue(t + SLOTS - 1, en);
 #pragma unroll
-      for (int u = 0; u < T; ++u) en[u] = entry(t + SLOTS, u);
+      for (int u = 0; u < TI; ++u) en[u] = entry(t + SLOTS, u);
     }
-    const int u0 = TEAM ? wave >> 1 : 0;
+    const int u0 = wave / S::RWV * UW;
     if (k0 + 32 * u0 >= kw) continue;
     f32x4 s[UW][NQ][2];
     bf16x8 pb[UW][NQ];
@@ -720,46 +726,44 @@ __device__ __forceinline__ void settle_rows(bf16x8 (&qf)[NQ][D / 32]) {
     for (int k = 0; k < D / 32; ++k) asm volatile("" : "+v"(qf[n][k]));
 }
 
-// What a streamed workgroup of 64 or 128 rows is: 16 rows a wave (128-element heads) or 32; and for 64 rows of 64-element
-// heads two teams of two waves, each with 32 rows a wave and one tile of every step (an operand read from LDS serves 32 rows
-// instead of 16), joined at the end.
-template <int D, int RW>
-struct Stream {
-  static constexpr bool team = D == 64 && RW == 64;
-  static constexpr int NQ = team ? 2 : RW / 64;
-};
-
-template <int D, int RW>
-__device__ __forceinline__ void store_stream(const PAttnArgs& a, const Item& w, int r0, bool odd, State<D, Stream<D, RW>::NQ>& st,
+template <int D, int RW, int NW>
+__device__ __forceinline__ void store_stream(const PAttnArgs& a, const Item& w, int r0, bool odd, State<D, Shape<D, RW, NW>::NQ>& st,
                                              char* smem) {
-  constexpr int NQ = Stream<D, RW>::NQ, NE = D / 16;
+  typedef Shape<D, RW, NW> S;
+  constexpr int NQ = S::NQ, NE = D / 16, HAND = NQ * (NE + 1) * 64;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15;
   odd = __any(odd);
   keep_nan(st);
-  if constexpr (Stream<D, RW>::team) {
-    f32x4* so = reinterpret_cast<f32x4*>(smem) + (wave & 1) * NQ * (NE + 1) * 64;  // [rows' wave][NQ][NE + 1][lane]
+  if constexpr (S::TEAMS > 1) {
+    static_assert((NW - S::RWV) * HAND * 16 <= S::LDS, "the teams' states take the ring's place");
+    f32x4* so = reinterpret_cast<f32x4*>(smem);  // [team 1 ..][rows' wave][NQ][NE + 1][lane]
     __syncthreads();
-    if (wave >= 2) {
+    if (wave >= S::RWV) {
+      f32x4* to = so + (wave - S::RWV) * HAND + lane;
 #pragma unroll
       for (int n = 0; n < NQ; ++n) {
 #pragma unroll
-        for (int e = 0; e < NE; ++e) so[(n * (NE + 1) + e) * 64 + lane] = st.o[n][e];
-        so[(n * (NE + 1) + NE) * 64 + lane] = f32x4{st.m[n], st.l[n][0], odd ? 1.f : 0.f, 0.f};
+        for (int e = 0; e < NE; ++e) to[(n * (NE + 1) + e) * 64] = st.o[n][e];
+        to[(n * (NE + 1) + NE) * 64] = f32x4{st.m[n], st.l[n][0], odd ? 1.f : 0.f, 0.f};
       }
     }
     __syncthreads();
-    if (wave >= 2) return;
+    if (wave >= S::RWV) return;
 #pragma unroll
-    for (int n = 0; n < NQ; ++n) {
-      const f32x4 x = so[(n * (NE + 1) + NE) * 64 + lane];
-      const float M = fmaxf(st.m[n], x[0]);
-      const float r0_ = st.m[n] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(st.m[n] - M);
-      const float r1_ = x[0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(x[0] - M);
-      st.l[n][0] = st.l[n][0] * r0_ + x[1] * r1_;
-      st.m[n] = M;
-      odd = odd || x[2] != 0.f;
+    for (int k = 0; k < S::TEAMS - 1; ++k) {
+      const f32x4* from = so + (k * S::RWV + wave) * HAND + lane;
 #pragma unroll
-      for (int e = 0; e < NE; ++e) st.o[n][e] = st.o[n][e] * r0_ + so[(n * (NE + 1) + e) * 64 + lane] * r1_;
+      for (int n = 0; n < NQ; ++n) {
+        const f32x4 x = from[(n * (NE + 1) + NE) * 64];
+        const float M = fmaxf(st.m[n], x[0]);
+        const float r0_ = st.m[n] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(st.m[n] - M);
+        const float r1_ = x[0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(x[0] - M);
+        st.l[n][0] = st.l[n][0] * r0_ + x[1] * r1_;
+        st.m[n] = M;
+        odd = odd || x[2] != 0.f;
+#pragma unroll
+        for (int e = 0; e < NE; ++e) st.o[n][e] = st.o[n][e] * r0_ + from[(n * (NE + 1) + e) * 64] * r1_;
+      }
     }
     odd = __any(odd);
   }
@@ -772,16 +776,16 @@ __device__ __forceinline__ void store_stream(const PAttnArgs& a, const Item& w, 
   }
 }
 
-template <int D, int RW>
+template <int D, int RW, int NW>
 __device__ __forceinline__ int wave_row(int rw) {  // a wave's first row
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  return rw + (Stream<D, RW>::team ? wave & 1 : wave) * 16 * Stream<D, RW>::NQ;
+  typedef Shape<D, RW, NW> S;
+  return rw + (__builtin_amdgcn_readfirstlane(threadIdx.x >> 6) % S::RWV) * 16 * S::NQ;
 }
 
-template <int D, int RW>
+template <int D, int RW, int NW>
 __device__ __forceinline__ void attn_stream(const PAttnArgs& a, Item w, char* smem) {
-  constexpr int NQ = Stream<D, RW>::NQ;
-  const int rw = w.mt * RW, r0 = wave_row<D, RW>(rw);
+  constexpr int NQ = Shape<D, RW, NW>::NQ;
+  const int rw = w.mt * RW, r0 = wave_row<D, RW, NW>(rw);
   bf16x8 qf[NQ][D / 32];
   load_rows<D, NQ>(a, w, r0, qf);
   asm volatile("" ::: "memory");  // the queries are requested before the length is waited for
@@ -789,8 +793,8 @@ __device__ __forceinline__ void attn_stream(const PAttnArgs& a, Item w, char* sm
   State<D, NQ> st;
   state_init(st);
   settle_rows<D, NQ>(qf);
-  const bool odd = stream_keys<D, NQ, Stream<D, RW>::team>(a, w, rw, r0, qf, st, smem);
-  store_stream<D, RW>(a, w, r0, odd, st, smem);
+  const bool odd = stream_keys<D, RW, NW>(a, w, rw, r0, qf, st, smem);
+  store_stream<D, RW, NW>(a, w, r0, odd, st, smem);
 }
 
 // kinds of a workgroup: direct with 16 or 32 rows, streamed with 64 or 128
@@ -800,16 +804,17 @@ template <int D, int KIND>
 __device__ __forceinline__ void attn_kind(const PAttnArgs& a, const Item& w, char* smem) {
   if constexpr (KIND == kD16) attn_direct<D, 1>(a, w, smem);
   else if constexpr (KIND == kD32) attn_direct<D, 2>(a, w, smem);
-  else if constexpr (KIND == kS64) attn_stream<D, 64>(a, w, smem);
-  else attn_stream<D, 128>(a, w, smem);
+  else if constexpr (KIND == kS64) attn_stream<D, 64, 4>(a, w, smem);
+  else attn_stream<D, 128, 4>(a, w, smem);
 }
-constexpr int kind_lds(int D, int kind) {
-  return kind >= kS64 ? ring_lds(D) : 2 * 4 * 16 * (kind + 1) * 4 + 2 * (kind + 1) * (D / 16) * 64 * 16;
+template <int D>
+constexpr int kind_lds(int kind) {
+  return kind == kS64 ? Shape<D, 64, 4>::LDS : kind == kS128 ? Shape<D, 128, 4>::LDS : 2 * 4 * 16 * (kind + 1) * 4 + 2 * (kind + 1) * (D / 16) * 64 * 16;
 }
 
 template <int D, int KP, int KO>
 __global__ __launch_bounds__(256, 2) void prefix_attn_kernel(PAttnArgs a) {
-  constexpr int LDS = kind_lds(D, KP) > kind_lds(D, KO) ? kind_lds(D, KP) : kind_lds(D, KO);
+  constexpr int LDS = kind_lds<D>(KP) > kind_lds<D>(KO) ? kind_lds<D>(KP) : kind_lds<D>(KO);
   __shared__ __attribute__((aligned(16))) char smem[LDS];
   unsigned b = blockIdx.x;
   const bool pre = b < a.n_pre;
@@ -850,9 +855,10 @@ __global__ __launch_bounds__(256, 2) void prefix_attn_kernel(PAttnArgs a) {
 
 // Many new tokens in many sequences: a workgroup takes 64 or 128 rows of ONE sequence through the prefix and then its own
 // keys, so there are no parts to write and join (the prefix is fetched again for every tile of rows, from L2).
-template <int D, int RW>
-__global__ __launch_bounds__(256, 2) void prefix_attn_whole_kernel(PAttnArgs a) {
-  __shared__ __attribute__((aligned(16))) char smem[ring_lds(D)];
+template <int D, int RW, int NW>
+__global__ __launch_bounds__(64 * NW, 2) void prefix_attn_whole_kernel(PAttnArgs a) {
+  constexpr int NQ = Shape<D, RW, NW>::NQ;
+  __shared__ __attribute__((aligned(16))) char smem[Shape<D, RW, NW>::LDS];
   unsigned b = blockIdx.x;  // [kv head][sequence][row tile]: neighbours share the prefix
   Item w;
   w.mt = (int)(b % (unsigned)a.mt_own);
@@ -862,8 +868,7 @@ __global__ __launch_bounds__(256, 2) void prefix_attn_whole_kernel(PAttnArgs a) 
   w.tok0 = (long)seq * a.Tq;
   w.ntok = a.Tq;
   w.range = w.part = 0;
-  constexpr int NQ = Stream<D, RW>::NQ;
-  const int rw = w.mt * RW, r0 = wave_row<D, RW>(rw);
+  const int rw = w.mt * RW, r0 = wave_row<D, RW, NW>(rw);
   bf16x8 qf[NQ][D / 32];
   load_rows<D, NQ>(a, w, r0, qf);
   asm volatile("" ::: "memory");  // the queries are requested before the lengths are waited for
@@ -872,12 +877,12 @@ __global__ __launch_bounds__(256, 2) void prefix_attn_whole_kernel(PAttnArgs a) 
   State<D, NQ> st;
   state_init(st);
   settle_rows<D, NQ>(qf);
-  stream_keys<D, NQ, Stream<D, RW>::team>(a, w, rw, r0, qf, st, smem);
+  stream_keys<D, RW, NW>(a, w, rw, r0, qf, st, smem);
   item_segment(w, a.own, seq, true);
   item_range(a, w, RW);
   lds_barrier();  // the ring is free when every wave has read the prefix's last tiles
-  const bool odd = stream_keys<D, NQ, Stream<D, RW>::team>(a, w, rw, r0, qf, st, smem);
-  store_stream<D, RW>(a, w, r0, odd, st, smem);
+  const bool odd = stream_keys<D, RW, NW>(a, w, rw, r0, qf, st, smem);
+  store_stream<D, RW, NW>(a, w, r0, odd, st, smem);
 }
 
 // Joins the parts of a row: D / 4 threads, four d each, times PG groups that share the parts out, B at a time: up to 8 parts at
@@ -957,8 +962,8 @@ __global__ __launch_bounds__(256) void prefix_attn_join_kernel(PAttnArgs a) {
 // whole rows at once: a tile then runs through its keys alone (1.7 us for 128 of them), but writes no parts. Against parts and
 // join, 14 heads on 2 of 64: 12 sequences of 77 tokens, 640 shared keys: 16.5 us, 24 + 5; 1280: 25, 28 + 5; 8000: 113, 71 + 6.
 // 96 sequences of 4 tokens, 798 shared keys: 17, 18 + 5; 1800: 30, 21 + 5.
-constexpr long kTarget = 768, kWhole = 192, kWholeUnits = 12;
-struct PAttnPlan { int kp, ko, mtp, mto, nsp, nso, whole; };
+constexpr long kTarget = 768, kWhole = 192, kWholeUnits = 12, kCUs = 256;
+struct PAttnPlan { int kp, ko, mtp, mto, nsp, nso, whole; };  // whole: waves of a workgroup, or 0
 static PAttnPlan plan_attn(const slx_prefix_attn_desc* d, int capp, int capo) {
   PAttnPlan p;
   const int gq = d->Hq / d->own_pool.heads;
@@ -974,8 +979,8 @@ static PAttnPlan plan_attn(const slx_prefix_attn_desc* d, int capp, int capo) {
   p.ko = kind(ro, d->own_pool);
   p.kp = capp > 0 ? kind(rp, d->prefix_pool) : p.ko;
   if (capp > 0 && p.kp >= kS64 && p.ko >= kS64 && seqs * t64 >= kWhole && up + uo <= kWholeUnits) {
-    p.whole = 1;
     p.ko = p.kp = seqs * t128 >= 2 * kWhole ? kS128 : kS64;
+    p.whole = p.ko == kS64 && seqs * t64 <= kCUs ? 8 : 4;  // one workgroup a CU: 8 waves (17.5 -> 14.9 us above); two of them: 4 (340: 23.4, 29.2)
     p.mto = p.mtp = (int)(p.ko == kS128 ? t128 : t64);
     p.nsp = p.nso = 1;
     return p;
@@ -1037,8 +1042,9 @@ static int check_attn(const slx_prefix_attn_desc* d, int* capp, int* capo) {
 template <int D>
 static bool launch_attn(const PAttnPlan& p, dim3 grid, hipStream_t st, const PAttnArgs& a) {
   if (p.whole) {
-    if (p.ko == kS128) hipLaunchKernelGGL((prefix_attn_whole_kernel<D, 128>), grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((prefix_attn_whole_kernel<D, 64>), grid, dim3(256), 0, st, a);
+    if (p.ko == kS128) hipLaunchKernelGGL((prefix_attn_whole_kernel<D, 128, 4>), grid, dim3(256), 0, st, a);
+    else if (p.whole == 8) hipLaunchKernelGGL((prefix_attn_whole_kernel<D, 64, 8>), grid, dim3(512), 0, st, a);
+    else hipLaunchKernelGGL((prefix_attn_whole_kernel<D, 64, 4>), grid, dim3(256), 0, st, a);
     return true;
   }
 #define SLX_PA(P, O)                                                                                         \

@@ -197,6 +197,23 @@ def test_prefix_attn(dev, c):
     check(dev, q, own, prefix, hq, n_q)
 
 
+@pytest.mark.parametrize("d", (64, 128))
+@pytest.mark.parametrize("n,n_q", ((6, 40), (9, 61), (12, 33), (3, 97)))
+def test_prefix_attn_whole_rows(dev, d, n, n_q):
+    """32 kv heads x n sequences of 64-row tiles, in one part: 8 waves or 4 a tile, and tiles of 128 rows; own keys that end in and
+    between tiles, a prefix that ends in one, a query of NaN and its neighbours, and the output in the queries' place."""
+    q, own, prefix = case(n, 32, 32, d, 1, n, n_q, [77], 16, [n_q + i * 23 % 70 for i in range(n)], 8)
+    q[5, d:2 * d] = 0.0
+    out = check(dev, q, own, prefix, 32, n_q)
+    x = q.clone()
+    x[5, d:2 * d] = float("nan")
+    x = x.to(dev)
+    got = PG.prefix_attn(x, x, own=on(dev, own), prefix=on(dev, prefix), n_heads=32, n_q=n_q).cpu()
+    assert torch.isnan(got[5, d:2 * d]).all()
+    got[5, d:2 * d] = out[5, d:2 * d]
+    assert torch.equal(got, out)
+
+
 def test_prefix_attn_many_ranges(dev):
     """Long keys, few rows: many ranges a row, and a second call with short lengths in the same tables."""
     q, own, prefix = case(3, 2, 1, 64, 1, 2, 1, [2100], 64, [1500, 40], 16)
