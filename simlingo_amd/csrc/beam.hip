@@ -14,11 +14,10 @@ namespace slx {
 
 typedef unsigned long long u64;
 typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
-constexpr int kSelChunk = 4096;          // columns a workgroup at least: 16 a thread
+constexpr int kSelChunk = 4096;          // columns a workgroup: 16 a thread
 constexpr int kSelMaxChunks = 64;        // one lane each in the second launch
 constexpr int kSelMaxK = 64, kSelMaxW = 64;
 constexpr int kSelList = 256;            // candidates of a chunk (64 a wave), or of a row's lists, that are ranked at once
-
 constexpr int kSelFew = 512;             // entries of the rows' lists that are ranked at once
 
 struct SelArgs {
@@ -95,8 +94,7 @@ __device__ __forceinline__ unsigned kth_below(const unsigned (&x)[N], unsigned l
   return lo;
 }
 
-// E columns a thread: 16, or 32 where the rows make workgroups enough (the threshold and the ranking are per workgroup).
-template <typename T, int E>
+template <typename T>
 __global__ __launch_bounds__(256) void beam_chunk_kernel(SelArgs a) {
   __shared__ float2 sml[4];
   __shared__ unsigned smax[256];
@@ -104,7 +102,7 @@ __global__ __launch_bounds__(256) void beam_chunk_kernel(SelArgs a) {
   __shared__ u64 list[kSelList];  // 64 a wave
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int row = (int)(blockIdx.x / (unsigned)a.C), c = (int)(blockIdx.x - (unsigned)row * a.C);
-  constexpr int VEC = 16 / (int)sizeof(T), U = E / VEC, CHUNK = 256 * E;  // 16-B loads, VEC columns each
+  constexpr int E = kSelChunk / 256, VEC = 16 / (int)sizeof(T), U = E / VEC, CHUNK = kSelChunk;  // 16-B loads, VEC columns each
   const T* xr = (const T*)a.x + (long)row * a.ldx;
   const int c0 = c * CHUNK;
   // the last chunk is read element by element and spread over all threads; a thread's columns rise with e, so those below V
@@ -489,14 +487,7 @@ static int check_select(const slx_beam_select_desc* d) {
   return 0;
 }
 
-// 8192 columns a workgroup instead of 4096 where that still leaves 512 workgroups
-static bool wide_chunks(const slx_beam_select_desc* d) {
-  return (int64_t)d->batch * d->width * ((d->vocab + 2 * kSelChunk - 1) / (2 * kSelChunk)) >= 512;
-}
-static int chunks_of(const slx_beam_select_desc* d) {
-  const int c = wide_chunks(d) ? 2 * kSelChunk : kSelChunk;
-  return (d->vocab + c - 1) / c;
-}
+static int chunks_of(const slx_beam_select_desc* d) { return (d->vocab + kSelChunk - 1) / kSelChunk; }
 
 }  // namespace slx
 
@@ -525,11 +516,8 @@ int slx_beam_select(const slx_beam_select_desc* d, slx_stream_t s) {
   a.ml = (float2*)d->ws;
   a.keys = (u64*)((char*)d->ws + (int64_t)a.B * a.W * a.C * 8);
   const dim3 grid((unsigned)((int64_t)a.C * a.B * a.W));
-  const bool wide = wide_chunks(d);
-  if (d->logits_bf16 && wide) hipLaunchKernelGGL((beam_chunk_kernel<bf16, 32>), grid, dim3(256), 0, (hipStream_t)s, a);
-  else if (d->logits_bf16) hipLaunchKernelGGL((beam_chunk_kernel<bf16, 16>), grid, dim3(256), 0, (hipStream_t)s, a);
-  else if (wide) hipLaunchKernelGGL((beam_chunk_kernel<float, 32>), grid, dim3(256), 0, (hipStream_t)s, a);
-  else hipLaunchKernelGGL((beam_chunk_kernel<float, 16>), grid, dim3(256), 0, (hipStream_t)s, a);
+  if (d->logits_bf16) hipLaunchKernelGGL((beam_chunk_kernel<bf16>), grid, dim3(256), 0, (hipStream_t)s, a);
+  else hipLaunchKernelGGL((beam_chunk_kernel<float>), grid, dim3(256), 0, (hipStream_t)s, a);
   SLX_LAUNCH_CHECK("slx_beam_select (chunks)");
   const int nw = a.W < 16 ? a.W : 16;
   const int wk = a.W * a.K, lds = 8 * (wk + (wk + 1) / 2) + nw * kSelList * 8;

@@ -957,13 +957,20 @@ __global__ __launch_bounds__(256) void prefix_attn_join_kernel(PAttnArgs a) {
 }
 
 // Row tiles and key ranges of a call: a rule on sizes, page sizes and the host's bounds alone, so a captured call replays
-// for any lengths up to them. As many ranges as give about kTarget workgroups, each of at least 128 keys; or, where the
-// tiles of 64 rows of single sequences make kWhole workgroups by themselves and there are up to kWholeUnits x 128 keys, the
-// whole rows at once: a tile then runs through its keys alone (1.7 us for 128 of them), but writes no parts. Against parts and
-// join, 14 heads on 2 of 64: 12 sequences of 77 tokens, 640 shared keys: 16.5 us, 24 + 5; 1280: 25, 28 + 5; 8000: 113, 71 + 6.
-// 96 sequences of 4 tokens, 798 shared keys: 17, 18 + 5; 1800: 30, 21 + 5.
-constexpr long kTarget = 768, kWhole = 192, kWholeUnits = 12, kCUs = 256;
+// for any lengths up to them. As many ranges as give about kTarget workgroups, each of at least 128 keys; or whole rows.
+//
+// Whole rows, a tile of 64 rows of one sequence through the prefix and its own keys, write no parts and need no join, but fetch the
+// prefix for every tile and run alone (1.3 us for 128 keys of 64 elements on an 8-wave workgroup, 2.6 us of 128). Measured against
+// parts + join (us; 14 heads on 2 of 64 unless said):
+//   12 sequences of 77 tokens:   640 shared keys 14.4, 26.7 + 5.3;  1800: 33 (4 waves), 32 + 5;  8000: 113 (4 waves), 71 + 6
+//   10 of 60 (140 tiles), 1280:  20.4, 25 + 6       4 of 40 (40 tiles), 640: 13.9, 13.0 + 3.9       1 of 3 (2 tiles), 200: 10.2, 6.9 + 2.3
+//   32 heads on 8 of 128:        8 of 64 (256 tiles), 1280: 33, 41 + 10   4 of 40 (96), 640: 20, 19.5 + 5   4 of 40, 1280: 36, 22 + 7
+// Ranges: 512 / 768 / 1024 / 1536 workgroups for 2 x 16 sequences on 32771 keys 22.6 / 21.5 / 19.9 / 19.6 with joins that grow, for 32
+// on 16411 keys of 8 heads of 128 63 / 53 / 55 / 63.
+constexpr long kTarget = 768, kCUs = 256;
 struct PAttnPlan { int kp, ko, mtp, mto, nsp, nso, whole; };  // whole: waves of a workgroup, or 0
+// the most units of 128 keys that tiles of whole rows run through
+static long whole_units(int D, long tiles) { return tiles >= (D == 64 ? 64 : 192) ? 12 : tiles >= (D == 64 ? 16 : 64) ? 7 : 0; }
 static PAttnPlan plan_attn(const slx_prefix_attn_desc* d, int capp, int capo) {
   PAttnPlan p;
   const int gq = d->Hq / d->own_pool.heads;
@@ -978,8 +985,8 @@ static PAttnPlan plan_attn(const slx_prefix_attn_desc* d, int capp, int capo) {
   p.whole = 0;
   p.ko = kind(ro, d->own_pool);
   p.kp = capp > 0 ? kind(rp, d->prefix_pool) : p.ko;
-  if (capp > 0 && p.kp >= kS64 && p.ko >= kS64 && seqs * t64 >= kWhole && up + uo <= kWholeUnits) {
-    p.ko = p.kp = seqs * t128 >= 2 * kWhole ? kS128 : kS64;
+  if (capp > 0 && p.kp >= kS64 && p.ko >= kS64 && up + uo <= whole_units(d->own_pool.head_dim, seqs * t64)) {
+    p.ko = p.kp = 2 * seqs * t128 >= 3 * kCUs ? kS128 : kS64;
     p.whole = p.ko == kS64 && seqs * t64 <= kCUs ? 8 : 4;  // one workgroup a CU: 8 waves (17.5 -> 14.9 us above); two of them: 4 (340: 23.4, 29.2)
     p.mto = p.mtp = (int)(p.ko == kS128 ? t128 : t64);
     p.nsp = p.nso = 1;
