@@ -30,7 +30,9 @@ static int log2_exact(int x) {
 
 // ---- slx_kv_append ---------------------------------------------------------------------------------------------
 // rotate_half RoPE: (x_j, x_{j + D/2}) -> (x_j cos - x_{j+D/2} sin, x_{j+D/2} cos + x_j sin), f32, rounded once.
-// One thread takes the pair of 8-element chunks c and c + D/16 of one head (16-B loads and stores).
+// One thread takes the pair of 8-element chunks c and c + D/16 of one head (16-B loads and stores); a workgroup takes as many rows
+// as fill it, so that neighbours read one row's cos and sin. Memory bound: 61 x 211 rows of 32 + 2 x 8 heads of 128, 317 MB in
+// 60 us = 5.3 TB/s, the rate of a large copy. 798 rows of 14 + 2 x 2 heads of 64: 3.0 us, 4 rows: 2.1 us, of which a launch is 2.
 struct AppendArgs {
   PoolView p;
   const bf16* qkv; long ldqkv;
@@ -103,14 +105,21 @@ __global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs a) {
 // of one d: a lane takes D/16 neighbouring d of each of its 8 keys and pairs them with v_perm_b32 (the MFMA row r of
 // product e stands for d = (D/16) r + e). The row sums are one more MFMA, with an A operand of ones.
 //
-// Two forms of a workgroup (4 waves), by the rows that share the keys:
-//   direct (up to 32 rows): all waves have the same rows; each takes every fourth 32-key tile straight into registers
-//     (K's next tile is requested once the scores have used the last, V's after the output has), the waves' states are
-//     merged through LDS at the end. Few rows: the bytes in flight count, and no wave waits for another.
-//   streamed (more rows): 64 or 128 rows, 16 or 32 a wave, so the keys are fetched once for all of them: tiles of 32 keys
-//     arrive by LDS-DMA in a ring, one barrier a step. Rows of K and V lie in LDS with their 16-B chunks XOR-ed by
-//     the slot (and slots with bits 0 and 2 swapped), which keeps both operands' reads free of bank conflicts. One page
-//     number a wave and tile (scalar load), so pages of at least 8 slots; smaller ones take the direct form.
+// Two forms of a workgroup, by the rows that share the keys:
+//   direct (up to 16 rows, or 32 of a cache with pages of less than 8 slots): all 4 waves have the same rows; each takes every
+//     fourth 32-key tile straight into registers (K's next tile is requested once the scores have used the last, V's after the
+//     output has), the waves' states are merged through LDS at the end. Few rows: the bytes in flight count, and no wave waits
+//     for another.
+//   streamed: 64 or 128 rows, so the keys are fetched once for all of them: tiles of 32 keys arrive by LDS-DMA in a ring, one
+//     barrier a step. Rows of K and V lie in LDS with their 16-B chunks XOR-ed by the slot (and slots with bits 0 and 2
+//     swapped), which keeps both operands' reads of 64 elements free of bank conflicts (of 128: 27 % of the LDS cycles). One
+//     page number for 8 keys (scalar load), so pages of at least 8 slots.
+//
+// Measured (main launch + join; 14 heads on 2 of 64 unless said). 2 x 16 sequences on 32771 shared and 300 .. 1000 own keys: 19.4 +
+// 4.9 us, of which memory needs 8.5 (44 MB at 5.2 TB/s); VALU 28 % and MFMA 10 % of the SIMDs' cycles, the rest is the wait for the
+// first tiles (5 us before and after the steps), the steps of few waves and uneven CUs. 32 on 16411 + 2000 of 32 heads on 8 of 128:
+// 52.8 + 4.9 us, 215 MB = 3.7 TB/s. 8 x 8 on 1086: 8.0 + 3.1 us and 1 x 4 on 798: 6.2 + 2.3 us, where a launch takes 2 and the chain
+// length -> page numbers -> keys -> merge the rest.
 struct Seg {
   PoolView p;
   const int* tab; long ldt;
@@ -886,7 +895,9 @@ __global__ __launch_bounds__(64 * NW, 2) void prefix_attn_whole_kernel(PAttnArgs
 }
 
 // Joins the parts of a row: D / 4 threads, four d each, times PG groups that share the parts out, B at a time: up to 8 parts at
-// once by one group, up to 16 by four, more by a whole workgroup, so that the loads of a row make few rounds.
+// once by one group, up to 16 by four, more by a whole workgroup, so that the loads of a row make few rounds. 8 parts of 56 rows:
+// 2.4 us by one group, 3.3 by four; 11 parts of 896 rows: 3.1 by four, 4.0 by one, 4.3 by the workgroup; 22 parts of 1024 rows of 128:
+// 4.9 (12 MB, 2.4 TB/s).
 template <int D, int PG, int B>
 __global__ __launch_bounds__(256) void prefix_attn_join_kernel(PAttnArgs a) {
   constexpr int TPR = D / 4, RPB = 256 / (TPR * PG);
@@ -975,7 +986,10 @@ static PAttnPlan plan_attn(const slx_prefix_attn_desc* d, int capp, int capo) {
   PAttnPlan p;
   const int gq = d->Hq / d->own_pool.heads;
   auto kind = [](long rows, const slx_kv_pool& pool) {
-    // streamed tiles: one page number for 8 keys, whose offsets on the page fit 32 bits
+    // Streamed tiles: one page number for 8 keys, whose offsets on the page fit 32 bits. Direct / streamed, us: 14 rows on 798
+    // keys 5.7 / 6.2, on 32771 11.5 / 12.5; 28 rows 7.0 / 6.4 and 13.8 / 12.3; heads of 128, 12 rows on 16411 18.4 / 19.4, 32
+    // rows 27.0 / 25.6. 64 / 128 rows a tile, with the join: 112 rows on 32771 keys 24.6 / 24.7, on 1086 12.9 / 13.8, heads of
+    // 128, 128 rows on 16411 62.4 / 58.3 (the keys pass through L2 once instead of twice).
     const bool streams = pool.page >= 8 && pool.slot_stride < (1 << 27);
     return rows <= 16 ? kD16 : !streams ? kD32 : rows <= 64 ? kS64 : kS128;
   };
