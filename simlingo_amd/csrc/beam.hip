@@ -13,6 +13,8 @@
 // -> candidates -> rank, with a barrier in between, is 3 us for one workgroup and 10 us where five share a CU; the second launch has one workgroup
 // a batch entry and follows scores, lists, logarithm, ranks and the last ranking. 8192 columns a workgroup: 22.2 us
 // instead of 20.2 together, 8 x 16 rows of f32, 32 chosen: 40.3 instead of 37.3.
+#include <type_traits>
+
 #include "common.h"
 #include "../../include/slx.h"
 
@@ -147,7 +149,7 @@ __global__ __launch_bounds__(256) void beam_chunk_kernel(SelArgs a) {
   for (int e = 0; e < E; ++e) l += __expf(v[e] - ms);
   l = wave_fsum(l);
 
-  // a threshold with at least K of the chunk's columns at or above it: the K-th largest of the 256 threads' own maxima, halved
+  // a threshold with at least K of the chunk's columns at or above it: the K-th largest of the threads' own maxima, halved
   // into from both ends until few more than K are left (-inf: fewer threads than K, or -inf itself)
   smax[tid] = n ? om : 0u;
   if (lane == 0) sml[wave] = make_float2(mw, l);
@@ -164,10 +166,15 @@ __global__ __launch_bounds__(256) void beam_chunk_kernel(SelArgs a) {
       x[i] = smax[64 * i + lane];
       mx = max(mx, x[i]);
     }
-    int finite = 0;
+    if (a.K <= 32) {  // of 64 groups of four threads: a few candidates more, a quarter of the work (12.5 -> 10.5 us of 16 chosen)
+      const unsigned y[1] = {mx};
+      if (__popcll(__ballot(mx > 0x007FFFFFu)) >= a.K) tv = unord_f(kth_below(y, 0x00800000u, wave_umax(mx), a.K));  // above -inf
+    } else {
+      int finite = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) finite += __popcll(__ballot(x[i] > 0x007FFFFFu));  // above -inf
-    if (finite >= a.K) tv = unord_f(kth_below(x, 0x00800000u, wave_umax(mx), a.K));
+      for (int i = 0; i < 4; ++i) finite += __popcll(__ballot(x[i] > 0x007FFFFFu));
+      if (finite >= a.K) tv = unord_f(kth_below(x, 0x00800000u, wave_umax(mx), a.K));
+    }
   }
   int at = 0;  // this wave's candidates
 #pragma unroll
@@ -295,10 +302,8 @@ __global__ __launch_bounds__(1024) void beam_pick_kernel(SelArgs a) {
         const int lists = __popcll(__ballot(head != 0)), q = (K + lists - 1) / lists;
         u64 bar;
         if (q == 1) {
-          int rank = 0;
-          for (int i = 0; i < a.C; ++i) rank += lane_u64(head, i) > head;
-          const u64 atk = __ballot(rank == K - 1 && head);  // (heads are all different, but for empty lists)
-          bar = lane_u64(head, (int)__ffsll((long long)atk) - 1);
+          const unsigned h[1] = {(unsigned)(head >> 32)};
+          bar = (u64)kth_below(h, 1, wave_umax(h[0]), K) << 32;
         } else {  // fewer lists than K: the least of their q-th keys has q keys of each list at or above it
           bar = ~wave_kmax(~(lane < a.C && head ? lp[q - 1] : ~0ull));
           if (!bar) bar = 1;
@@ -328,7 +333,7 @@ __global__ __launch_bounds__(1024) void beam_pick_kernel(SelArgs a) {
           x[i] = (unsigned)(k[i] >> 32);
           mx = max(mx, x[i]);
         }
-        if (cnt > K + 16) t = kth_below(x, 0, wave_umax(mx), K);
+        if (cnt > 64) t = kth_below(x, 0, wave_umax(mx), K);
         wave_fence();
         cnt = 0;
 #pragma unroll
@@ -385,10 +390,12 @@ __global__ __launch_bounds__(1024) void beam_pick_kernel(SelArgs a) {
   if (a.W * K <= kSelFew) {
     // few entries: those from the K-th largest high word of the scores on, and the rank of each among them; equal scores in
     // the order of the lists, which is that of w * V + t
-    u64 k[kSelFew / 64];
-    unsigned x[kSelFew / 64], mx = 0, t = 0;
+    auto few = [&](auto nn) {
+      constexpr int N = decltype(nn)::value;
+    u64 k[N];
+    unsigned x[N], mx = 0, t = 0;
 #pragma unroll
-    for (int i = 0; i < kSelFew / 64; ++i) {
+    for (int i = 0; i < N; ++i) {
       const int j = lane + 64 * i;
       k[i] = j < a.W * K && ti[j] >= 0 ? sc[j] : 0;  // 0: none (-inf has bits)
       x[i] = (unsigned)(k[i] >> 32);
@@ -397,7 +404,7 @@ __global__ __launch_bounds__(1024) void beam_pick_kernel(SelArgs a) {
     if (a.W * K > K + 16) t = kth_below(x, 0, wave_umax(mx), K);
     int cnt = 0;
 #pragma unroll
-    for (int i = 0; i < kSelFew / 64; ++i) {
+    for (int i = 0; i < N; ++i) {
       const bool in = k[i] && x[i] >= t;
       const u64 m = __ballot(in);
       const int to = cnt + __popcll(m & ((1ull << lane) - 1));
@@ -412,6 +419,9 @@ __global__ __launch_bounds__(1024) void beam_pick_kernel(SelArgs a) {
       for (int i = 0; i < cnt; ++i) r += cand[i] > v || (cand[i] == v && i < j);
       if (r < K) write(r, ci[j], v);
     }
+    };
+    if (a.W * K <= 128) few(std::integral_constant<int, 2>());
+    else few(std::integral_constant<int, kSelFew / 64>());
     return;
   }
   // The k best of the rows' sorted lists, a list a lane: k rounds of the wave's largest head (its low word among the lanes
