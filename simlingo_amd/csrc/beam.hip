@@ -8,11 +8,11 @@
 // second launch forms the row sums, the scores (64 bits, from exact 32-bit maxima and sums of at most 4096 terms each)
 // and the k best of all rows.
 //
-// Measured: 4 rows of 151655 f32 logits, 4 chosen: 5.2 + 5.3 us (the logits alone: 0.5 us at 5.2 TB/s); 8 x 8 rows of bf16, a quarter of
-// them at their end, 16 chosen: 12.5 + 8.8 us (2.8). Bound by latency: a launch takes 2 us; the chain load -> maximum -> threshold
-// -> candidates -> rank, with a barrier in between, is 3 us for one workgroup and 10 us where five share a CU; the second launch has one workgroup
-// a batch entry and follows scores, lists, logarithm, ranks and the last ranking. 8192 columns a workgroup: 22.2 us
-// instead of 20.2 together, 8 x 16 rows of f32, 32 chosen: 40.3 instead of 37.3.
+// Measured: 4 rows of 151655 f32 logits, 4 chosen: 4.8 + 4.8 us (the logits alone: 0.5 us at 5.2 TB/s); 8 x 8 rows of bf16, a
+// quarter of them at their end, 16 chosen: 10.6 + 7.4 us (2.8). Bound by latency (a launch takes 2 us, the chain load -> maximum
+// -> threshold -> candidates -> rank with two barriers 3) and, where seven workgroups share a CU, by the instructions of that
+// chain; the second launch has one workgroup a batch entry, a wave a row: scores, lists, logarithm, ranks, the last ranking.
+// 8192 columns a workgroup instead: 2 us more, at 8 x 16 rows of f32, 32 chosen, 3 of 37.
 #include <type_traits>
 
 #include "common.h"
@@ -388,37 +388,37 @@ __global__ __launch_bounds__(1024) void beam_pick_kernel(SelArgs a) {
     if (a.fin_out) a.fin_out[o] = fin_s[w] || t == a.eos;
   };
   if (a.W * K <= kSelFew) {
-    // few entries: those from the K-th largest high word of the scores on, and the rank of each among them; equal scores in
+    // few entries (8 values a lane, or 2: 0.4 us of 8 rows' 16): those from the K-th largest high word of the scores on, and the rank of each among them; equal scores in
     // the order of the lists, which is that of w * V + t
     auto few = [&](auto nn) {
       constexpr int N = decltype(nn)::value;
-    u64 k[N];
-    unsigned x[N], mx = 0, t = 0;
+      u64 k[N];
+      unsigned x[N], mx = 0, t = 0;
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int j = lane + 64 * i;
-      k[i] = j < a.W * K && ti[j] >= 0 ? sc[j] : 0;  // 0: none (-inf has bits)
-      x[i] = (unsigned)(k[i] >> 32);
-      mx = max(mx, x[i]);
-    }
-    if (a.W * K > K + 16) t = kth_below(x, 0, wave_umax(mx), K);
-    int cnt = 0;
+      for (int i = 0; i < N; ++i) {
+        const int j = lane + 64 * i;
+        k[i] = j < a.W * K && ti[j] >= 0 ? sc[j] : 0;  // 0: none (-inf has bits)
+        x[i] = (unsigned)(k[i] >> 32);
+        mx = max(mx, x[i]);
+      }
+      if (a.W * K > K + 16) t = kth_below(x, 0, wave_umax(mx), K);
+      int cnt = 0;
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const bool in = k[i] && x[i] >= t;
-      const u64 m = __ballot(in);
-      const int to = cnt + __popcll(m & ((1ull << lane) - 1));
-      if (in) { cand[to] = k[i]; ci[to] = lane + 64 * i; }
-      cnt += __popcll(m);
-    }
-    wave_fence();
-    for (int j = lane; j < cnt; j += 64) {
-      const u64 v = cand[j];
-      int r = 0;
+      for (int i = 0; i < N; ++i) {
+        const bool in = k[i] && x[i] >= t;
+        const u64 m = __ballot(in);
+        const int to = cnt + __popcll(m & ((1ull << lane) - 1));
+        if (in) { cand[to] = k[i]; ci[to] = lane + 64 * i; }
+        cnt += __popcll(m);
+      }
+      wave_fence();
+      for (int j = lane; j < cnt; j += 64) {
+        const u64 v = cand[j];
+        int r = 0;
 #pragma unroll 4
-      for (int i = 0; i < cnt; ++i) r += cand[i] > v || (cand[i] == v && i < j);
-      if (r < K) write(r, ci[j], v);
-    }
+        for (int i = 0; i < cnt; ++i) r += cand[i] > v || (cand[i] == v && i < j);
+        if (r < K) write(r, ci[j], v);
+      }
     };
     if (a.W * K <= 128) few(std::integral_constant<int, 2>());
     else few(std::integral_constant<int, kSelFew / 64>());
