@@ -576,7 +576,7 @@ int64_t slx_beam_select_ws_bytes(const slx_beam_select_desc* d); /* < 0: bad arg
 typedef struct slx_beam_reorder_desc {
   const void* src; void* dst;
   int64_t s0, s1, src_row, d0, d1, dst_row, row_bytes;
-  int n0, n1, batch, width;                  /* width <= 64                                                            */
+  int n0, n1, batch, width;                  /* width <= 64, n0 * n1 * batch < 2^31                                    */
   const int* parent;                         /* [batch][width]                                                         */
 } slx_beam_reorder_desc;
 int slx_beam_reorder(const slx_beam_reorder_desc* d, slx_stream_t s);

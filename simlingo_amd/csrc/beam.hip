@@ -445,8 +445,8 @@ __global__ __launch_bounds__(1024) void beam_pick_kernel(SelArgs a) {
 // ---- slx_beam_reorder: x[o, b, w] = x[o, b, parent[b, w]] -------------------------------------------------------
 // A thread takes one column of all `width` rows of a batch entry: every row is loaded before any is stored, so the
 // state may be reordered in place, whatever the parents; in place, rows that stay are neither read nor written. Memory bound where
-// it is large: 24 x 4 x 8 rows of bf16, the first 16256 of 32768 elements used, in place with half of the rows staying: 6.6 us for 25 MB
-// read and written; a table of 8 x 8 rows of 101 numbers 4.2 us, of which a launch takes 2 and the chain parent -> row the rest.
+// it is large: 24 x 4 x 8 rows of bf16, the first 16256 of 32768 elements used, in place with half of the rows staying: 6.0 us for 25 MB
+// read and written; a table of 8 x 8 rows of 101 numbers 3.5 us, of which a launch takes 2 and the chain parent -> row the rest.
 struct ReorderArgs {
   const char* src; char* dst;
   long s0, s1, sr, d0, d1, dr;  // byte strides: two outer axes and the rows, of source and destination
@@ -460,19 +460,22 @@ template <typename T, int MW>
 __global__ __launch_bounds__(256) void beam_reorder_kernel(ReorderArgs a) {
   const long c = (long)blockIdx.x * 256 + threadIdx.x;
   if (c >= a.cols) return;
-  for (long o = blockIdx.y; o < (long)a.n0 * a.n1 * a.B; o += gridDim.y) {
-    const long b = o % a.B, q = o / a.B, i1 = q % a.n1, i0 = q / a.n1;
-    const int* par = a.parent + b * a.W;
-    const char* sp = a.src + i0 * a.s0 + i1 * a.s1 + b * a.W * a.sr + c * (long)sizeof(T);
-    char* dp = a.dst + i0 * a.d0 + i1 * a.d1 + b * a.W * a.dr + c * (long)sizeof(T);
+  const unsigned n = (unsigned)a.n0 * (unsigned)a.n1 * (unsigned)a.B;  // < 2^31
+  for (unsigned o = blockIdx.y; o < n; o += gridDim.y) {
+    const unsigned q = o / (unsigned)a.B, b = o - q * (unsigned)a.B, i0 = q / (unsigned)a.n1, i1 = q - i0 * (unsigned)a.n1;
+    const int* par = a.parent + (long)b * a.W;
+    int from[MW];  // all requested before one is looked at
+#pragma unroll
+    for (int w = 0; w < MW; ++w) from[w] = par[min(w, a.W - 1)];
+    const char* sp = a.src + i0 * a.s0 + i1 * a.s1 + (long)b * a.W * a.sr + c * (long)sizeof(T);
+    char* dp = a.dst + i0 * a.d0 + i1 * a.d1 + (long)b * a.W * a.dr + c * (long)sizeof(T);
     T v[MW];
     bool mv[MW];
 #pragma unroll
     for (int w = 0; w < MW; ++w) {
       mv[w] = w < a.W;
       if (mv[w]) {
-        int p = par[w];
-        if ((unsigned)p >= (unsigned)a.W) p = w;  // no such beam: the row stays
+        const int p = (unsigned)from[w] < (unsigned)a.W ? from[w] : w;  // no such beam: the row stays
         mv[w] = !(a.in_place && p == w);
         if (mv[w]) v[w] = *reinterpret_cast<const T*>(sp + p * a.sr);
       }
@@ -567,6 +570,7 @@ int slx_beam_reorder(const slx_beam_reorder_desc* d, slx_stream_t s) {
   const int w = (u & 15) == 0 ? 16 : (u & 3) == 0 ? 4 : (u & 1) == 0 ? 2 : 1;
   a.cols = d->row_bytes / w;
   SLX_CHECK_ARG((a.cols + 255) / 256 < 2147483648L, "slx_beam_reorder: rows too long");
+  SLX_CHECK_ARG((double)d->n0 * d->n1 * d->batch < 2147483648.0, "slx_beam_reorder: n0 * n1 * batch must be < 2^31");
   if (w == 16) reorder_launch<u32x4>(a, (hipStream_t)s);
   else if (w == 4) reorder_launch<unsigned>(a, (hipStream_t)s);
   else if (w == 2) reorder_launch<unsigned short>(a, (hipStream_t)s);

@@ -189,7 +189,7 @@ def test_c_entries_refuse():
     assert lib.slx_beam_select(ctypes.byref(PG.BeamSelectDesc(**{**se, "batch": 0})), None) == 0
     re_ = dict(src=4096, dst=4096, src_row=64, dst_row=64, row_bytes=64, n0=1, n1=1, batch=1, width=2, parent=4096)
     for kw, text in ((dict(width=0), b"width"), (dict(width=65), b"width"), (dict(batch=-1), b"extents"), (dict(row_bytes=-4), b"extents"), (dict(parent=0), b"null"),
-                     (dict(dst_row=128), b"equal strides")):
+                     (dict(dst_row=128), b"equal strides"), (dict(n0=1 << 16, n1=1 << 15), b"2^31")):
         refused("slx_beam_reorder", PG.BeamReorderDesc(**{**re_, **kw}), text)
     refused("slx_beam_reorder", None, b"null")
 
