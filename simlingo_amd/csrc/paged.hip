@@ -118,7 +118,7 @@ __global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs a) {
 // Measured (main launch + join; 14 heads on 2 of 64 unless said). 2 x 16 sequences on 32771 shared and 300 .. 1000 own keys: 19.4 +
 // 4.9 us, of which memory needs 8.5 (44 MB at 5.2 TB/s); VALU 28 % and MFMA 10 % of the SIMDs' cycles, the rest is the wait for the
 // first tiles (5 us before and after the steps), the steps of few waves and uneven CUs. 32 on 16411 + 2000 of 32 heads on 8 of 128:
-// 52.8 + 4.9 us, 215 MB = 3.7 TB/s. 8 x 8 on 1086: 8.0 + 3.1 us and 1 x 4 on 798: 6.2 + 2.3 us, where a launch takes 2 and the chain
+// 52.8 + 4.9 us, 215 MB = 3.7 TB/s. 8 x 8 on 1086: 7.5 + 3.1 us and 1 x 4 on 798: 5.6 + 2.4 us, where a launch takes 2 and the chain
 // length -> page numbers -> keys -> merge the rest.
 struct Seg {
   PoolView p;
@@ -571,13 +571,16 @@ __device__ __forceinline__ void wait_tiles(int younger) {
 __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 // 16 B a lane from base + off (bytes) to LDS at lds + 16 * lane
 __device__ __forceinline__ void dma16(const void* base, unsigned off, unsigned lds) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base) : "memory");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base) : "memory", "m0");
 }
-// A streamed workgroup: NW waves over RW rows, 16 NQ rows a wave, and as many teams as that leaves, each of which takes tiles of
-// its own of every step of the ring, T tiles of 32 keys; the teams are joined at the end.
-template <int D, int RW, int NW>
+
+// A streamed workgroup: NW waves, RV of them side by side over RW rows, and as many teams as that leaves, each of which takes tiles
+// of its own of every step of the ring, T tiles of 32 keys; the teams are joined at the end. With two teams of 64 rows of 64 elements
+// an operand read from LDS serves 32 rows of a wave instead of 16: 23.2 us instead of 24.4 for 340 whole-row tiles; a range of
+// 128 keys is over before that pays for the join of the teams: 6.5 us instead of 5.6 for 4 sequences on 798 keys.
+template <int D, int RW, int NW, int RV>
 struct Shape {
-  static constexpr int RWV = D == 64 ? RW / 32 : 4, NQ = RW / 16 / RWV, TEAMS = NW / RWV;
+  static constexpr int RWV = RV, NQ = RW / 16 / RWV, TEAMS = NW / RWV;
   static constexpr int T = TEAMS > 1 ? TEAMS : D == 64 ? 2 : 1, UW = T / TEAMS;  // tiles a step, and of them a team's
   static constexpr int SLOTS = D == 128 && T == 1 ? 4 : 3;
   static constexpr int LDS = SLOTS * (T * 2 * 32 * D * 2 + 4 * T);
@@ -585,10 +588,10 @@ struct Shape {
 
 // The keys of one segment into the state of a wave's rows r0 .. (the workgroup's from rw); whether values were sifted out.
 // The LDS is free when it is called, and its last tiles may still be read when it returns.
-template <int D, int RW, int NW>
+template <int D, int RW, int NW, int RV>
 __device__ __forceinline__ bool stream_keys(const PAttnArgs& a, const Item& w, int rw, int r0,
-                                            const bf16x8 (&qf)[Shape<D, RW, NW>::NQ][D / 32], State<D, Shape<D, RW, NW>::NQ>& st, char* smem) {
-  typedef Shape<D, RW, NW> S;
+                                            const bf16x8 (&qf)[Shape<D, RW, NW, RV>::NQ][D / 32], State<D, Shape<D, RW, NW, RV>::NQ>& st, char* smem) {
+  typedef Shape<D, RW, NW, RV> S;
   constexpr int KK = D / 32, NE = D / 16, CH = D / 8, TILE = 32 * D * 2, T = S::T, SLOTS = S::SLOTS, STEP = 32 * T, NQ = S::NQ, UW = S::UW;
   constexpr int TI = 4 * T / NW;       // tiles of a step that a wave brings 8 keys of
   constexpr int PER = TI * 2 * D / 64;  // DMA pieces a wave and step
@@ -735,10 +738,10 @@ __device__ __forceinline__ void settle_rows(bf16x8 (&qf)[NQ][D / 32]) {
     for (int k = 0; k < D / 32; ++k) asm volatile("" : "+v"(qf[n][k]));
 }
 
-template <int D, int RW, int NW>
-__device__ __forceinline__ void store_stream(const PAttnArgs& a, const Item& w, int r0, bool odd, State<D, Shape<D, RW, NW>::NQ>& st,
+template <int D, int RW, int NW, int RV>
+__device__ __forceinline__ void store_stream(const PAttnArgs& a, const Item& w, int r0, bool odd, State<D, Shape<D, RW, NW, RV>::NQ>& st,
                                              char* smem) {
-  typedef Shape<D, RW, NW> S;
+  typedef Shape<D, RW, NW, RV> S;
   constexpr int NQ = S::NQ, NE = D / 16, HAND = NQ * (NE + 1) * 64;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15;
   odd = __any(odd);
@@ -785,16 +788,16 @@ __device__ __forceinline__ void store_stream(const PAttnArgs& a, const Item& w, 
   }
 }
 
-template <int D, int RW, int NW>
+template <int D, int RW, int NW, int RV>
 __device__ __forceinline__ int wave_row(int rw) {  // a wave's first row
-  typedef Shape<D, RW, NW> S;
+  typedef Shape<D, RW, NW, RV> S;
   return rw + (__builtin_amdgcn_readfirstlane(threadIdx.x >> 6) % S::RWV) * 16 * S::NQ;
 }
 
-template <int D, int RW, int NW>
+template <int D, int RW, int NW, int RV>
 __device__ __forceinline__ void attn_stream(const PAttnArgs& a, Item w, char* smem) {
-  constexpr int NQ = Shape<D, RW, NW>::NQ;
-  const int rw = w.mt * RW, r0 = wave_row<D, RW, NW>(rw);
+  constexpr int NQ = Shape<D, RW, NW, RV>::NQ;
+  const int rw = w.mt * RW, r0 = wave_row<D, RW, NW, RV>(rw);
   bf16x8 qf[NQ][D / 32];
   load_rows<D, NQ>(a, w, r0, qf);
   asm volatile("" ::: "memory");  // the queries are requested before the length is waited for
@@ -802,8 +805,8 @@ __device__ __forceinline__ void attn_stream(const PAttnArgs& a, Item w, char* sm
   State<D, NQ> st;
   state_init(st);
   settle_rows<D, NQ>(qf);
-  const bool odd = stream_keys<D, RW, NW>(a, w, rw, r0, qf, st, smem);
-  store_stream<D, RW, NW>(a, w, r0, odd, st, smem);
+  const bool odd = stream_keys<D, RW, NW, RV>(a, w, rw, r0, qf, st, smem);
+  store_stream<D, RW, NW, RV>(a, w, r0, odd, st, smem);
 }
 
 // kinds of a workgroup: direct with 16 or 32 rows, streamed with 64 or 128
@@ -813,12 +816,12 @@ template <int D, int KIND>
 __device__ __forceinline__ void attn_kind(const PAttnArgs& a, const Item& w, char* smem) {
   if constexpr (KIND == kD16) attn_direct<D, 1>(a, w, smem);
   else if constexpr (KIND == kD32) attn_direct<D, 2>(a, w, smem);
-  else if constexpr (KIND == kS64) attn_stream<D, 64, 4>(a, w, smem);
-  else attn_stream<D, 128, 4>(a, w, smem);
+  else if constexpr (KIND == kS64) attn_stream<D, 64, 4, 4>(a, w, smem);
+  else attn_stream<D, 128, 4, 4>(a, w, smem);
 }
 template <int D>
 constexpr int kind_lds(int kind) {
-  return kind == kS64 ? Shape<D, 64, 4>::LDS : kind == kS128 ? Shape<D, 128, 4>::LDS : 2 * 4 * 16 * (kind + 1) * 4 + 2 * (kind + 1) * (D / 16) * 64 * 16;
+  return kind == kS64 ? Shape<D, 64, 4, 4>::LDS : kind == kS128 ? Shape<D, 128, 4, 4>::LDS : 2 * 4 * 16 * (kind + 1) * 4 + 2 * (kind + 1) * (D / 16) * 64 * 16;
 }
 
 template <int D, int KP, int KO>
@@ -864,10 +867,10 @@ __global__ __launch_bounds__(256, 2) void prefix_attn_kernel(PAttnArgs a) {
 
 // Many new tokens in many sequences: a workgroup takes 64 or 128 rows of ONE sequence through the prefix and then its own
 // keys, so there are no parts to write and join (the prefix is fetched again for every tile of rows, from L2).
-template <int D, int RW, int NW>
+template <int D, int RW, int NW, int RV>
 __global__ __launch_bounds__(64 * NW, 2) void prefix_attn_whole_kernel(PAttnArgs a) {
-  constexpr int NQ = Shape<D, RW, NW>::NQ;
-  __shared__ __attribute__((aligned(16))) char smem[Shape<D, RW, NW>::LDS];
+  constexpr int NQ = Shape<D, RW, NW, RV>::NQ;
+  __shared__ __attribute__((aligned(16))) char smem[Shape<D, RW, NW, RV>::LDS];
   unsigned b = blockIdx.x;  // [kv head][sequence][row tile]: neighbours share the prefix
   Item w;
   w.mt = (int)(b % (unsigned)a.mt_own);
@@ -877,7 +880,7 @@ __global__ __launch_bounds__(64 * NW, 2) void prefix_attn_whole_kernel(PAttnArgs
   w.tok0 = (long)seq * a.Tq;
   w.ntok = a.Tq;
   w.range = w.part = 0;
-  const int rw = w.mt * RW, r0 = wave_row<D, RW, NW>(rw);
+  const int rw = w.mt * RW, r0 = wave_row<D, RW, NW, RV>(rw);
   bf16x8 qf[NQ][D / 32];
   load_rows<D, NQ>(a, w, r0, qf);
   asm volatile("" ::: "memory");  // the queries are requested before the lengths are waited for
@@ -886,12 +889,12 @@ __global__ __launch_bounds__(64 * NW, 2) void prefix_attn_whole_kernel(PAttnArgs
   State<D, NQ> st;
   state_init(st);
   settle_rows<D, NQ>(qf);
-  stream_keys<D, RW, NW>(a, w, rw, r0, qf, st, smem);
+  stream_keys<D, RW, NW, RV>(a, w, rw, r0, qf, st, smem);
   item_segment(w, a.own, seq, true);
   item_range(a, w, RW);
   lds_barrier();  // the ring is free when every wave has read the prefix's last tiles
-  const bool odd = stream_keys<D, RW, NW>(a, w, rw, r0, qf, st, smem);
-  store_stream<D, RW, NW>(a, w, r0, odd, st, smem);
+  const bool odd = stream_keys<D, RW, NW, RV>(a, w, rw, r0, qf, st, smem);
+  store_stream<D, RW, NW, RV>(a, w, r0, odd, st, smem);
 }
 
 // Joins the parts of a row: D / 4 threads, four d each, times PG groups that share the parts out, B at a time: up to 8 parts at
@@ -987,7 +990,7 @@ static PAttnPlan plan_attn(const slx_prefix_attn_desc* d, int capp, int capo) {
   const int gq = d->Hq / d->own_pool.heads;
   auto kind = [](long rows, const slx_kv_pool& pool) {
     // Streamed tiles: one page number for 8 keys, whose offsets on the page fit 32 bits. Direct / streamed, us: 14 rows on 798
-    // keys 5.7 / 6.2, on 32771 11.5 / 12.5; 28 rows 7.0 / 6.4 and 13.8 / 12.3; heads of 128, 12 rows on 16411 18.4 / 19.4, 32
+    // keys 5.7 / 6.2, on 32771 11.5 / 12.5; 28 rows 7.0 / 5.6 and 13.8 / 12.3; heads of 128, 12 rows on 16411 18.4 / 19.4, 32
     // rows 27.0 / 25.6. 64 / 128 rows a tile, with the join: 112 rows on 32771 keys 24.6 / 24.7, on 1086 12.9 / 13.8, heads of
     // 128, 128 rows on 16411 62.4 / 58.3 (the keys pass through L2 once instead of twice).
     const bool streams = pool.page >= 8 && pool.slot_stride < (1 << 27);
@@ -1063,9 +1066,9 @@ static int check_attn(const slx_prefix_attn_desc* d, int* capp, int* capo) {
 template <int D>
 static bool launch_attn(const PAttnPlan& p, dim3 grid, hipStream_t st, const PAttnArgs& a) {
   if (p.whole) {
-    if (p.ko == kS128) hipLaunchKernelGGL((prefix_attn_whole_kernel<D, 128, 4>), grid, dim3(256), 0, st, a);
-    else if (p.whole == 8) hipLaunchKernelGGL((prefix_attn_whole_kernel<D, 64, 8>), grid, dim3(512), 0, st, a);
-    else hipLaunchKernelGGL((prefix_attn_whole_kernel<D, 64, 4>), grid, dim3(256), 0, st, a);
+    if (p.ko == kS128) hipLaunchKernelGGL((prefix_attn_whole_kernel<D, 128, 4, 4>), grid, dim3(256), 0, st, a);
+    else if (p.whole == 8) hipLaunchKernelGGL((prefix_attn_whole_kernel<D, 64, 8, D == 64 ? 2 : 4>), grid, dim3(512), 0, st, a);
+    else hipLaunchKernelGGL((prefix_attn_whole_kernel<D, 64, 4, D == 64 ? 2 : 4>), grid, dim3(256), 0, st, a);
     return true;
   }
 #define SLX_PA(P, O)                                                                                         \
