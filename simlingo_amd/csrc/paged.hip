@@ -106,7 +106,7 @@ __global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs a) {
 // product e stands for d = (D/16) r + e). The row sums are one more MFMA, with an A operand of ones.
 //
 // Two forms of a workgroup, by the rows that share the keys:
-//   direct (up to 16 rows, or 32 of a cache with pages of less than 8 slots): all 4 waves have the same rows; each takes every
+//   direct (up to 8 rows of a prefix, 16 of own keys, or 32 of a cache with pages of less than 8 slots): all 4 waves have the same rows; each takes every
 //     fourth 32-key tile straight into registers (K's next tile is requested once the scores have used the last, V's after the
 //     output has), the waves' states are merged through LDS at the end. Few rows: the bytes in flight count, and no wave waits
 //     for another.
@@ -988,20 +988,21 @@ static long whole_units(int D, long tiles) { return tiles >= (D == 64 ? 64 : 192
 static PAttnPlan plan_attn(const slx_prefix_attn_desc* d, int capp, int capo) {
   PAttnPlan p;
   const int gq = d->Hq / d->own_pool.heads;
-  auto kind = [](long rows, const slx_kv_pool& pool) {
-    // Streamed tiles: one page number for 8 keys, whose offsets on the page fit 32 bits. Direct / streamed, us: 14 rows on 798
-    // keys 5.7 / 6.2, on 32771 11.5 / 12.5; 28 rows 7.0 / 5.6 and 13.8 / 12.3; heads of 128, 12 rows on 16411 18.4 / 19.4, 32
-    // rows 27.0 / 25.6. 64 / 128 rows a tile, with the join: 112 rows on 32771 keys 24.6 / 24.7, on 1086 12.9 / 13.8, heads of
-    // 128, 128 rows on 16411 62.4 / 58.3 (the keys pass through L2 once instead of twice).
+  auto kind = [](long rows, const slx_kv_pool& pool, long direct) {
+    // Streamed tiles: one page number for 8 keys, whose offsets on the page fit 32 bits. Direct / streamed prefixes, us: 14 rows on
+    // 798 keys 5.6 / 5.5, on 32771 11.8 / 11.5; 16 rows on 4 x 16411 11.6 / 10.0; 28 rows 7.0 / 5.6 and 13.8 / 12.3; heads of
+    // 128, 12 rows on 16411 18.2 / 19.1, 32 rows 27.0 / 25.6. Own keys, many short sequences of 7 rows beside the prefix:
+    // 19.0 / 22.5 and 7.7 / 8.5. 64 / 128 rows a tile, with the join: 112 rows on 32771 keys 24.6 / 24.7, on 1086
+    // 12.9 / 13.8, heads of 128, 128 rows on 16411 62.4 / 58.3 (the keys pass through L2 once instead of twice).
     const bool streams = pool.page >= 8 && pool.slot_stride < (1 << 27);
-    return rows <= 16 ? kD16 : !streams ? kD32 : rows <= 64 ? kS64 : kS128;
+    return rows <= (streams ? direct : 16) ? kD16 : !streams ? kD32 : rows <= 64 ? kS64 : kS128;
   };
   const long rp = (long)d->width * d->n_q * gq, ro = (long)d->n_q * gq, heads = d->own_pool.heads;
   const long seqs = (long)d->groups * d->width * heads, t64 = (ro + 63) / 64, t128 = (ro + 127) / 128;
   const long up = (capp + 127) / 128, uo = (capo + 127) / 128;  // units of 128 keys
   p.whole = 0;
-  p.ko = kind(ro, d->own_pool);
-  p.kp = capp > 0 ? kind(rp, d->prefix_pool) : p.ko;
+  p.ko = kind(ro, d->own_pool, 16);
+  p.kp = capp > 0 ? kind(rp, d->prefix_pool, 8) : p.ko;
   if (capp > 0 && p.kp >= kS64 && p.ko >= kS64 && up + uo <= whole_units(d->own_pool.head_dim, seqs * t64)) {
     p.ko = p.kp = 2 * seqs * t128 >= 3 * kCUs ? kS128 : kS64;
     p.whole = p.ko == kS64 && seqs * t64 <= kCUs ? 8 : 4;  // one workgroup a CU: 8 waves (17.5 -> 14.9 us above); two of them: 4 (340: 23.4, 29.2)
