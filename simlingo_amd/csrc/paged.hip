@@ -294,8 +294,9 @@ __device__ __forceinline__ void keep_nan(State<D, NQ>& st) {
   for (int n = 0; n < NQ; ++n) st.m[n] = st.l[n][0] != st.l[n][0] && st.m[n] == -INFINITY ? 0.f : st.m[n];
 }
 
-// V of keys that are not there becomes 0 (0 * NaN would reach every row); with `sift`, so do values that are not finite
-// in keys that some row does not see yet -> whether there were any (they are added at the end: add_nonfinite)
+// V of keys that are not there becomes 0 (0 * NaN would reach every row); with `sift`, in a tile that some row of the wave does
+// not see to its end, so do values that are not finite -> whether there were any (they are added at the end: add_nonfinite). A tile
+// that every row sees keeps them: the product takes them to every row.
 template <int D>
 __device__ __forceinline__ bool clean_v(unsigned (&vr)[8][D / 32], unsigned dead, bool sift) {
   bool odd = false;
@@ -363,8 +364,9 @@ __device__ __forceinline__ void store_row(const PAttnArgs& a, const Item& w, int
   }
 }
 
-// Values that are not finite, of the keys from the first that some row of the tile does not see: onto the rows that see
-// them (p > 0 there, so inf and NaN arrive whatever p is), in what this thread has just stored. Rare, so kept small.
+// Values that are not finite, of the keys from the 32 on that hold the first which some row does not see (no tile before is sifted):
+// onto the rows that see them (p > 0 there, so inf and NaN arrive whatever p is; where a tile was not sifted they are there already and
+// stay what they are), in what this thread has just stored. Rare, so kept small.
 template <int D>
 __device__ __forceinline__ void add_nonfinite(const PAttnArgs& a, const Item& w, int r) {
   const int grp = (threadIdx.x & 63) >> 4, t = row_token(a, r), head = w.kvh * a.gq + r - t * a.gq;
@@ -490,7 +492,7 @@ __device__ __forceinline__ void attn_direct(const PAttnArgs& a, Item w, char* sm
       entries_k(k0 + 256);
     }
     softmax_step<D, NQ, 1>(s, a.c, st, pb);
-    if (edge) odd = clean_v<D>(vr, dead, w.causal && a.Tq > 1) || odd;
+    if (edge) odd = clean_v<D>(vr, dead, w.causal && a.Tq > 1 && k0 + 32 > free_end) || odd;
     output_step<D, NQ>(vr, pb[0], st);
     if (more) {
       load_v(k0 + 128);
@@ -720,7 +722,7 @@ __device__ __forceinline__ bool stream_keys(const PAttnArgs& a, const Item& w, i
     softmax_step<D, NQ, UW>(s, a.c, st, pb);
     if (edge) {
 #pragma unroll
-      for (int v = 0; v < UW; ++v) odd = clean_v<D>(vr[v], dead[v], w.causal && a.Tq > 1) || odd;
+      for (int v = 0; v < UW; ++v) odd = clean_v<D>(vr[v], dead[v], w.causal && a.Tq > 1 && k0 + 32 * (u0 + v + 1) > free_end) || odd;
     }
 #pragma unroll
     for (int v = 0; v < UW; ++v) output_step<D, NQ>(vr[v], pb[v], st);
