@@ -524,7 +524,7 @@ typedef struct slx_kv_pool {
 typedef struct slx_kv_append_desc {
   slx_kv_pool pool;
   const void* qkv; int64_t ldqkv;            /* bf16 rows q (Hq heads) | k | v (pool.heads each)                       */
-  void* q_out; int64_t ldq;                  /* rotated q rows [rows][Hq * head_dim]; may be qkv itself; NULL: q is not read */
+  void* q_out; int64_t ldq;                  /* rotated q rows [rows][Hq * head_dim], apart from each other; may be qkv itself; NULL: q is not read */
   const int* table; int64_t ldt; int n_seq, cols;
   const int* seq;                            /* [rows] sequence of each row; NULL: row / rows_per_seq                  */
   const int* pos;                            /* [rows] position in the sequence; < 0: padding, nothing is written      */
@@ -539,7 +539,7 @@ int slx_kv_append(const slx_kv_append_desc* d, slx_stream_t s);
 typedef struct slx_prefix_attn_desc {
   slx_kv_pool prefix_pool, own_pool;
   const void* q; int64_t ldq;                /* bf16 rows [groups * width * n_q][Hq * head_dim], a sequence's n_q tokens together */
-  void* out; int64_t ldo;                    /* bf16 [rows][Hq * head_dim]; may be q                                   */
+  void* out; int64_t ldo;                    /* bf16 [rows][Hq * head_dim], rows apart from each other; may be q       */
   float* lse;                                /* optional f32 [rows][Hq]: natural log of the softmax sum (-inf: no key) */
   const int* ptab; int64_t ldpt; const int* plen;  /* [groups] prefixes; ptab NULL: none                               */
   const int* otab; int64_t ldot; const int* olen;  /* [groups * width] own keys, the n_q new tokens' last among them   */

@@ -1114,6 +1114,7 @@ int slx_kv_append(const slx_kv_append_desc* d, slx_stream_t s) {
   SLX_CHECK_ARG(d->qkv && d->table && d->pos, "slx_kv_append: null argument");
   SLX_CHECK_ARG(((uintptr_t)d->qkv & 15) == 0 && d->ldqkv % 8 == 0 && ((uintptr_t)d->q_out & 15) == 0 && d->ldq % 8 == 0,
                 "slx_kv_append: qkv and q_out rows must be 16-B aligned");
+  SLX_CHECK_ARG(!d->q_out || d->rows == 1 || d->ldq >= (int64_t)d->Hq * d->pool.head_dim, "slx_kv_append: rows of q_out overlap (ldq < Hq * head_dim)");
   SLX_CHECK_ARG((((uintptr_t)d->cos_tab | (uintptr_t)d->sin_tab) & 15) == 0, "slx_kv_append: cos and sin must be 16-B aligned");
   AppendArgs a{view(d->pool), (const bf16*)d->qkv, (long)d->ldqkv, (bf16*)d->q_out, (long)d->ldq, d->table, (long)d->ldt,
                d->n_seq, d->cols, d->seq, d->rows_per_seq > 0 ? d->rows_per_seq : 1, d->pos, (long)d->rows, d->Hq,
@@ -1144,8 +1145,9 @@ int slx_prefix_attn(const slx_prefix_attn_desc* d, slx_stream_t s) {
   SLX_CHECK_ARG(d->q && d->out && d->otab && d->olen, "slx_prefix_attn: null argument");
   SLX_CHECK_ARG((((uintptr_t)d->q | (uintptr_t)d->out) & 15) == 0 && d->ldq % 8 == 0 && d->ldo % 8 == 0,
                 "slx_prefix_attn: q and out rows must be 16-B aligned");
-  const PAttnPlan p = plan_attn(d, capp, capo);
   const int D = d->own_pool.head_dim, Hkv = d->own_pool.heads;
+  SLX_CHECK_ARG(d->ldo >= (int64_t)d->Hq * D || (int64_t)d->groups * d->width * d->n_q == 1, "slx_prefix_attn: rows of out overlap (ldo < Hq * head_dim)");
+  const PAttnPlan p = plan_attn(d, capp, capo);
   PAttnArgs a;
   memset(&a, 0, sizeof(a));
   a.q = (const bf16*)d->q; a.ldq = d->ldq; a.out = (bf16*)d->out; a.ldo = d->ldo; a.lse = d->lse;

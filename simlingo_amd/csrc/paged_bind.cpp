@@ -73,12 +73,13 @@ constexpr int64_t kIntMax = 2147483647;
 bool is_bool(const Tensor& t) { return t.scalar_type() == at::kBool || t.scalar_type() == at::kByte; }
 
 struct Rows { void* p; int64_t ld; };
-Rows rows_of(const char* who, const char* name, const Tensor& t, int64_t n, int64_t cols) {
+Rows rows_of(const char* who, const char* name, const Tensor& t, int64_t n, int64_t cols, bool written = false) {
   NEED(t.scalar_type() == at::kBFloat16 && t.dim() == 2, "%s must be a bf16 matrix", name);
   NEED(t.size(0) == n && t.size(1) >= cols, "%s must have %lld rows of at least %lld, got %lld x %lld", name, (long long)n,
        (long long)cols, (long long)t.size(0), (long long)t.size(1));
   const int64_t s0 = n > 1 ? t.stride(0) : t.size(1) / 8 * 8, s1 = t.stride(1);  // one row's stride says nothing
   NEED(s1 == 1 && s0 % 8 == 0 && ((uintptr_t)t.data_ptr() & 15) == 0, "rows of %s must be contiguous and 16-B aligned", name);
+  NEED(!written || n <= 1 || s0 >= cols, "rows of %s overlap each other", name);
   return {t.data_ptr(), s0};
 }
 
@@ -194,7 +195,7 @@ PyObject* kv_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
     d.pos = ints_of(who, "pos", pos, d.rows);
     if (seq) d.seq = ints_of(who, "seq", *seq, d.rows);
     if (q) {
-      const Rows y = rows_of(who, "q_out", *q, d.rows, heads * hd);
+      const Rows y = rows_of(who, "q_out", *q, d.rows, heads * hd, true);
       NEED(may_write(x, (heads + 2 * hkv) * hd, y, heads * hd, d.rows), "q_out overlaps qkv other than in its own q columns");
       d.q_out = y.p; d.ldq = y.ld;
     }
@@ -263,7 +264,7 @@ PyObject* prefix_attn(PyObject*, PyObject* const* a, Py_ssize_t n) {
     Tensor made;
     if (a[1] == Py_None) made = at::empty({rows, cols}, q.options());
     const Tensor& out = a[1] == Py_None ? made : tensor(a[1], who, "out");
-    const Rows o = rows_of(who, "out", out, rows, cols);
+    const Rows o = rows_of(who, "out", out, rows, cols, true);
     NEED(may_write(x, cols, o, cols, rows), "out overlaps q other than in its place");
     d.out = o.p; d.ldo = o.ld;
     if (lse) {
