@@ -7,6 +7,7 @@
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty.h>
 
+#include <algorithm>
 #include <cmath>
 #include <cstdarg>
 #include <cstdio>
@@ -94,6 +95,85 @@ bool may_write(const Rows& x, int64_t wx, const Rows& y, int64_t wy, int64_t n) 
   return delta > 0 ? delta >= wx && delta + wy <= x.ld : -delta >= wy && -delta + wx <= x.ld;
 }
 
+// ---- what is written lies apart ---------------------------------------------------------------------------------
+// The memory of a strided array in bytes: runs of `run` bytes from p, ext[i] of them st[i] apart along each axis.
+struct Box {
+  const char* p;
+  int64_t run;
+  int n;
+  int64_t ext[4], st[4];
+  Box(const void* at, int64_t run_) : p((const char*)at), run(run_), n(0) {}
+  Box& axis(int64_t e, int64_t s) {  // a run without elements stands for an empty array
+    if (e == 0) run = 0;
+    if (e > 1 && s != 0) { ext[n] = e; st[n++] = s; }
+    return *this;
+  }
+  const char* end() const {
+    const char* q = p + run;
+    for (int i = 0; i < n; ++i) q += (ext[i] - 1) * st[i];
+    return q;
+  }
+};
+Box box_of(const Rows& r, int64_t n, int64_t cols) { return Box(r.p, 2 * cols).axis(n, 2 * r.ld); }
+Box box_of(const slx_kv_pool& p, const void* at) {
+  return Box(at, 2 * p.head_dim).axis(p.n_pages, 2 * p.page_stride).axis(p.page, 2 * p.slot_stride).axis(p.heads, 2 * p.head_stride);
+}
+Box box_of(const Tensor& t) {  // contiguous, or rows of a table
+  const int64_t es = (int64_t)t.element_size();
+  if (t.dim() == 2) return Box(t.data_ptr(), es * t.size(1)).axis(t.size(0), es * t.stride(0));
+  return Box(t.data_ptr(), es * t.numel());
+}
+
+// Whether sum x_i s_i falls into [lo, hi] for whole x_i in [from_i, to_i], the largest s first: the x of an axis are those that leave
+// what the axes after it can reach, one or two where an axis is longer than all after it together. Arrays that take more than a few
+// thousand trials are taken to meet.
+struct Sum {
+  int n = 0, tries = 4096;
+  int64_t s[8], from[8], to[8], least[9], most[9];  // least, most: of the axes from i on
+  void add(int64_t stride, int64_t f, int64_t t) {
+    for (int i = 0; i < n; ++i)
+      if (s[i] == stride) { from[i] += f; to[i] += t; return; }
+    int i = n++;
+    for (; i > 0 && s[i - 1] < stride; --i) { s[i] = s[i - 1]; from[i] = from[i - 1]; to[i] = to[i - 1]; }
+    s[i] = stride; from[i] = f; to[i] = t;
+  }
+  static int64_t floor_div(int64_t a, int64_t b) { return a / b - (a % b < 0); }
+  bool reaches(int i, int64_t lo, int64_t hi) {
+    if (i == n) return lo <= 0 && hi >= 0;
+    const int64_t a = std::max(from[i], -floor_div(most[i + 1] - lo, s[i])), b = std::min(to[i], floor_div(hi - least[i + 1], s[i]));
+    for (int64_t x = a; x <= b; ++x)
+      if (--tries < 0 || reaches(i + 1, lo - x * s[i], hi - x * s[i])) return true;
+    return false;
+  }
+  bool reaches(int64_t lo, int64_t hi) {
+    least[n] = most[n] = 0;
+    for (int i = n - 1; i >= 0; --i) {
+      least[i] = least[i + 1] + from[i] * s[i];
+      most[i] = most[i + 1] + to[i] * s[i];
+    }
+    return reaches(0, lo, hi);
+  }
+};
+bool meet(const Box& a, const Box& b) {
+  if (!a.run || !b.run || a.end() <= b.p || b.end() <= a.p) return false;
+  Sum s;
+  for (int i = 0; i < a.n; ++i) s.add(a.st[i], 1 - a.ext[i], 0);
+  for (int i = 0; i < b.n; ++i) s.add(b.st[i], 0, b.ext[i] - 1);
+  const int64_t delta = b.p - a.p;
+  return s.reaches(1 - b.run - delta, a.run - 1 - delta);
+}
+// Whether two runs of one array share memory: those that differ along axis i first, by x_i > 0
+bool folds(const Box& a) {
+  if (!a.run) return false;
+  for (int i = 0; i < a.n; ++i) {
+    Sum s;
+    s.add(a.st[i], 1, a.ext[i] - 1);
+    for (int j = i + 1; j < a.n; ++j) s.add(a.st[j], 1 - a.ext[j], a.ext[j] - 1);
+    if (s.reaches(1 - a.run, a.run - 1)) return true;
+  }
+  return false;
+}
+
 slx_kv_pool pool_of(const char* who, const Tensor& k, const Tensor& v, bool written) {
   NEED(k.scalar_type() == at::kBFloat16 && v.scalar_type() == at::kBFloat16 && k.dim() == 4,
        "k and v must be bf16 [pages, page, heads, head size]");
@@ -112,6 +192,8 @@ slx_kv_pool pool_of(const char* who, const Tensor& k, const Tensor& v, bool writ
   p.v = v.data_ptr();
   p.page_stride = st[0]; p.slot_stride = st[1]; p.head_stride = st[2];
   p.n_pages = (int)sh[0]; p.page = (int)sh[1]; p.heads = (int)sh[2]; p.head_dim = (int)sh[3];
+  NEED(!written || !folds(box_of(p, p.k)), "heads of the cache overlap each other");
+  NEED(!written || !meet(box_of(p, p.k), box_of(p, p.v)), "k and v overlap");
   return p;
 }
 
@@ -207,6 +289,11 @@ PyObject* kv_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
            (long long)(hd / 2));
       d.cos_tab = (const float*)cs->data_ptr(); d.sin_tab = (const float*)sn->data_ptr(); d.rope_rows = (int)cs->size(0);
     }
+    const Box to[3] = {box_of(d.pool, d.pool.k), box_of(d.pool, d.pool.v), Box(d.q_out, 2 * heads * hd).axis(q ? d.rows : 0, 2 * d.ldq)};
+    for (int i = 0; i < 3; ++i) {
+      for (const Tensor* t : {&table, &pos, seq, cs, sn}) NEED(!t || !meet(to[i], box_of(*t)), "%s overlaps the table, positions, sequences or rotation", i < 2 ? "the cache" : "q_out");
+      if (i < 2) NEED(!meet(to[i], box_of(x, d.rows, (heads + 2 * hkv) * hd)) && !meet(to[i], to[2]), "the cache overlaps qkv or q_out");
+    }
     const slx_stream_t s = stream_of(who, {&qkv, &k, &v, &table, &pos, q, cs, sn, seq});
     check(lib.kv_append(&d, s), "slx_kv_append");
     return none();
@@ -275,6 +362,13 @@ PyObject* prefix_attn(PyObject*, PyObject* const* a, Py_ssize_t n) {
         return !rows || (char*)(d.lse + rows * heads) <= (char*)r.p || (char*)r.p + 2 * ((rows - 1) * r.ld + cols) <= (char*)d.lse;
       };
       NEED(apart(x) && apart(o), "lse overlaps q or out");
+    }
+    const Box to[2] = {box_of(o, rows, cols), Box(d.lse, lse ? 4 * rows * heads : 0)};
+    for (const Box& y : to) {
+      for (const slx_kv_pool* p : {&d.own_pool, &d.prefix_pool}) {
+        if (p->k) NEED(!meet(y, box_of(*p, p->k)) && !meet(y, box_of(*p, p->v)), "%s overlaps a cache", &y == to ? "out" : "lse");
+      }
+      for (const Tensor* t : {(const Tensor*)&otab, (const Tensor*)&olen, ptab, plen}) NEED(!t || !meet(y, box_of(*t)), "%s overlaps a table or lengths", &y == to ? "out" : "lse");
     }
     const slx_stream_t s = stream_of(who, {&q, &ok, &ov, &otab, &olen, &out, pk, pv, ptab, plen, lse});
     if (ot.n) {

@@ -92,7 +92,7 @@ def kv_append(qkv, k, v, table, pos, q_out=None, *, n_heads, cos=None, sin=None,
 
     A row with pos < 0, or one that names no slot (behind the table or the rotation's rows, a sequence or page that there
     is not), is padding: nothing of it is written. Two rows of one call must not name the same slot. k and v are apart from
-    each other and from qkv and q_out."""
+    each other and from qkv and q_out, and what is written from what is read beside; columns or slots of one buffer may be."""
     (_native or _bind()).kv_append(qkv, k, v, table, pos, q_out, n_heads, cos, sin, seq, rows_per_seq)
 
 
@@ -104,7 +104,8 @@ def prefix_attn(q, out=None, *, own, prefix=None, n_heads, n_q=1, scale=None, ma
     gives zeros. scale > 0: 1 / sqrt(head size) by default. max_own, max_prefix: bounds of the lengths where they are known
     to be lower than the tables' columns (longer ones are cut to them), at most 2^30; the split of the work goes by them.
     Keys on a page number outside the cache are masked. lse: optional f32 [N * n_q, n_heads], natural log of the softmax
-    sum (-inf without keys). Returns out (bf16, like q); it may be q itself."""
+    sum (-inf without keys). Returns out (bf16, like q); it may be q itself, or other columns of its rows. out and lse are apart from the
+    caches, tables and lengths."""
     ok, ov, otab, olen = own
     pk, pv, ptab, plen = prefix if prefix is not None else (None, None, None, None)
     return (_native or _bind()).prefix_attn(q, out, ok, ov, otab, olen, pk, pv, ptab, plen, n_heads, n_q, scale, max_own, max_prefix, lse)
