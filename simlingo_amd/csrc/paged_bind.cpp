@@ -477,14 +477,6 @@ PyObject* beam_select(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
-// bytes [from, to) that a view touches
-void span_of(const Tensor& t, uintptr_t* from, uintptr_t* to) {
-  int64_t last = 0;
-  for (int64_t i = 0; i < t.dim(); ++i) last += (t.size(i) - 1) * t.stride(i);
-  *from = (uintptr_t)t.data_ptr();
-  *to = *from + (uintptr_t)((last + 1) * (int64_t)t.element_size());
-}
-
 // (x, parent, dim, out) -> out
 PyObject* beam_reorder(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded("beam_reorder", n, 4, [&]() -> PyObject* {
@@ -519,19 +511,21 @@ PyObject* beam_reorder(PyObject*, PyObject* const* a, Py_ssize_t n) {
       }
       NEED(out.stride(dim) || b * w == 1, "out must not be expanded");
       NEED(m[0] <= kIntMax && m[1] <= kIntMax, "dimensions too long");
-      if (x.data_ptr() != out.data_ptr() || x.strides() != out.strides()) {
-        uintptr_t x0, x1, o0, o1;
-        span_of(x, &x0, &x1);
-        span_of(out, &o0, &o1);
-        NEED(x1 <= o0 || o1 <= x0, "out overlaps x");
-      }
+      const auto box = [&](const Tensor& u, const int64_t* st) {
+        return Box(u.data_ptr(), run * es).axis(m[1], st[1] * es).axis(m[0], st[0] * es).axis(b * w, u.stride(dim) * es);
+      };
+      const bool same = x.data_ptr() == out.data_ptr() && s[0] == t[0] && s[1] == t[1] && (x.stride(dim) == out.stride(dim) || b * w == 1);
+      NEED(same || !meet(box(x, s), box(out, t)), "out overlaps x");
+      NEED(!folds(box(out, t)), "rows of out overlap each other");
+      NEED(!meet(box(out, t), box_of(parent)), "out overlaps parent");
     }
     const slx_stream_t st = stream_of(who, {&x, &out, &parent});
     if (x.numel()) {
       slx_beam_reorder_desc d{};
       d.src = x.data_ptr(); d.dst = out.data_ptr();
-      d.s0 = s[1] * es; d.s1 = s[0] * es; d.src_row = x.stride(dim) * es;
-      d.d0 = t[1] * es; d.d1 = t[0] * es; d.dst_row = out.stride(dim) * es;
+      const bool one = b * w == 1;  // its stride says nothing
+      d.s0 = s[1] * es; d.s1 = s[0] * es; d.src_row = one ? 0 : x.stride(dim) * es;
+      d.d0 = t[1] * es; d.d1 = t[0] * es; d.dst_row = one ? 0 : out.stride(dim) * es;
       d.row_bytes = run * es;
       d.n0 = (int)m[1]; d.n1 = (int)m[0]; d.batch = (int)b; d.width = (int)w;
       d.parent = (const int*)parent.data_ptr();

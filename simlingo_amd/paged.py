@@ -126,5 +126,5 @@ def beam_reorder(x, parent, *, dim=0, out=None):
     """out[..., b * W + w, ...] = x[..., b * W + parent[b, w], ...] along `dim` of a state of any type; parent int32 [batch, W]
     as beam_select returns it. Without out (or with x itself) in place, for any parents. The other dimensions may be
     strided as long as they make at most two runs of rows. A parent outside 0 .. W - 1 stands for w itself.
-    Returns out."""
+    out is apart from x (or x itself) and from parent. Returns out."""
     return (_native or _bind()).beam_reorder(x, parent, dim, out)

@@ -141,3 +141,31 @@ def test_tables_apart_from_what_is_written():
     k, v = pool[:4096].view(4, 8, 2, 64), pool[4096:].view(4, 8, 2, 64)
     for at in (0, 2047, 2048, 4092):
         taken(lambda: PG.kv_append(**append_args(k=k, v=v, pos=ints(at, 3))), False, "the cache overlaps the table")
+
+
+def test_reorder_out_apart():
+    """Rows of out that overlap each other, or the parents, are refused; other columns or rows of x's own buffer are not."""
+    parent = torch.zeros(2, 2, dtype=I32)
+    b = torch.zeros(256)
+    x = torch.zeros(4, 6)
+    for st in ((5, 1), (6, 1), (1, 4), (1, 3), (2, 4), (2, 8), (2, 9), (4, 17), (5, 21), (4, 6), (3, 5)):
+        out = b.as_strided((4, 6), st)
+        ok = len(set(touched(out))) == 24
+        taken(lambda: PG.beam_reorder(x, parent, out=out), ok, "rows of out overlap")
+        taken(lambda: PG.beam_reorder(out, parent), ok, "rows of out overlap")
+    buf = torch.zeros(8, 20)
+    for out, ok in ((buf[:4, 6:12], True), (buf[4:, :6], True), (buf[:4, 5:11], False), (buf[1:5, :6], False), (buf[1:5, 6:12], True), (buf[::2, :6], False), (buf[:4, :6], True)):
+        taken(lambda: PG.beam_reorder(buf[:4, :6], parent, out=out), ok, "out overlaps x")
+    taken(lambda: PG.beam_reorder(buf[::2, :6], parent, out=buf[1::2, :6]), True, "")
+    taken(lambda: PG.beam_reorder(buf[:, :6], torch.zeros(4, 2, dtype=I32), out=buf[:, 6:18:2]), True, "")
+    ints = torch.zeros(4, 3, dtype=I32)
+    ints4 = ints.view(-1)[2:6].view(2, 2)
+    taken(lambda: PG.beam_reorder(ints, ints4), False, "out overlaps parent")
+    taken(lambda: PG.beam_reorder(ints[:, :1], ints.view(-1)[1:3].view(1, 2).expand(2, 2).contiguous()), True, "")
+    taken(lambda: PG.beam_reorder(ints4.view(4, 1), ints4, out=torch.zeros(4, 1, dtype=I32)), True, "")
+
+
+def test_one_row_in_place_whatever_its_stride():
+    """A single row's stride says nothing: x and out of one memory are in place."""
+    b = torch.zeros(64)
+    taken(lambda: PG.beam_reorder(b.as_strided((1, 8), (3, 1)), torch.zeros(1, 1, dtype=I32), out=b.as_strided((1, 8), (8, 1))), True, "")
