@@ -550,7 +550,7 @@ typedef struct slx_prefix_attn_desc {
   float* ws; int64_t ws_floats;              /* slx_prefix_attn_ws_floats(d); one call at a time                       */
 } slx_prefix_attn_desc;
 /* token t of a sequence's n_q attends the plen[group] keys of its group's prefix and its own keys j <= olen - n_q + t; a
- * row without any key gives zeros.                                                                                   */
+ * row without any key gives zeros. out and lse overlap nothing that is read (but out q itself, or other columns of its rows). */
 int slx_prefix_attn(const slx_prefix_attn_desc* d, slx_stream_t s);
 int64_t slx_prefix_attn_ws_floats(const slx_prefix_attn_desc* d); /* < 0: bad argument                                 */
 
@@ -562,7 +562,7 @@ int64_t slx_prefix_attn_ws_floats(const slx_prefix_attn_desc* d); /* < 0: bad ar
  * finished when k == width; the outputs overlap nothing else.                                                          */
 typedef struct slx_beam_select_desc {
   const void* logits; int64_t ldx; int logits_bf16;  /* [batch * width][vocab] f32 or bf16, any alignment of the type  */
-  int batch, width, vocab, k;                /* width, k <= 64; vocab <= 262144                                        */
+  int batch, width, vocab, k;                /* width, k <= 64; vocab <= 262144; batch * width * ceil(vocab / 4096) < 2^24 */
   const float* score;                        /* [batch * width]; not finite: the beam is out                           */
   const unsigned char* finished; int pad;    /* optional [batch * width]                                               */
   float* score_out; int* parent; int* token; /* [batch][k]                                                             */

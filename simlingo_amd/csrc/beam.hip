@@ -497,18 +497,18 @@ static void reorder_launch(const ReorderArgs& a, hipStream_t st) {
   else hipLaunchKernelGGL((beam_reorder_kernel<T, 64>), grid, dim3(256), 0, st, a);
 }
 
+static int chunks_of(const slx_beam_select_desc* d) { return (d->vocab + kSelChunk - 1) / kSelChunk; }
+
 static int check_select(const slx_beam_select_desc* d) {
   SLX_CHECK_ARG(d != nullptr, "slx_beam_select: null desc");
-  SLX_CHECK_ARG(d->batch >= 0 && d->width > 0 && d->width <= kSelMaxW && (int64_t)d->batch * d->width * kSelMaxChunks < 2147483648L,
-                "slx_beam_select: 0 <= batch, 0 < width <= %d, batch * width < 2^25", kSelMaxW);
+  SLX_CHECK_ARG(d->batch >= 0 && d->width > 0 && d->width <= kSelMaxW, "slx_beam_select: 0 <= batch, 0 < width <= %d", kSelMaxW);
   SLX_CHECK_ARG(d->vocab > 0 && d->vocab <= kSelChunk * kSelMaxChunks, "slx_beam_select: 0 < vocab <= %d", kSelChunk * kSelMaxChunks);
+  SLX_CHECK_ARG(launch_fits((int64_t)d->batch * d->width * chunks_of(d), 256), "slx_beam_select: batch * width rows of %d chunks of %d must be < 2^24 chunks", chunks_of(d), kSelChunk);
   SLX_CHECK_ARG(d->k > 0 && d->k <= kSelMaxK && d->k <= (int64_t)d->width * d->vocab, "slx_beam_select: 0 < k <= %d and <= width * vocab", kSelMaxK);
   SLX_CHECK_ARG(d->ldx >= d->vocab, "slx_beam_select: ldx >= vocab");
   SLX_CHECK_ARG(!d->finished || (d->pad >= 0 && d->pad < d->vocab), "slx_beam_select: pad outside the vocabulary");
   return 0;
 }
-
-static int chunks_of(const slx_beam_select_desc* d) { return (d->vocab + kSelChunk - 1) / kSelChunk; }
 
 }  // namespace slx
 
@@ -569,7 +569,7 @@ int slx_beam_reorder(const slx_beam_reorder_desc* d, slx_stream_t s) {
                      (uint64_t)d->src_row | (uint64_t)d->d0 | (uint64_t)d->d1 | (uint64_t)d->dst_row | (uint64_t)d->row_bytes;
   const int w = (u & 15) == 0 ? 16 : (u & 3) == 0 ? 4 : (u & 1) == 0 ? 2 : 1;
   a.cols = d->row_bytes / w;
-  SLX_CHECK_ARG((a.cols + 255) / 256 < 2147483648L, "slx_beam_reorder: rows too long");
+  SLX_CHECK_ARG(launch_fits((a.cols + 255) / 256, 256), "slx_beam_reorder: rows too long");
   SLX_CHECK_ARG((double)d->n0 * d->n1 * d->batch < 2147483648.0, "slx_beam_reorder: n0 * n1 * batch must be < 2^31");
   if (w == 16) reorder_launch<u32x4>(a, (hipStream_t)s);
   else if (w == 4) reorder_launch<unsigned>(a, (hipStream_t)s);

@@ -47,6 +47,9 @@ int det_reduce(const float* part, int nparts, long n, long stride, float* out, i
     }                                                                       \
   } while (0)
 
+// a launch holds fewer than 2^32 threads along an axis
+inline bool launch_fits(long blocks, long threads) { return blocks < (1L << 32) / threads; }
+
 __device__ __forceinline__ float bf2f(bf16 x) { return (float)x; }
 __device__ __forceinline__ bf16 f2bf(float x) { return (bf16)x; }
 

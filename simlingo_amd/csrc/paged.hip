@@ -1084,16 +1084,18 @@ static bool launch_attn(const PAttnPlan& p, dim3 grid, hipStream_t st, const PAt
 #undef SLX_PA
   return false;
 }
-template <int D, int PG, int B>
-static void launch_join(hipStream_t st, const PAttnArgs& a) {
-  constexpr int RPB = 256 / (D / 4 * PG);
-  hipLaunchKernelGGL((prefix_attn_join_kernel<D, PG, B>), dim3((unsigned)((a.R + RPB - 1) / RPB)), dim3(256), 0, st, a);
+static int join_groups(int D, int parts) { return parts <= 8 ? 1 : parts <= 16 ? 4 : 1024 / D; }
+static long join_blocks(int D, int parts, long R) {
+  const int rpb = 256 / (D / 4 * join_groups(D, parts));
+  return (R + rpb - 1) / rpb;
 }
 template <int D>
 static void join_parts(int parts, hipStream_t st, const PAttnArgs& a) {
-  if (parts <= 8) launch_join<D, 1, 8>(st, a);
-  else if (parts <= 16) launch_join<D, 4, 4>(st, a);
-  else launch_join<D, 1024 / D, 4>(st, a);
+  const dim3 grid((unsigned)join_blocks(D, parts, a.R));
+  const int groups = join_groups(D, parts);
+  if (groups == 1) hipLaunchKernelGGL((prefix_attn_join_kernel<D, 1, 8>), grid, dim3(256), 0, st, a);
+  else if (groups == 4) hipLaunchKernelGGL((prefix_attn_join_kernel<D, 4, 4>), grid, dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((prefix_attn_join_kernel<D, 1024 / D, 4>), grid, dim3(256), 0, st, a);
 }
 
 }  // namespace slx
@@ -1123,7 +1125,7 @@ int slx_kv_append(const slx_kv_append_desc* d, slx_stream_t s) {
   SLX_CHECK_ARG(items < (1 << 24), "slx_kv_append: too many heads");
   a.rows_per_block = items >= 256 ? 1 : (int)(256 / items);
   const long blocks = (d->rows + a.rows_per_block - 1) / a.rows_per_block;
-  SLX_CHECK_ARG(blocks < 2147483648L, "slx_kv_append: too many rows");
+  SLX_CHECK_ARG(launch_fits(blocks, 256), "slx_kv_append: too many rows");
   if (d->pool.head_dim == 64) hipLaunchKernelGGL(kv_append_kernel<64>, dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)s, a);
   else hipLaunchKernelGGL(kv_append_kernel<128>, dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)s, a);
   SLX_LAUNCH_CHECK("slx_kv_append");
@@ -1166,7 +1168,8 @@ int slx_prefix_attn(const slx_prefix_attn_desc* d, slx_stream_t s) {
   SLX_CHECK_ARG(need == 0 || (d->ws && ((uintptr_t)d->ws & 15) == 0 && d->ws_floats >= need),
                 "slx_prefix_attn: needs a 16-B aligned workspace of %lld floats", (long long)need);
   const long blocks = n_pre + (long)d->groups * d->width * Hkv * p.mto * p.nso;
-  SLX_CHECK_ARG(blocks < 2147483648L, "slx_prefix_attn: too many rows");
+  SLX_CHECK_ARG(launch_fits(blocks, p.whole ? 64 * p.whole : 256) && (a.direct || launch_fits(join_blocks(D, p.nsp + p.nso, a.R), 256)),
+                "slx_prefix_attn: too many rows");
   a.n_pre = (unsigned)n_pre;
   const bool known = D == 64 ? launch_attn<64>(p, dim3((unsigned)blocks), (hipStream_t)s, a)
                              : launch_attn<128>(p, dim3((unsigned)blocks), (hipStream_t)s, a);

@@ -113,7 +113,8 @@ def prefix_attn(q, out=None, *, own, prefix=None, n_heads, n_q=1, scale=None, ma
 
 def beam_select(logits, scores, *, width, k=None, finished=None, pad_id=0, eos_id=None, out=None, finished_out=None):
     """The k (default: width) best continuations of each batch entry by scores[b, w] + log_softmax(logits[b, w])[t], in
-    descending order, ties to the lowest w * V + t. logits [batch * width, V] f32 or bf16, rows contiguous; scores
+    descending order, ties to the lowest w * V + t. logits [batch * width, V] f32 or bf16, rows contiguous, V up to MAX_VOCAB
+    and fewer than 2^24 pieces of 4096 in all the rows; width, k up to MAX_WIDTH, MAX_K; scores
     [batch * width] f32 (not finite: the beam is out). finished [batch * width] bool / uint8: such a row offers `pad_id` alone,
     its score unchanged. The scores of a row that is out, is -inf throughout or holds a NaN or +inf count as -inf.
 
