@@ -1050,7 +1050,7 @@ static int check_attn(const slx_prefix_attn_desc* d, int* capp, int* capo) {
   // row / gq is a multiplication (exact while row * gq < 2^32)
   SLX_CHECK_ARG((double)d->width * d->n_q * (d->Hq / d->own_pool.heads) * (d->Hq / d->own_pool.heads) < 4294967296.0,
                 "slx_prefix_attn: too many rows");
-  SLX_CHECK_ARG(d->scale > 0.0f && d->scale < INFINITY, "slx_prefix_attn: scale must be positive");
+  SLX_CHECK_ARG(d->scale > 0.0f && d->scale * 1.44269504088896341f < INFINITY, "slx_prefix_attn: scale must be positive and, times log2(e), finite");
   SLX_CHECK_ARG(d->max_own >= 0 && d->ocols > 0 && d->ldot >= d->ocols, "slx_prefix_attn: max_own >= 0, ldot >= ocols > 0");
   *capo = cap_of(d->max_own, d->ocols, d->own_pool.page);
   *capp = 0;

@@ -319,8 +319,8 @@ PyObject* prefix_attn(PyObject*, PyObject* const* a, Py_ssize_t n) {
     d.n_q = (int)n_q;
     double scale = a[12] == Py_None ? 1.0 / std::sqrt((double)hd) : PyFloat_AsDouble(a[12]);
     if (PyErr_Occurred()) throw Raised();
-    NEED(scale > 0 && scale < INFINITY, "scale must be positive");
     d.scale = (float)scale;
+    NEED(d.scale > 0 && d.scale * 1.44269504088896341f < INFINITY, "scale must be positive and, times log2(e), finite in 32 bits");
     const int64_t rows = (int64_t)ot.n * n_q, cols = heads * hd;
     const Rows x = rows_of(who, "q", q, rows, cols);
     d.q = x.p; d.ldq = x.ld;

@@ -53,3 +53,12 @@ def test_launches_of_2_to_the_32_threads():
         r = {**reorder, "src_row": size << 33, "dst_row": size << 33}
         assert launched("slx_beam_reorder", PG.BeamReorderDesc(**{**r, "row_bytes": size * ((1 << 32) - 256 - (size < 16))}))
         assert refused("slx_beam_reorder", PG.BeamReorderDesc(**{**r, "row_bytes": size * ((1 << 32) - 255 + 2 * (size < 16))}), b"too long")
+
+
+@pytest.mark.parametrize("scale,ok", ((1e-50, False), (1e-46, False), (1e-44, True), (0.125, True), (2e38, True), (2.4e38, False), (3e38, False), (1e39, False)))
+def test_scales(scale, ok):
+    """The scale and its product with log2(e) are held in 32 bits: one that becomes 0 or infinite there is refused."""
+    with pytest.raises(RuntimeError if ok else ValueError, match="no CPU" if ok else "scale"):
+        PG.prefix_attn(**attn_args(scale=scale))
+    d = PG.PrefixAttnDesc(own_pool=POOL, q=4096, ldq=256, out=4096, ldo=256, otab=4096, ldot=2, olen=4096, max_own=16, ocols=2, groups=1, width=2, n_q=1, Hq=4, scale=scale)
+    assert launched("slx_prefix_attn", d) if ok else refused("slx_prefix_attn", d, b"scale")
