@@ -56,9 +56,14 @@ void check(int64_t rc, const char* name) {
 }
 
 // ---- arguments -------------------------------------------------------------------------------------------------
-const Tensor& tensor(PyObject* o, const char* who, const char* name) {
+const Tensor& any_tensor(PyObject* o, const char* who, const char* name) {
   if (!THPVariable_Check(o)) fail(PyExc_TypeError, who, "%s must be a tensor", name);
   return THPVariable_Unpack(o);
+}
+const Tensor& tensor(PyObject* o, const char* who, const char* name) {
+  const Tensor& t = any_tensor(o, who, name);
+  NEED(!t.is_neg(), "%s is a lazily negated view (resolve_neg)", name);  // none of the types taken here can be conjugated
+  return t;
 }
 const Tensor* maybe(PyObject* o, const char* who, const char* name) { return o == Py_None ? nullptr : &tensor(o, who, name); }
 int64_t integer(PyObject* o, const char* who, const char* name) {
@@ -481,9 +486,10 @@ PyObject* beam_select(PyObject*, PyObject* const* a, Py_ssize_t n) {
 PyObject* beam_reorder(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded("beam_reorder", n, 4, [&]() -> PyObject* {
     const char* who = "beam_reorder";
-    const Tensor &x = tensor(a[0], who, "x"), &parent = tensor(a[1], who, "parent");
+    const Tensor &x = any_tensor(a[0], who, "x"), &parent = tensor(a[1], who, "parent");
     PyObject* back = a[3] == Py_None ? a[0] : a[3];
-    const Tensor& out = tensor(back, who, "out");
+    const Tensor& out = any_tensor(back, who, "out");
+    NEED(x.is_neg() == out.is_neg() && x.is_conj() == out.is_conj(), "x or out alone is lazily negated or conjugated");
     NEED(parent.scalar_type() == at::kInt && parent.dim() == 2 && parent.is_contiguous(), "parent must be contiguous int32 [batch, W]");
     const int64_t b = parent.size(0), w = parent.size(1), nd = x.dim();
     int64_t dim = integer(a[2], who, "dim");

@@ -169,3 +169,22 @@ def test_one_row_in_place_whatever_its_stride():
     """A single row's stride says nothing: x and out of one memory are in place."""
     b = torch.zeros(64)
     taken(lambda: PG.beam_reorder(b.as_strided((1, 8), (3, 1)), torch.zeros(1, 1, dtype=I32), out=b.as_strided((1, 8), (8, 1))), True, "")
+
+
+def test_lazily_negated_views():
+    """The memory of a view that torch negates or conjugates on reading holds other numbers: refused, but where it moves as it is."""
+    z = torch.zeros(4, 9, dtype=torch.complex64)
+    neg = z.conj().imag  # the imaginary part with its sign to be turned
+    parent = torch.zeros(2, 2, dtype=I32)
+    assert neg.is_neg() and z.conj().is_conj()
+    logits = torch.zeros(8, 18).view(4, 2, 18)[:, 0, :9]
+    taken(lambda: PG.beam_select(logits, torch.zeros(4), width=2), True, "")
+    taken(lambda: PG.beam_select(torch._neg_view(logits), torch.zeros(4), width=2), False, "negated")
+    taken(lambda: PG.beam_select(logits, torch._neg_view(torch.zeros(4)), width=2), False, "negated")
+    taken(lambda: PG.prefix_attn(**attn_args(q=torch._neg_view(torch.zeros(4, 256, dtype=BF16)))), False, "negated")
+    taken(lambda: PG.prefix_attn(**attn_args(out=torch._neg_view(torch.zeros(4, 256, dtype=BF16)))), False, "negated")
+    taken(lambda: PG.kv_append(**append_args(cos=torch._neg_view(torch.zeros(16, 32)))), False, "negated")
+    for x in (neg, z.conj()):
+        taken(lambda: PG.beam_reorder(x, parent), True, "")
+        taken(lambda: PG.beam_reorder(x, parent, out=torch.empty(4, 9, dtype=x.dtype)), False, "negated")
+    taken(lambda: PG.beam_reorder(z.conj(), parent, out=torch.empty(4, 9, dtype=z.dtype).conj()), True, "")
