@@ -308,9 +308,9 @@ class BeamDecoder(GreedyDecoder):
     keys are a table of single slots, so a step reorders the table and no keys (slx_beam_reorder). One step is the batched
     kernels over num_beams rows, slx_kv_append and slx_prefix_attn per layer, then slx_beam_select over the whole vocabulary.
     Stands in for LLM.greedy_sample (simlingo_training/models/language_model/llm.py:178-250) wherever a decoder is taken
-    (infer_example); num_beams 1 is that loop."""
+    (infer_example); num_beams 1 is that loop. It takes GreedyDecoder's arguments; its steps run eagerly, whatever use_graph says."""
 
-    def __init__(self, engine, num_beams: int = 4, **kw):
+    def __init__(self, engine, num_beams: int = 4, *, use_graph: bool = False, **kw):
         if not 1 <= num_beams <= PG.MAX_WIDTH:
             raise ValueError(f"num_beams must be 1 .. {PG.MAX_WIDTH}")
         super().__init__(engine, use_graph=False, **kw)
@@ -371,6 +371,8 @@ class BeamDecoder(GreedyDecoder):
         if W > cfg.vocab:
             raise ValueError(f"{W} beams over {cfg.vocab} tokens")
         pad = self.eos if 0 <= self.eos < cfg.vocab else 0
+        ev = [torch.cuda.Event(enable_timing=True) for _ in range(3)]
+        ev[0].record()
         Xl = self._llm_batched(prefix, self.cache)
         self._plen.fill_(S0)
         table, pos, lens = self._slots.clone(), torch.zeros(W, dtype=torch.int32, device=dev), torch.ones(W, dtype=torch.int32, device=dev)
@@ -380,6 +382,8 @@ class BeamDecoder(GreedyDecoder):
                                           finished_out=done)
         history[:, 0] = token[0]
         parent = torch.empty(1, W, dtype=torch.int32, device=dev)
+        ev[1].record()
+        done_steps = 0
         for j in range(n_max - 1):
             if j % self.check_every == 0 and bool(done.all()):
                 break
@@ -391,7 +395,12 @@ class BeamDecoder(GreedyDecoder):
             history[:, j + 1] = token[0]
             pos += 1
             lens += 1
-        return history.long().cpu(), scores.view(-1).cpu()
+            done_steps += 1
+        ev[2].record()
+        ids, scores = history.long().cpu(), scores.view(-1).cpu()
+        self.last_timing = {"prefill_ms": ev[0].elapsed_time(ev[1]), "decode_ms": ev[1].elapsed_time(ev[2]),
+                            "decode_steps": done_steps}
+        return ids, scores
 
     def generate(self, prefix: torch.Tensor, max_new_tokens: int | None = None) -> torch.Tensor:
         """The best beam's ids (int64, CPU), up to and with the end token if it was produced."""
