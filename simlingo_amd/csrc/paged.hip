@@ -258,8 +258,15 @@ __device__ __forceinline__ void mask_scores(f32x4 (&s)[NQ][2], unsigned dead, co
 }
 
 // Scores of T tiles to probabilities, with the state rescaled where a row's maximum has moved.
+//
+// A probability goes to the MFMA as two bf16 terms, p (1 + 2^-17) = hi + lo: hi its upper 16 bits as they are (so hi <= p), lo the rest,
+// rounded (half a step of at most p 2^-7: 2^-15 p). One bf16 term alone is off by 2^-8 p and made the output's error up to 1.4 times
+// that of its own rounding. The factor cancels in o / l; it keeps lo above 0, so that an infinite V keeps its sign in both products
+// (0 * inf would be NaN). It costs a second product with V: 19.5 -> 22.1 us for 2 x 16 sequences on 32771 keys, 14.8 -> 16.2 for
+// 12 x 77 tokens on 640, 45 -> 54 for 64 x 77; next to nothing where memory or latency bounds (57.8 -> 58.7 with the join for 32 on 16411
+// keys of 8 heads of 128).
 template <int D, int NQ, int T>
-__device__ __forceinline__ void softmax_step(const f32x4 (&s)[T][NQ][2], float c, State<D, NQ>& st, bf16x8 (&pb)[T][NQ]) {
+__device__ __forceinline__ void softmax_step(const f32x4 (&s)[T][NQ][2], float c, State<D, NQ>& st, bf16x8 (&ph)[T][NQ], bf16x8 (&pl)[T][NQ]) {
 #pragma unroll
   for (int n = 0; n < NQ; ++n) {
     float mx = s[0][n][0][0];
@@ -278,12 +285,22 @@ __device__ __forceinline__ void softmax_step(const f32x4 (&s)[T][NQ][2], float c
       for (int e = 0; e < D / 16; ++e) st.o[n][e] *= r;
     }
     const float mu = st.m[n] == -INFINITY ? 0.f : st.m[n];
-    // P in bf16 for the MFMA (half a step, 2^-8 of each term at most, as the output itself is rounded); l sums the same
-    // rounded values, so what is left is the terms' own scatter
 #pragma unroll
     for (int u = 0; u < T; ++u)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) pb[u][n][j] = (bf16)__builtin_amdgcn_exp2f(__builtin_fmaf(s[u][n][j >> 2][j & 3], c, -mu));
+      for (int j = 0; j < 8; j += 2) {
+        unsigned h[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][n][j >> 2][(j & 3) + i], c, -mu));
+          h[i] = __float_as_uint(p) & 0xFFFF0000u;
+          pl[u][n][j + i] = (bf16)__builtin_fmaf(p, 1.0f + 0x1p-17f, -__uint_as_float(h[i]));
+        }
+        union { unsigned u; bf16x2 b; } x;
+        x.u = __builtin_amdgcn_perm(h[1], h[0], 0x07060302u);
+        ph[u][n][j] = x.b[0];
+        ph[u][n][j + 1] = x.b[1];
+      }
   }
 }
 
@@ -316,19 +333,29 @@ __device__ __forceinline__ bool clean_v(unsigned (&vr)[8][D / 32], unsigned dead
 }
 
 template <int D, int NQ>
-__device__ __forceinline__ void output_step(const unsigned (&vr)[8][D / 32], const bf16x8 (&pb)[NQ], State<D, NQ>& st) {
+__device__ __forceinline__ void output_step(const unsigned (&vr)[8][D / 32], const bf16x8 (&ph)[NQ], const bf16x8 (&pl)[NQ], State<D, NQ>& st) {
   union { unsigned u[4]; bf16x8 b; } vt;
   vt.u[0] = vt.u[1] = vt.u[2] = vt.u[3] = 0x3F803F80u;  // ones
 #pragma unroll
-  for (int n = 0; n < NQ; ++n) st.l[n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vt.b, pb[n], st.l[n], 0, 0, 0);
+  for (int n = 0; n < NQ; ++n) {
+    st.l[n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vt.b, ph[n], st.l[n], 0, 0, 0);
+    st.l[n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vt.b, pl[n], st.l[n], 0, 0, 0);
+  }
 #pragma unroll
   for (int e = 0; e < D / 16; ++e) {
 #pragma unroll
     for (int p = 0; p < 4; ++p)
       vt.u[p] = __builtin_amdgcn_perm(vr[2 * p + 1][e >> 1], vr[2 * p][e >> 1], (e & 1) ? 0x07060302u : 0x05040100u);
 #pragma unroll
-    for (int n = 0; n < NQ; ++n) st.o[n][e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vt.b, pb[n], st.o[n][e], 0, 0, 0);
+    for (int n = 0; n < NQ; ++n) {
+      st.o[n][e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vt.b, ph[n], st.o[n][e], 0, 0, 0);
+      st.o[n][e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vt.b, pl[n], st.o[n][e], 0, 0, 0);
+    }
   }
+}
+
+__device__ __forceinline__ float natural_lse(float m, float l) {  // l sums p (1 + 2^-17)
+  return m == -INFINITY ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f - 0x1p-17f;
 }
 
 // A row's (m, l, o) to the output or the workspace; a lane has d = (D/4) grp + (D/16) i + e of row r.
@@ -347,7 +374,7 @@ __device__ __forceinline__ void store_row(const PAttnArgs& a, const Item& w, int
       for (int j = 0; j < 8; ++j) y[j] = (bf16)(o[(8 * b + j) % NE][(8 * b + j) / NE] * inv);
       *reinterpret_cast<bf16x8*>(op + 8 * b) = y;
     }
-    if (a.lse && grp == 0) a.lse[row] = m == -INFINITY ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
+    if (a.lse && grp == 0) a.lse[row] = natural_lse(m, l);
   } else {
     float* op = a.ws + ((long)w.part * a.R + row) * D + (D / 4) * grp;
 #pragma unroll
@@ -476,7 +503,7 @@ __device__ __forceinline__ void attn_direct(const PAttnArgs& a, Item w, char* sm
   }
   for (; k0 < ke; k0 += 128) {
     f32x4 s[1][NQ][2];
-    bf16x8 pb[1][NQ];
+    bf16x8 ph[1][NQ], pl[1][NQ];
     scores<D, NQ>(kf, qf, s[0]);
     const bool edge = k0 + 32 > free_end || __any(bad != 0);
     unsigned dead = bad;
@@ -491,9 +518,9 @@ __device__ __forceinline__ void attn_direct(const PAttnArgs& a, Item w, char* sm
       load_k(k0 + 128);
       entries_k(k0 + 256);
     }
-    softmax_step<D, NQ, 1>(s, a.c, st, pb);
+    softmax_step<D, NQ, 1>(s, a.c, st, ph, pl);
     if (edge) odd = clean_v<D>(vr, dead, w.causal && a.Tq > 1 && k0 + 32 > free_end) || odd;
-    output_step<D, NQ>(vr, pb[0], st);
+    output_step<D, NQ>(vr, ph[0], pl[0], st);
     if (more) {
       load_v(k0 + 128);
       entries_v(k0 + 256);
@@ -673,7 +700,7 @@ __device__ __forceinline__ bool stream_keys(const PAttnArgs& a, const Item& w, i
     const int u0 = wave / S::RWV * UW;
     if (k0 + 32 * u0 >= kw) continue;
     f32x4 s[UW][NQ][2];
-    bf16x8 pb[UW][NQ];
+    bf16x8 ph[UW][NQ], pl[UW][NQ];
     unsigned vr[UW][8][NE / 2], bads[UW], dead[UW];
 #pragma unroll
     for (int v = 0; v < UW; ++v) {
@@ -719,13 +746,13 @@ __device__ __forceinline__ bool stream_keys(const PAttnArgs& a, const Item& w, i
         mask_scores<NQ>(s[v], dead[v], lim, kv);
       }
     }
-    softmax_step<D, NQ, UW>(s, a.c, st, pb);
+    softmax_step<D, NQ, UW>(s, a.c, st, ph, pl);
     if (edge) {
 #pragma unroll
       for (int v = 0; v < UW; ++v) odd = clean_v<D>(vr[v], dead[v], w.causal && a.Tq > 1 && k0 + 32 * (u0 + v + 1) > free_end) || odd;
     }
 #pragma unroll
-    for (int v = 0; v < UW; ++v) output_step<D, NQ>(vr[v], pb[v], st);
+    for (int v = 0; v < UW; ++v) output_step<D, NQ>(vr[v], ph[v], pl[v], st);
   }
   return odd;
 }
@@ -969,7 +996,7 @@ __global__ __launch_bounds__(256) void prefix_attn_join_kernel(PAttnArgs a) {
 #pragma unroll
   for (int j = 0; j < 4; ++j) y[j] = (bf16)(o[j] * inv);
   *reinterpret_cast<bf16x4*>(a.out + tok * a.ldo + (row - tok * a.Hq) * D + 4 * d4) = y;
-  if (a.lse && d4 == 0) a.lse[row] = m == -INFINITY ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
+  if (a.lse && d4 == 0) a.lse[row] = natural_lse(m, l);
 }
 
 // Row tiles and key ranges of a call: a rule on sizes, page sizes and the host's bounds alone, so a captured call replays

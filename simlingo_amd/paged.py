@@ -105,7 +105,10 @@ def prefix_attn(q, out=None, *, own, prefix=None, n_heads, n_q=1, scale=None, ma
     to be lower than the tables' columns (longer ones are cut to them), at most 2^30; the split of the work goes by them.
     Keys on a page number outside the cache are masked. lse: optional f32 [N * n_q, n_heads], natural log of the softmax
     sum (-inf without keys). Returns out (bf16, like q); it may be q itself, or other columns of its rows. out and lse are apart from the
-    caches, tables and lengths."""
+    caches, tables and lengths.
+
+    Scores, softmax, sums and partial outputs are held in f32 (probabilities enter the product with V as two bf16 terms, 2^-15); the
+    output is rounded once."""
     ok, ov, otab, olen = own
     pk, pv, ptab, plen = prefix if prefix is not None else (None, None, None, None)
     return (_native or _bind()).prefix_attn(q, out, ok, ov, otab, olen, pk, pv, ptab, plen, n_heads, n_q, scale, max_own, max_prefix, lse)
