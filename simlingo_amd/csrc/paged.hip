@@ -106,8 +106,8 @@ __global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs a) {
 // product e stands for d = (D/16) r + e). The row sums are one more MFMA, with an A operand of ones.
 //
 // Two forms of a workgroup, by the rows that share the keys:
-//   direct (up to 8 rows of a prefix, 16 of own keys, or 32 of a cache with pages of less than 8 slots): all 4 waves have the same rows; each takes every
-//     fourth 32-key tile straight into registers (K's next tile is requested once the scores have used the last, V's after the
+//   direct (up to 8 rows of a prefix of 64-element heads, 16 of 128 or of own keys, 32 of a cache with pages of less than 8 slots): all 4
+//     waves have the same rows; each takes every fourth 32-key tile straight into registers (K's next tile is requested once the scores have used the last, V's after the
 //     output has), the waves' states are merged through LDS at the end. Few rows: the bytes in flight count, and no wave waits
 //     for another.
 //   streamed: 64 or 128 rows, so the keys are fetched once for all of them: tiles of 32 keys arrive by LDS-DMA in a ring, one
@@ -115,8 +115,8 @@ __global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs a) {
 //     swapped), which keeps both operands' reads of 64 elements free of bank conflicts (of 128: 27 % of the LDS cycles). One
 //     page number for 8 keys (scalar load), so pages of at least 8 slots.
 //
-// Measured (main launch + join; 14 heads on 2 of 64 unless said). 2 x 16 sequences on 32771 shared and 300 .. 1000 own keys: 19.4 +
-// 4.9 us, of which memory needs 8.5 (44 MB at 5.2 TB/s); VALU 28 % and MFMA 10 % of the SIMDs' cycles, the rest is the wait for the
+// Measured (main launch + join; 14 heads on 2 of 64 unless said). 2 x 16 sequences on 32771 shared and 300 .. 1000 own keys: 21.9 +
+// 5.1 us, of which memory needs 8.5 (44 MB at 5.2 TB/s); VALU 28 % and MFMA 10 % of the SIMDs' cycles, the rest is the wait for the
 // first tiles (5 us before and after the steps), the steps of few waves and uneven CUs. 32 on 16411 + 2000 of 32 heads on 8 of 128:
 // 52.8 + 4.9 us, 215 MB = 3.7 TB/s. 8 x 8 on 1086: 7.5 + 3.1 us and 1 x 4 on 798: 5.6 + 2.4 us, where a launch takes 2 and the chain
 // length -> page numbers -> keys -> merge the rest.
@@ -1003,13 +1003,13 @@ __global__ __launch_bounds__(256) void prefix_attn_join_kernel(PAttnArgs a) {
 // for any lengths up to them. As many ranges as give about kTarget workgroups, each of at least 128 keys; or whole rows.
 //
 // Whole rows, a tile of 64 rows of one sequence through the prefix and its own keys, write no parts and need no join, but fetch the
-// prefix for every tile and run alone (1.3 us for 128 keys of 64 elements on an 8-wave workgroup, 2.6 us of 128). Measured against
+// prefix for every tile and run alone (1.5 us for 128 keys of 64 elements on an 8-wave workgroup, 3 us of 128). Measured against
 // parts + join (us; 14 heads on 2 of 64 unless said):
-//   12 sequences of 77 tokens:   640 shared keys 14.4, 26.7 + 5.3;  1800: 33 (4 waves), 32 + 5;  8000: 113 (4 waves), 71 + 6
-//   10 of 60 (140 tiles), 1280:  20.4, 25 + 6       4 of 40 (40 tiles), 640: 13.9, 13.0 + 3.9       1 of 3 (2 tiles), 200: 10.2, 6.9 + 2.3
-//   32 heads on 8 of 128:        8 of 64 (256 tiles), 1280: 33, 41 + 10   4 of 40 (96), 640: 20, 19.5 + 5   4 of 40, 1280: 36, 22 + 7
-// Ranges: 512 / 768 / 1024 / 1536 workgroups for 2 x 16 sequences on 32771 keys 22.6 / 21.5 / 19.9 / 19.6 with joins that grow, for 32
-// on 16411 keys of 8 heads of 128 63 / 53 / 55 / 63.
+//   12 sequences of 77 tokens:   640 shared keys 16.2, 28.3 + 5.3;  1800: 30.8, 36.4 + 5.3;  8000: 100, 83 + 6
+//   10 of 60 (140 tiles), 1280:  22.4, 24.2 + 6.3   4 of 40 (40 tiles), 640: 14.6, 10.8 + 3.9       1 of 3 (2 tiles), 200: 10.4, 6.8 + 2.0
+//   32 heads on 8 of 128:        8 of 64 (256 tiles), 1280: 37, 45 + 9   4 of 40 (96), 640: 19.7, 19.7 + 4.8   4 of 40, 1280: 30.1, 23.2 + 7.5
+// Ranges: 512 / 768 / 1024 / 1536 workgroups for 2 x 16 sequences on 32771 keys 24.4 + 4.9 / 22.0 + 5.1 / 23.3 + 6.2 / 23.4 + 6.2, for 32
+// on 16411 keys of 8 heads of 128 64.8 + 4.7 / 54.8 + 4.9 / 53.8 + 5.3 / 61.0 + 6.9.
 constexpr long kTarget = 768, kCUs = 256;
 struct PAttnPlan { int kp, ko, mtp, mto, nsp, nso, whole; };  // whole: waves of a workgroup, or 0
 // the most units of 128 keys that tiles of whole rows run through
@@ -1018,11 +1018,12 @@ static PAttnPlan plan_attn(const slx_prefix_attn_desc* d, int capp, int capo) {
   PAttnPlan p;
   const int gq = d->Hq / d->own_pool.heads;
   auto kind = [](long rows, const slx_kv_pool& pool, long direct) {
-    // Streamed tiles: one page number for 8 keys, whose offsets on the page fit 32 bits. Direct / streamed prefixes, us: 14 rows on
-    // 798 keys 5.6 / 5.5, on 32771 11.8 / 11.5; 16 rows on 4 x 16411 11.6 / 10.0; 28 rows 7.0 / 5.6 and 13.8 / 12.3; heads of
-    // 128, 12 rows on 16411 18.2 / 19.1, 32 rows 27.0 / 25.6. Own keys, many short sequences of 7 rows beside the prefix:
-    // 19.0 / 22.5 and 7.7 / 8.5. 64 / 128 rows a tile, with the join: 112 rows on 32771 keys 24.6 / 24.7, on 1086
-    // 12.9 / 13.8, heads of 128, 128 rows on 16411 62.4 / 58.3 (the keys pass through L2 once instead of twice).
+    // Streamed tiles: one page number for 8 keys, whose offsets on the page fit 32 bits. Direct / streamed prefixes, us of the main
+    // launch: 7 rows on 798 keys 5.7 / 5.7, on 32771 7.8 / 7.3 (5.2 / 5.3 of them joined); 14 rows 5.8 / 5.8 and 8.4 / 8.2; 28 rows
+    // 7.0 / 6.0 and 11.8 / 9.8. Heads of 128: 12 rows on 16411 17.6 / 18.7, 16 rows on 4 x 16411 60.3 / 59.7, 32 rows on 16411
+    // 23.5 / 20.5. Own keys, many short sequences of 7 rows beside the prefix: 21.8 / 25.2 (2 x 16 on 32771) and 8.5 / 20.8 (8 x 8 on
+    // 1086). 64 / 128 rows a tile: 112 rows on 32771 keys 21.5 / 21.9, on 1086 6.7 / 7.9; heads of 128, 128 rows on 16411 58.8 / 53.8
+    // (the keys pass through L2 once instead of twice).
     const bool streams = pool.page >= 8 && pool.slot_stride < (1 << 27);
     return rows <= (streams ? direct : 16) ? kD16 : !streams ? kD32 : rows <= 64 ? kS64 : kS128;
   };
@@ -1031,10 +1032,10 @@ static PAttnPlan plan_attn(const slx_prefix_attn_desc* d, int capp, int capo) {
   const long up = (capp + 127) / 128, uo = (capo + 127) / 128;  // units of 128 keys
   p.whole = 0;
   p.ko = kind(ro, d->own_pool, 16);
-  p.kp = capp > 0 ? kind(rp, d->prefix_pool, 8) : p.ko;
+  p.kp = capp > 0 ? kind(rp, d->prefix_pool, d->own_pool.head_dim == 64 ? 8 : 16) : p.ko;
   if (capp > 0 && p.kp >= kS64 && p.ko >= kS64 && up + uo <= whole_units(d->own_pool.head_dim, seqs * t64)) {
     p.ko = p.kp = 2 * seqs * t128 >= 3 * kCUs ? kS128 : kS64;
-    p.whole = p.ko == kS64 && seqs * t64 <= kCUs ? 8 : 4;  // one workgroup a CU: 8 waves (17.5 -> 14.9 us above); two of them: 4 (340: 23.4, 29.2)
+    p.whole = p.ko == kS64 && seqs * t64 <= kCUs ? 8 : 4;  // one workgroup a CU: 8 waves (16.2 us above, 4 waves 19.0); two of them: 4 (340 tiles: 24.6, 30.4)
     p.mto = p.mtp = (int)(p.ko == kS128 ? t128 : t64);
     p.nsp = p.nso = 1;
     return p;

@@ -28,6 +28,9 @@ MORE = [  # many ranges, whole rows of 64 and 128, wide tiles
     (32, 32, 128, 1, 9, 40, [77], 16, [40 + i for i in range(9)], 8, "slots"),
     (14, 2, 64, 1, 16, 1, [1500], 128, [5] * 16, 16, "slots"),
     (32, 8, 128, 1, 20, 1, [900], 16, [3] * 20, 16, "slots"),
+    (32, 8, 128, 1, 3, 1, [500], 16, [3, 40, 9], 16, "slots"),       # 12, 16 and 20 rows of a prefix
+    (32, 8, 128, 2, 4, 1, [500, 77], 16, [3] * 8, 8, "heads"),
+    (32, 8, 128, 1, 5, 1, [500], 16, [3] * 5, 16, "pair"),
 ]
 
 
