@@ -167,9 +167,21 @@ bool meet(const Box& a, const Box& b) {
   const int64_t delta = b.p - a.p;
   return s.reaches(1 - b.run - delta, a.run - 1 - delta);
 }
-// Whether two runs of one array share memory: those that differ along axis i first, by x_i > 0
+// Whether two runs of one array share memory: not where each axis steps over all that lies within it; else by the runs that differ
+// along axis i first, by x_i > 0.
 bool folds(const Box& a) {
   if (!a.run) return false;
+  int64_t within = a.run;
+  int left = a.n;
+  for (unsigned done = 0; left; --left) {
+    int least = -1;
+    for (int i = 0; i < a.n; ++i)
+      if (!(done >> i & 1) && (least < 0 || a.st[i] < a.st[least])) least = i;
+    if (a.st[least] < within) break;
+    within += (a.ext[least] - 1) * a.st[least];
+    done |= 1u << least;
+  }
+  if (!left) return false;
   for (int i = 0; i < a.n; ++i) {
     Sum s;
     s.add(a.st[i], 1, a.ext[i] - 1);
@@ -520,10 +532,11 @@ PyObject* beam_reorder(PyObject*, PyObject* const* a, Py_ssize_t n) {
       const auto box = [&](const Tensor& u, const int64_t* st) {
         return Box(u.data_ptr(), run * es).axis(m[1], st[1] * es).axis(m[0], st[0] * es).axis(b * w, u.stride(dim) * es);
       };
+      const Box to = box(out, t);
       const bool same = x.data_ptr() == out.data_ptr() && s[0] == t[0] && s[1] == t[1] && (x.stride(dim) == out.stride(dim) || b * w == 1);
-      NEED(same || !meet(box(x, s), box(out, t)), "out overlaps x");
-      NEED(!folds(box(out, t)), "rows of out overlap each other");
-      NEED(!meet(box(out, t), box_of(parent)), "out overlaps parent");
+      NEED(same || !meet(box(x, s), to), "out overlaps x");
+      NEED(!folds(to), "rows of out overlap each other");
+      NEED(!meet(to, box_of(parent)), "out overlaps parent");
     }
     const slx_stream_t st = stream_of(who, {&x, &out, &parent});
     if (x.numel()) {
