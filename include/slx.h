@@ -550,7 +550,8 @@ typedef struct slx_prefix_attn_desc {
   float* ws; int64_t ws_floats;              /* slx_prefix_attn_ws_floats(d); one call at a time                       */
 } slx_prefix_attn_desc;
 /* token t of a sequence's n_q attends the plen[group] keys of its group's prefix and its own keys j <= olen - n_q + t; a
- * row without any key gives zeros. out and lse overlap nothing that is read (but out q itself, or other columns of its rows). */
+ * row without any key, or with scores of -inf alone, gives zeros. out and lse overlap nothing that is read (but out q itself,
+ * or other columns of its rows).                                                                                     */
 int slx_prefix_attn(const slx_prefix_attn_desc* d, slx_stream_t s);
 int64_t slx_prefix_attn_ws_floats(const slx_prefix_attn_desc* d); /* < 0: bad argument                                 */
 

@@ -446,7 +446,9 @@ __global__ __launch_bounds__(1024) void beam_pick_kernel(SelArgs a) {
 // A thread takes one column of all `width` rows of a batch entry: every row is loaded before any is stored, so the
 // state may be reordered in place, whatever the parents; in place, rows that stay are neither read nor written. Memory bound where
 // it is large: 24 x 4 x 8 rows of bf16, the first 16256 of 32768 elements used, in place with half of the rows staying: 6.0 us for 25 MB
-// read and written; a table of 8 x 8 rows of 101 numbers 3.5 us, of which a launch takes 2 and the chain parent -> row the rest.
+// read and written; a table of 8 x 8 rows of 101 numbers 3.6 us, of which a launch takes 2 and the chain parent -> row the rest. Wide
+// states pay for a row's parent and address in scalars, which spill from 9 rows on: 2 x 8 / 16 / 32 / 64 rows of 101 numbers
+// 2.8 / 4.6 / 9.0 / 17.6 us, 6 x 2 x 8 / 16 / 32 / 64 rows of 32 KB 4.2 / 6.4 / 11.4 / 21.3 (6 .. 50 MB, 4.7 TB/s at the widest).
 struct ReorderArgs {
   const char* src; char* dst;
   long s0, s1, sr, d0, d1, dr;  // byte strides: two outer axes and the rows, of source and destination

@@ -103,23 +103,26 @@ __global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs a) {
 // lane holds 8 keys of ONE query, and the probabilities are already the B operand of O^T += V^T P^T (the sum over keys
 // may take them in any order: slot j of lane group g is key 4g + j, or 16 + 4g + j - 4). V^T's A operand needs 8 keys
 // of one d: a lane takes D/16 neighbouring d of each of its 8 keys and pairs them with v_perm_b32 (the MFMA row r of
-// product e stands for d = (D/16) r + e). The row sums are one more MFMA, with an A operand of ones.
+// product e stands for d = (D/16) r + e). The row sums are one more MFMA, with an A operand of ones; a
+// probability is two bf16 terms (softmax_step), so each product with P is two.
 //
 // Two forms of a workgroup, by the rows that share the keys:
 //   direct (up to 8 rows of a prefix of 64-element heads, 16 of 128 or of own keys, 32 of a cache with pages of less than 8 slots): all 4
-//     waves have the same rows; each takes every fourth 32-key tile straight into registers (K's next tile is requested once the scores have used the last, V's after the
-//     output has), the waves' states are merged through LDS at the end. Few rows: the bytes in flight count, and no wave waits
-//     for another.
+//     waves have the same rows; each takes every fourth 32-key tile straight into registers (K's next tile is requested once the
+//     scores have used the last, V's after the output has), the waves' states are merged through LDS at the end. Few rows: the bytes
+//     in flight count, and no wave waits for another. Many rows on such small pages cost twice the streamed form's time: 12 x 77
+//     tokens on 640 keys 33 + 5 us on pages of 4 or 1, 15.6 on pages of 64.
 //   streamed: 64 or 128 rows, so the keys are fetched once for all of them: tiles of 32 keys arrive by LDS-DMA in a ring, one
 //     barrier a step. Rows of K and V lie in LDS with their 16-B chunks XOR-ed by the slot (and slots with bits 0 and 2
-//     swapped), which keeps both operands' reads of 64 elements free of bank conflicts (of 128: 27 % of the LDS cycles). One
-//     page number for 8 keys (scalar load), so pages of at least 8 slots.
+//     swapped), which keeps both operands' reads of 64 elements free of bank conflicts (of 128: 27 % of the LDS's cycles).
+//     One page number for 8 keys (scalar load), so pages of at least 8 slots.
 //
 // Measured (main launch + join; 14 heads on 2 of 64 unless said). 2 x 16 sequences on 32771 shared and 300 .. 1000 own keys: 21.9 +
-// 5.1 us, of which memory needs 8.5 (44 MB at 5.2 TB/s); VALU 28 % and MFMA 10 % of the SIMDs' cycles, the rest is the wait for the
-// first tiles (5 us before and after the steps), the steps of few waves and uneven CUs. 32 on 16411 + 2000 of 32 heads on 8 of 128:
-// 52.8 + 4.9 us, 215 MB = 3.7 TB/s. 8 x 8 on 1086: 7.5 + 3.1 us and 1 x 4 on 798: 5.6 + 2.4 us, where a launch takes 2 and the chain
-// length -> page numbers -> keys -> merge the rest.
+// 5.1 us, of which memory needs 8.5 (44 MB at 5.2 TB/s); VALU 26 % and MFMA 14 % of the SIMDs' cycles, the rest is the wait for the
+// first tiles (5 us before and after the steps), the steps of few waves and uneven CUs (65 % of the CUs' cycles have a wave). 32 on 16411
+// + 2000 of 32 heads on 8 of 128: 53.8 + 5.0 us, 215 MB = 3.7 TB/s. 8 x 8 on 1086: 7.6 + 3.1 us and 1 x 4 on 798: 5.9 + 2.5 us, where a
+// launch takes 2 and the chain length -> page numbers -> keys -> merge the rest. Without a prefix, the whole call: one sequence of 839
+// keys 8.1 us; 32 of 300 .. 1800 12.0, with 32 heads on 8 of 128 39.5 (137 MB, 3.5 TB/s); 16 of 8000 .. 16000 of those 177 (976 MB, 5.5 TB/s).
 struct Seg {
   PoolView p;
   const int* tab; long ldt;
@@ -605,8 +608,8 @@ __device__ __forceinline__ void dma16(const void* base, unsigned off, unsigned l
 
 // A streamed workgroup: NW waves, RV of them side by side over RW rows, and as many teams as that leaves, each of which takes tiles
 // of its own of every step of the ring, T tiles of 32 keys; the teams are joined at the end. With two teams of 64 rows of 64 elements
-// an operand read from LDS serves 32 rows of a wave instead of 16: 23.2 us instead of 24.4 for 340 whole-row tiles; a range of
-// 128 keys is over before that pays for the join of the teams: 6.5 us instead of 5.6 for 4 sequences on 798 keys.
+// an operand read from LDS serves 32 rows of a wave instead of 16: 24.4 us instead of 25.0 for 340 whole-row tiles; a range of
+// 128 keys is over before that pays for the join of the teams: 6.7 us instead of 6.0 for 4 sequences on 798 keys.
 template <int D, int RW, int NW, int RV>
 struct Shape {
   static constexpr int RWV = RV, NQ = RW / 16 / RWV, TEAMS = NW / RWV;

@@ -11,7 +11,8 @@ instructions about one frame and the beams of one answer share the image prompt,
 A cache is a pair of bf16 tensors k, v [pages, page, kv heads, head size], any strides with the last dimension
 contiguous (page a power of two, head size 64 or 128); a table [sequences, columns] int32 names the pages of each
 sequence in order. Everything runs on the current stream of the current device and can be captured in a graph; lengths,
-positions and tables are read on the device, so a captured call follows their contents.
+positions and tables are read on the device, so a captured call follows their contents. These are operators for serving: they have no
+gradients, and what they return is detached.
 """
 from __future__ import annotations
 
@@ -99,9 +100,10 @@ def kv_append(qkv, k, v, table, pos, q_out=None, *, n_heads, cos=None, sin=None,
 def prefix_attn(q, out=None, *, own, prefix=None, n_heads, n_q=1, scale=None, max_own=None, max_prefix=None, lse=None):
     """Attention of n_q new tokens per sequence. own = (k, v, table [N, columns], lengths [N]): each sequence's keys, its new
     tokens' among them as the last; prefix = (k, v, table [G, columns], lengths [G]): keys that sequences g * N/G ...
-    share, before their own. q rows [N * n_q, n_heads * head size], a sequence's tokens together, already rotated; the
-    kv heads are the caches'. Token t sees the whole prefix and own keys up to length - n_q + t; a row without any key
-    gives zeros. scale > 0: 1 / sqrt(head size) by default. max_own, max_prefix: bounds of the lengths where they are known
+    share, before their own (groups of one size: a smaller one is filled up with sequences of length 0, which cost what the others
+    do). q rows [N * n_q, n_heads * head size], a sequence's tokens together, already rotated; the
+    kv heads are the caches'. Token t sees the whole prefix and own keys up to length - n_q + t; a row without any key,
+    or with scores of -inf alone, gives zeros. scale > 0: 1 / sqrt(head size) by default. max_own, max_prefix: bounds of the lengths where they are known
     to be lower than the tables' columns (longer ones are cut to them), at most 2^30; the split of the work goes by them.
     Keys on a page number outside the cache are masked. lse: optional f32 [N * n_q, n_heads], natural log of the softmax
     sum (-inf without keys). Returns out (bf16, like q); it may be q itself, or other columns of its rows. out and lse are apart from the

@@ -63,3 +63,32 @@ def test_values_that_are_not_finite_reach_their_rows(dev, form, bad_page):
         if not same.all():
             wrong += [(X, i) for i in (~same).flatten(1).any(1).nonzero().view(-1).tolist()]
     assert not wrong, (len(wrong), wrong[:20])
+
+
+@pytest.mark.parametrize("form", FORMS)
+def test_scores_of_minus_infinity_alone_count_as_none(dev, form):
+    """A sequence whose keys all score -inf gives zeros and a log sum of -inf, like one without keys; its neighbours are not touched."""
+    hq, hkv, d, n_q, plen, page = FORMS[form]
+    g = torch.Generator(device=dev).manual_seed(4)
+    n, length = 5, 40 + n_q
+    cols = -(-length // page)
+    k, v = (torch.randn(n * cols, page, hkv, d, generator=g, device=dev).to(BF16) for _ in range(2))
+    table = torch.arange(n * cols, dtype=I32, device=dev).view(n, cols)
+    lens = torch.full((n,), length, dtype=I32, device=dev)
+    q = torch.rand(n * n_q, hq * d, generator=g, device=dev).add_(0.1).to(BF16)
+    prefix = None
+    if plen:  # the second sequence's group alone has a prefix of -inf
+        pages = -(-plen // 16)
+        pk, pv = (torch.randn(2 * pages, 16, hkv, d, generator=g, device=dev).to(BF16) for _ in range(2))
+        prefix = (pk, pv, torch.stack([torch.arange(pages, device=dev) + i * pages for i in (0, 1, 0, 0, 0)]).to(I32),
+                  torch.full((n,), plen, dtype=I32, device=dev))
+    call = lambda lse: PG.prefix_attn(q, own=(k, v, table, lens), prefix=prefix, n_heads=hq, n_q=n_q, lse=lse).view(n, n_q, hq * d)  # noqa: E731
+    lse = [torch.full((n * n_q, hq), 3.0, device=dev) for _ in range(2)]
+    before = call(lse[0])
+    k[table[1].long()] = -INF
+    if plen:
+        pk[pages:] = -INF
+    after = call(lse[1])
+    assert not after[1].any() and (lse[1].view(n, -1)[1] == -INF).all()
+    rest = [0, 2, 3, 4]
+    assert torch.equal(after[rest], before[rest]) and torch.equal(lse[0].view(n, -1)[rest], lse[1].view(n, -1)[rest])
