@@ -130,7 +130,8 @@ Box box_of(const Tensor& t) {  // contiguous, or rows of a table
 }
 
 // Whether sum x_i s_i falls into [lo, hi] for whole x_i in [from_i, to_i], the largest s first: the x of an axis are those that leave
-// what the axes after it can reach, one or two where an axis is longer than all after it together. Arrays that take more than a few
+// what the axes after it can reach, one or two where an axis is longer than all after it together. An axis that another one's steps fill
+// without a gap (pages of whole slots, slots that are another array's rows) is joined to it first. Arrays that take more than a few
 // thousand trials are taken to meet.
 struct Sum {
   int n = 0, tries = 4096;
@@ -150,7 +151,21 @@ struct Sum {
       if (--tries < 0 || reaches(i + 1, lo - x * s[i], hi - x * s[i])) return true;
     return false;
   }
+  void join() {
+    for (int j = 1; j < n; ++j)
+      for (int i = j - 1; i >= 0; --i) {
+        const int64_t q = s[i] / s[j];
+        if (s[i] % s[j] || to[j] - from[j] + 1 < q) continue;
+        from[j] += q * from[i];
+        to[j] += q * to[i];
+        --n;
+        for (int m = i; m < n; ++m) { s[m] = s[m + 1]; from[m] = from[m + 1]; to[m] = to[m + 1]; }
+        j = 0;  // from the start: a longer axis may be filled now
+        break;
+      }
+  }
   bool reaches(int64_t lo, int64_t hi) {
+    join();
     least[n] = most[n] = 0;
     for (int i = n - 1; i >= 0; --i) {
       least[i] = least[i + 1] + from[i] * s[i];

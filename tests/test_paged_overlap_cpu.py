@@ -188,3 +188,17 @@ def test_lazily_negated_views():
         taken(lambda: PG.beam_reorder(x, parent), True, "")
         taken(lambda: PG.beam_reorder(x, parent, out=torch.empty(4, 9, dtype=x.dtype)), False, "negated")
     taken(lambda: PG.beam_reorder(z.conj(), parent, out=torch.empty(4, 9, dtype=z.dtype).conj()), True, "")
+
+
+def test_long_buffers_are_told_apart():
+    """Many rows of a fused buffer whose other columns are the cache: the search stays short, whatever the number of rows and pages."""
+    S, hkv, d = 1 << 17, 1, 64
+    b = torch.empty(S, 3 * hkv * d, dtype=BF16)  # not touched
+    table, lens = torch.zeros(S, 1, dtype=I32), torch.zeros(S, dtype=I32)
+    for page in (1, 16, 4096):
+        k, v = (b.as_strided((S // page, page, hkv, d), (page * b.stride(0), b.stride(0), d, 1), at) for at in (d, 2 * d))
+        call = lambda out: PG.prefix_attn(b[:, :d], out, own=(k, v, table, lens), n_heads=1)  # noqa: E731
+        taken(lambda: call(b[:, :d]), True, "")
+        taken(lambda: call(b[:, 8:72]), False, "overlaps")
+        taken(lambda: call(b[:, d:2 * d]), False, "overlaps a cache")
+        taken(lambda: PG.kv_append(torch.zeros(S, 192, dtype=BF16), k, v, table, lens, b[:, :d], n_heads=1), True, "")
