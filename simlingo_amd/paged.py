@@ -100,17 +100,17 @@ def kv_append(qkv, k, v, table, pos, q_out=None, *, n_heads, cos=None, sin=None,
 def prefix_attn(q, out=None, *, own, prefix=None, n_heads, n_q=1, scale=None, max_own=None, max_prefix=None, lse=None):
     """Attention of n_q new tokens per sequence. own = (k, v, table [N, columns], lengths [N]): each sequence's keys, its new
     tokens' among them as the last; prefix = (k, v, table [G, columns], lengths [G]): keys that sequences g * N/G ...
-    share, before their own (groups of one size: a smaller one is filled up with sequences of length 0, which cost what the others
-    do). q rows [N * n_q, n_heads * head size], a sequence's tokens together, already rotated; the
-    kv heads are the caches'. Token t sees the whole prefix and own keys up to length - n_q + t; a row without any key,
-    or with scores of -inf alone, gives zeros. scale > 0: 1 / sqrt(head size) by default. max_own, max_prefix: bounds of the lengths where they are known
-    to be lower than the tables' columns (longer ones are cut to them), at most 2^30; the split of the work goes by them.
-    Keys on a page number outside the cache are masked. lse: optional f32 [N * n_q, n_heads], natural log of the softmax
-    sum (-inf without keys). Returns out (bf16, like q); it may be q itself, or other columns of its rows. out and lse are apart from the
-    caches, tables and lengths.
+    share, before their own (groups of one size: a smaller one is filled up with sequences of length 0, which cost what the
+    others do). q rows [N * n_q, n_heads * head size], a sequence's tokens together, already rotated; the kv heads are the
+    caches'. Token t sees the whole prefix and own keys up to length - n_q + t; a row without any key, or with scores of -inf
+    alone, gives zeros. scale > 0: 1 / sqrt(head size) by default. max_own, max_prefix: bounds of the lengths where they are
+    known to be lower than the tables' columns (longer ones are cut to them), at most 2^30; the split of the work goes by
+    them. Keys on a page number outside the cache are masked. lse: optional f32 [N * n_q, n_heads], natural log of the softmax
+    sum (-inf without keys). Returns out (bf16, like q); it may be q itself, or other columns of its rows. out and lse are
+    apart from the caches, tables and lengths.
 
-    Scores, softmax, sums and partial outputs are held in f32 (probabilities enter the product with V as two bf16 terms, 2^-15); the
-    output is rounded once."""
+    Scores, softmax, sums and partial outputs are held in f32 (probabilities enter the product with V as two bf16 terms,
+    2^-15); the output is rounded once."""
     ok, ov, otab, olen = own
     pk, pv, ptab, plen = prefix if prefix is not None else (None, None, None, None)
     return (_native or _bind()).prefix_attn(q, out, ok, ov, otab, olen, pk, pv, ptab, plen, n_heads, n_q, scale, max_own, max_prefix, lse)
